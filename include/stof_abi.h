@@ -416,6 +416,48 @@ int stof_gemm_bias_res_ln_cluster_dt(const void* A, const void* Wt, const void* 
                                      float eps, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
 /*
+ * Attention with score rules (no counterpart in the reference, whose kernels take 0/1 masks only).
+ * Query i of sample b stands at position p_i = q_start + i, or kv_len[b] - Sq + i with q_end; query
+ * head h reads key head h / (Hq / Hkv).  head size D 64 or 128, any Sq >= 1 and Sk >= 0:
+ *   t_ij = scale * q_i.k_j;  with cap > 0  t_ij = cap * tanh(t_ij / cap)
+ *   s_ij = t_ij + table[h][clip(j - p_i, -radius, radius) + radius]     (table [Hq, 2 radius + 1], the tensors' format)
+ *       or t_ij - slopes[h] * |p_i - j|                                 (slopes [Hq], fp32; not both)
+ *   allowed(i, j): j < kv_len[b], and with causal j <= p_i or j < prefix[b], and with documents
+ *                  docs_q[b][i] == docs_k[b][j] >= 0
+ *   out_i = softmax over the allowed j, times v;  lse_i = log of the softmax's denominator
+ * A row without allowed keys gives zeros and lse = -inf.  prefix, kv_len (clamped to [0, Sk]), docs_*:
+ * int32, each may be NULL; they are read by the launch, not before.  Keys at or past kv_len and keys of a
+ * negative document are not used as values, whatever they hold (NaN included).
+ * Strides: (batch, head, row) in elements, multiples of 8, rows at most 2^23; pointers 16-byte aligned.
+ * lse [B, Hq, Sq] fp32 may be NULL.  form: -1 the library's choice, 0 128-query tiles, 1 32-row tiles with
+ * the keys split over waves and workgroups.  The workspace (bytes below, 0 = none) needs no initial
+ * contents and belongs to this call until its work is done.
+ */
+#define STOF_SCORE_MAX_RADIUS 1024
+int64_t stof_score_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int docs, int form);
+int stof_score_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                        const void* table, const float* slopes, const int32_t* prefix, const int32_t* kv_len,
+                        const int32_t* docs_q, const int32_t* docs_k,
+                        float scale, float cap, int radius, int causal, int q_start, int q_end,
+                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
+                        int B, int Hq, int Hkv, int Sq, int Sk, int D, int dtype, int form,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Its gradients, from the forward pass's out and lse: dq [B, Hq, Sq, D], dk and dv [B, Hkv, Sk, D] contiguous, dtable
+ * [Hq, 2 radius + 1] in the tensors' format.  No atomics: the same inputs give the same bits.  The rule's tensors must hold what they held in the forward pass.
+ */
+int64_t stof_score_attn_bwd_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int docs);
+int stof_score_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                        void* dq, void* dk, void* dv, void* dtable,
+                        const void* table, const float* slopes, const int32_t* prefix, const int32_t* kv_len,
+                        const int32_t* docs_q, const int32_t* docs_k,
+                        float scale, float cap, int radius, int causal, int q_start, int q_end,
+                        const int64_t* dout_strides, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                        const int64_t* out_strides, int B, int Hq, int Hkv, int Sq, int Sk, int D, int dtype,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Measurement probes (no counterpart in the reference; used by bench.py, not by any operator).
  * stof_device_compute_units: compute units of the current device (hipDeviceAttributeMultiprocessorCount),
  * or a negative status.  stof_probe_clock: one wavefront spins for `iters` x 16 dependent adds between

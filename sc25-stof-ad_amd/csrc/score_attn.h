@@ -1,0 +1,222 @@
+// Shared pieces of the attention kernels with score rules (score_attn_gfx950.hip: forward,
+// score_attn_bwd_gfx950.hip: backward).
+//
+// Query i of a sample stands at position p_i = first + i, query head h reads key head
+// h / (Hq / Hkv).  With c = scale * log2(e) the kernels work on scores in units of log2:
+//     t_ij = c q_i.k_j                                        without a cap
+//     t_ij = cap' (1 - 2 / (1 + exp2(2 c q_i.k_j / cap')))     cap' = cap * log2(e): cap tanh(scale q.k / cap)
+//     t_ij += table[h][clip(j - p_i, -R, R) + R] * log2(e)     or   t_ij -= slope_h * log2(e) * |p_i - j|
+// over the allowed keys j < limit_i (and of the query's document), where limit_i = kv_len, or
+// min(kv_len, max(p_i + 1, prefix)) for a causal rule: every mask but the documents is one
+// per-row limit.  A row without allowed keys yields zeros, lse = -inf and no gradients.
+#pragma once
+#include "stof_common.h"
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef float floatx2_t __attribute__((ext_vector_type(2)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef short short8_t __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) short4_t lds_short4;
+
+enum { kBiasNone = 0, kBiasTable = 1, kBiasSlopes = 2 };
+
+constexpr int kBlock = 64;          // keys per tile, and rows per block of the document ranges
+constexpr int kTabPad = 32;         // entries by which the table in LDS continues its two ends
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// Finite table entries are held inside +-kTabMax (log2 units): the lowest value of the bfloat16
+// format times log2(e) would otherwise become -inf, that is a masked key instead of a very small one.
+constexpr float kTabMax = 1.0e38f;
+
+// Smallest and largest document of a block of 64 positions over its valid (non-negative) ids, and
+// whether all its ids are valid.  No valid id: lo > hi, which no range intersects.
+struct DocRange { int lo, hi, all, pad; };
+// Whether two blocks can hold a pair of one document, and whether all their pairs are of one document.
+__device__ __forceinline__ bool ranges_meet(const DocRange& a, const DocRange& b) {
+  return a.lo <= b.hi && b.lo <= a.hi && a.lo <= a.hi && b.lo <= b.hi;
+}
+__device__ __forceinline__ bool ranges_one(const DocRange& a, const DocRange& b) {
+  return a.all && b.all && a.lo == a.hi && b.lo == b.hi && a.lo == b.lo;
+}
+
+struct ScoreParams {
+  const half_t* q; const half_t* k; const half_t* v; half_t* out; float* lse;
+  int64_t qs[3], ks[3], vs[3], os[3];      // element strides (batch, head, row)
+  const half_t* table; const float* slopes;
+  const int* prefix; const int* kv_len;    // per sample, or NULL
+  const int* docs_q; const int* docs_k;    // [B, Sq], [B, Sk], or NULL
+  const DocRange* dr_q; const DocRange* dr_k;   // [B, ceil(Sq / 64)], [B, ceil(Sk / 64)]
+  int B, Hq, Hkv, Sq, Sk;
+  int radius, bias_kind, causal;
+  int q_start, q_end;                      // p_0 = q_start, or kv_len - Sq with q_end
+  int tiles, chunk;                        // workgroups per (batch, head); workgroups per XCD
+  float c, k1, capl;                       // scale log2e; 2 scale log2e / cap (0: no cap); cap log2e
+  float cc;                                // what turns a rule's result into log2 units: c when it is the raw product, else 1
+  // form for few rows
+  int splits, group; float* part;
+};
+
+// Per-sample scalars: number of keys and position of query 0.
+__device__ __forceinline__ int sample_keys(const ScoreParams& p, int b) {
+  int n = p.Sk;
+  if (p.kv_len) n = min(max(__builtin_amdgcn_readfirstlane(p.kv_len[b]), 0), p.Sk);
+  return n;
+}
+__device__ __forceinline__ int sample_first(const ScoreParams& p, int klen) { return p.q_end ? klen - p.Sq : p.q_start; }
+__device__ __forceinline__ int sample_prefix(const ScoreParams& p, int b) {
+  return p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[b]) : 0;
+}
+// Keys j < row_limit are allowed for a query at position `pos` (documents aside).
+__device__ __forceinline__ int row_limit(int causal, int klen, int prefix, int pos) {
+  return causal ? min(klen, max(pos + 1, prefix)) : klen;
+}
+
+__device__ __forceinline__ float pair_max(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+
+// LDS tile: unpadded rows of D elements, the 16-byte chunk c of row r at chunk position c ^ swz(r).
+// 128-byte rows: row bits 1, 2, 3 onto chunk bits 2, 0, 1 (two rows fill the 64 banks); 256-byte rows:
+// row bits 0, 1 onto chunk bits 2, 3 and row bits 2, 3 onto chunk bits 0, 1.  The 16 rows of a fragment
+// read then take 16 different chunks, the four rows of a transposing read four different 64-byte groups.
+template <int D> __device__ __forceinline__ int swz(int row) {
+  if constexpr (D == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else return ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+// Byte offsets inside a tile of the two fragment reads of lane (j32, g):
+//  * rows as the A operand (v_mfma_f32_32x32x16: row j32, 8 elements from 16 ks + 8 g): frag_off + 32 rows * pitch;
+//  * columns as the A operand through the transposing read: element row 8 hh + 4 g + (0..3), column 32 dt + j32.
+template <int D> __device__ __forceinline__ int frag_off(int j32, int g, int ks) {
+  return j32 * (2 * D) + (((2 * ks + g) ^ swz<D>(j32)) << 4);
+}
+template <int D> __device__ __forceinline__ int tr_off(int lane, int dt, int hh) {
+  const int g = lane >> 5, j = lane & 15, dh = (lane >> 4) & 1;
+  const int row = 8 * hh + 4 * g + (j >> 2);
+  const int chunk = 4 * dt + 2 * dh + ((j >> 1) & 1);
+  return row * (2 * D) + ((chunk ^ swz<D>(row)) << 4) + 8 * (j & 1);
+}
+__device__ __forceinline__ half8_t lds_frag(const lds_byte* p) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) half8_t*>(p);
+}
+__device__ __forceinline__ half8_t lds_frag_tr(const lds_byte* p0, const lds_byte* p1) {
+  const short4_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p0);
+  const short4_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p1);
+  return __builtin_bit_cast(half8_t, (short8_t)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// ROWS rows of a [rows, D] operand as a buffer resource: base in scalar registers, extent up to the last
+// valid row, so rows past it arrive as zeros whatever memory holds there.
+template <int D>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const half_t* base, int64_t stride, int64_t first, int valid) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base + first * stride);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  const int bytes = valid > 0 ? ((valid - 1) * (int)stride + D) * 2 : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
+// Direct-to-LDS load of a tile of ROWS rows by WAVES waves: one instruction brings 1 KB (1024 / (2 D) rows).
+template <int D, int ROWS, int WAVES> struct TileLoad {
+  static constexpr int kPitch = 2 * D;
+  static constexpr int kRowsPI = 1024 / kPitch;
+  static constexpr int kChunks = kPitch / 16;
+  static constexpr int kN = ROWS / kRowsPI / WAVES;     // instructions per wave
+  static constexpr int kBytes = ROWS * kPitch;
+  static __device__ __forceinline__ int row(int wave, int lane, int i) { return kRowsPI * (kN * wave + i) + lane / kChunks; }
+  static __device__ __forceinline__ void offsets(uint32_t (&off)[kN], int wave, int lane, int64_t stride) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int r = row(wave, lane, i);
+      off[i] = (uint32_t)r * (uint32_t)(stride * 2) + 16 * ((lane % kChunks) ^ swz<D>(r));
+    }
+  }
+  static __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t rs, const uint32_t (&off)[kN], int wave, lds_byte* dst) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(dst + (kN * wave + i) * 1024), 16, off[i], 0, 0, 0);
+  }
+  // Zeros over the rows of this wave's share whose bit in `rows` is clear (the lane overwrites the chunk it
+  // loaded itself, so the caller's barrier after the load also covers this).
+  static __device__ __forceinline__ void keep(uint64_t rows, int wave, int lane, lds_byte* dst) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (!((rows >> row(wave, lane, i)) & 1)) {
+        const half8_t z = {};
+        *reinterpret_cast<__attribute__((address_space(3))) half8_t*>(dst + (kN * wave + i) * 1024 + 16 * lane) = z;
+      }
+  }
+};
+
+// A head's distance table in LDS: entry x + kTabPad + R holds table[clip(x)] * log2(e), x from -R - kTabPad to R + kTabPad.
+template <bool BF>
+__device__ __forceinline__ void load_table(const ScoreParams& p, int head, float* tab, int tid, int threads) {
+  const int n = 2 * p.radius + 1;
+  for (int x = tid; x < n + 2 * kTabPad; x += threads) {
+    const float e = from_elem<BF>(p.table[(int64_t)head * n + min(max(x - kTabPad, 0), n - 1)]);
+    const float s = e * kLog2e;
+    tab[x] = (e == -INFINITY || e == INFINITY) ? s : fminf(fmaxf(s, -kTabMax), kTabMax);   // (NaN: fminf / fmaxf would drop it)
+    if (e != e) tab[x] = e;
+  }
+}
+
+// What one lane knows of its query.
+struct LaneRow { int pos, limit, doc; float slope; const float* tab; };
+
+// The rule on 16 scores of the lane's query: s[r] belongs to key jb + 4 g + 8 (r / 4) + r % 4.  Raw products
+// in, what p.cc turns into log2 units out.
+__device__ __forceinline__ int key_off(int r) { return 8 * (r >> 2) + (r & 3); }
+
+__device__ __forceinline__ void cap_scores(const ScoreParams& p, floatx16& s) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float u = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * p.k1));
+    s[r] = __builtin_fmaf(u, -2.f * p.capl, p.capl);
+  }
+}
+__device__ __forceinline__ void bias_scores(const ScoreParams& p, const LaneRow& L, int j0 /* jb + 4 g */, floatx16& s) {
+  const float mul = p.k1 != 0.f ? 1.f : p.c;
+  if (p.bias_kind == kBiasTable) {
+    const int x = min(max(j0 - L.pos, -p.radius - kTabPad), p.radius);
+    const float* t = L.tab + (x + p.radius + kTabPad);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, t[key_off(r)]);
+  } else if (p.bias_kind == kBiasSlopes) {
+    const float x = (float)(j0 - L.pos);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, -L.slope * __builtin_fabsf(x + (float)key_off(r)));
+  }
+}
+__device__ __forceinline__ void limit_scores(const LaneRow& L, int j0, floatx16& s) {
+  const int rel = L.limit - j0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = key_off(r) < rel ? s[r] : -INFINITY;
+}
+// ids: the documents of the tile's keys in LDS, from key jb + 4 g on
+__device__ __forceinline__ void doc_scores(const LaneRow& L, const int* ids, floatx16& s) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = ids[key_off(r)] == L.doc ? s[r] : -INFINITY;
+}
+
+// Document of position i of a sequence of n: -1 for none (queries), -2 for none (keys), so that they never match.
+__device__ __forceinline__ int doc_at(const int* docs, int64_t i, bool inside, int none) {
+  const int d = inside ? docs[i] : none;
+  return d < 0 ? none : d;
+}
+
+// Host helpers shared by the forward and backward entry points (score_attn_gfx950.hip).
+#pragma GCC visibility push(hidden)
+int score_attn_check(const void* const* req, int n_req, const int64_t* const* strides, int n_strides, int B, int Hq, int Hkv, int Sq, int Sk, int D,
+                     int dtype, float scale, float cap, int radius);
+void score_attn_params(ScoreParams& p, const void* q, const void* k, const void* v, const void* table, const void* slopes, const void* prefix,
+                       const void* kv_len, const void* docs_q, const void* docs_k, float scale, float cap, int radius, int causal, int q_start,
+                       int q_end, const int64_t* qs, const int64_t* ks, const int64_t* vs, int B, int Hq, int Hkv, int Sq, int Sk);
+void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st);
+#pragma GCC visibility pop

@@ -1,0 +1,692 @@
+// Attention with score rules, forward: stof_score_attn_fwd (see score_attn.h for the rule).
+//
+// Two forms, the same wave program: a wave keeps 32 query rows in registers, scores are produced
+// transposed (S^T = K Q^T, v_mfma_f32_32x32x16), so a lane owns ONE query: its position, limit,
+// document, running maximum and sum are per-lane scalars and the rule is a register loop; P never
+// touches LDS (the accumulator layout of S^T is the B operand layout of O^T = V^T P^T) and V is
+// transposed by the LDS read.
+//
+//  * wide form: four waves x 32 queries of one head share K and V tiles of 64 keys, direct-to-LDS
+//    loads double buffered, one barrier per tile.  Which tiles a workgroup visits and which of them
+//    need the element test is decided for 64 tiles at a time, one tile per lane: limits and document
+//    ranges become three 64-bit sets that the walk takes bit by bit.
+//  * row form, for few rows and long keys (single tokens) and for small grids: one workgroup owns 32
+//    rows, row r = (query r / G, head r % G of the G heads that share a key head), so a token's heads
+//    read the cache once; its four waves take every fourth tile of 32 keys through buffers of their own
+//    without barriers, and the keys can be split further over workgroups, joined by a second kernel.
+#include "score_attn.h"
+
+namespace {
+
+constexpr float kLazy = 8.0f;       // log2 slack before the running maximum is raised
+
+// Document ranges of the 64-position blocks of both sequences: one wave per block.
+__global__ __launch_bounds__(64) void doc_ranges_kernel(const int* docs_q, const int* docs_k, DocRange* dr_q, DocRange* dr_k,
+                                                        int B, int Sq, int Sk) {
+  const int nq = (Sq + kBlock - 1) / kBlock, nk = (Sk + kBlock - 1) / kBlock;
+  const bool is_q = (int)blockIdx.x < B * nq;
+  const int idx = is_q ? blockIdx.x : blockIdx.x - B * nq;
+  const int n = is_q ? nq : nk, S = is_q ? Sq : Sk;
+  const int b = idx / n, blk = idx - b * n, i = blk * kBlock + threadIdx.x;
+  const bool inside = i < S;
+  const int d = inside ? (is_q ? docs_q : docs_k)[(int64_t)b * S + i] : -1;
+  int lo = d >= 0 ? d : 0x7fffffff, hi = d >= 0 ? d : -1;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64)); }
+  const int all = !__any(inside && d < 0);
+  if (threadIdx.x == 0) (is_q ? dr_q : dr_k)[idx] = DocRange{lo, hi, all, 0};
+}
+
+// Online softmax of one wave over 16 MT scores per lane: raises the running maximum (rescaling O when it
+// moves by more than kLazy), turns scores into probabilities in the tensors' format (the B operand of the
+// second product) and adds to the running sum.  The sum is taken in fp32 from the unrounded
+// probabilities; their rounding to 16 bits is the only one between the scores and the output.
+template <int D, int MT, bool BF>
+struct Softmax {
+  floatx16 o[D / 32];
+  float m = -INFINITY, mc = 0.f, raise_at = -INFINITY, l = 0.f;
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  }
+  __device__ __forceinline__ void step(float cc, const floatx16 (&s)[MT], half8_t (&pf)[MT][2]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mt][r]);
+    mx = pair_max(mx) * cc;
+    if (__any(mx > raise_at)) {
+      const float m_new = mx > raise_at ? mx : m;
+      const float m_sub = m_new == -INFINITY ? 0.f : m_new;   // a row that has seen no key: exp2(-inf) = 0 and no inf - inf
+      const float alpha = __builtin_amdgcn_exp2f(m - m_sub);
+      mc = m_sub;
+      m = m_new;
+      raise_at = m_new + kLazy;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+    }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], cc, -mc));
+        sum[r & 1] += e;
+        pf[mt][r >> 3][r & 7] = to_elem<BF>(e);
+      }
+    l += sum[0] + sum[1];
+  }
+  // O^T += V^T P^T over the tile's 32 MT keys
+  __device__ __forceinline__ void accumulate(const lds_byte* vt, const int (&tr)[D / 32][2], const half8_t (&pf)[MT][2]) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          const lds_byte* vp = vt + (32 * mt + 16 * s2) * (2 * D);
+          o[dt] = mfma32<BF>(lds_frag_tr(vp + tr[dt][0], vp + tr[dt][1]), pf[mt][s2], o[dt]);
+        }
+  }
+};
+
+// S^T = K Q^T for 32 MT keys
+template <int D, int MT, bool BF>
+__device__ __forceinline__ void scores_product(const lds_byte* kt, const int (&rd)[D / 16], const half8_t (&qf)[D / 16], floatx16 (&s)[MT]) {
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[mt][r] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) s[mt] = mfma32<BF>(lds_frag(kt + 32 * mt * (2 * D) + rd[ks]), qf[ks], s[mt]);
+}
+
+// One row's 32-bit outputs (O^T layout: o[dt][r] of lane (j32, g) is row j32, column 32 dt + 8 (r / 4) + 4 g + r % 4)
+// through the wave's LDS stage (rows of 2 D bytes, 16-byte chunks XOR-ed by the row) to memory, whole rows at a time.
+template <int D, bool BF>
+__device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float inv, lds_byte* stage, int j32, int g) {
+  constexpr int kC = D / 8 - 1;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      half4_t o4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o4[e] = to_elem<BF>(o[dt][4 * q4 + e] * inv);
+      *reinterpret_cast<__attribute__((address_space(3))) half4_t*>(stage + j32 * (2 * D) + (((4 * dt + q4) ^ (j32 & kC)) << 4) + 8 * g) = o4;
+    }
+}
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScoreParams p) {
+  typedef TileLoad<D, kBlock, 4> TL;
+  __shared__ __attribute__((aligned(1024))) unsigned char k0[TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char k1[TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char v0[TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char v1[TL::kBytes];
+  __shared__ int doc_ids[4][kBlock];            // per wave: the documents of the current tile's keys
+  extern __shared__ float tab[];                // distance table (kBiasTable)
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
+
+  // XCD x takes a contiguous range of (batch, head, query tile); the tiles with most keys go first
+  const int id = (blockIdx.x & 7) * p.chunk + (blockIdx.x >> 3);
+  if (id >= p.B * p.Hq * p.tiles) return;
+  const int bh = id / p.tiles, tile = p.tiles - 1 - (id - bh * p.tiles);
+  const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
+
+  const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
+  const int row0 = tile * 128 + 32 * wave;               // this wave's first query
+  const int rows = min(p.Sq - row0, 32);                 // (<= 0: none)
+  const int i = row0 + j32;
+  const bool docs = p.docs_q != nullptr;
+
+  LaneRow L;
+  L.pos = first + i;
+  L.limit = row_limit(p.causal, klen, prefix, L.pos);
+  L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, i < p.Sq, -1) : 0;
+  L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
+  L.tab = tab;
+  if (p.bias_kind == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);   // (the walk's first barrier covers it)
+
+  // Q^T as the B operand: lane (query j32, group g) holds 8 consecutive d per step; rows past the end re-read the last
+  half8_t qf[D / 16];
+  {
+    const half_t* src = p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)min(i, p.Sq - 1) * p.qs[2];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const half8_t*>(src + 16 * ks + 8 * g);
+  }
+
+  const half_t* kb = p.k + b * p.ks[0] + hk * p.ks[1];
+  const half_t* vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  uint32_t k_off[TL::kN], v_off[TL::kN];
+  TL::offsets(k_off, wave, lane, p.ks[2]);
+  TL::offsets(v_off, wave, lane, p.vs[2]);
+  int rd[D / 16], tr[D / 32][2];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) rd[ks] = frag_off<D>(j32, g, ks);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) tr[dt][hh] = tr_off<D>(lane, dt, hh);
+
+  // ---- which key tiles: lane l decides tile 64 w + l
+  const int wg_rows = min(p.Sq - tile * 128, 128);
+  const int wg_hi = row_limit(p.causal, klen, prefix, first + tile * 128 + wg_rows - 1);
+  const int my_hi = rows > 0 ? row_limit(p.causal, klen, prefix, first + row0 + rows - 1) : 0;
+  const int my_lo = rows > 0 ? row_limit(p.causal, klen, prefix, first + row0) : 0;   // every row allows the keys below this
+  DocRange qa = {0, 0, 1, 0}, qb = qa;                    // documents of the workgroup's two 64-row blocks
+  const int nqb = (p.Sq + kBlock - 1) / kBlock, nkb = (p.Sk + kBlock - 1) / kBlock;
+  if (docs) {
+    const DocRange* dr = p.dr_q + (int64_t)b * nqb + 2 * tile;
+    qa = dr[0];
+    qb = 2 * tile + 1 < nqb ? dr[1] : DocRange{1, 0, 0, 0};
+  }
+  const DocRange mine = wave < 2 ? qa : qb;
+  const int n_tiles = (wg_hi + kBlock - 1) / kBlock;
+  const int n_win = (n_tiles + 63) >> 6;
+  uint64_t set_load = 0, set_mine = 0, set_full = 0;
+  auto window = [&](int w) {
+    const int t = 64 * w + lane, j0 = t * kBlock;
+    bool load = j0 < wg_hi, own = j0 < my_hi, full = j0 + kBlock <= my_lo;
+    if (docs && load) {
+      const DocRange r = p.dr_k[(int64_t)b * nkb + t];
+      const bool ia = ranges_meet(r, qa), ib = ranges_meet(r, qb);
+      load = ia || ib;
+      own = own && (wave < 2 ? ia : ib);
+      full = full && ranges_one(r, mine);
+    }
+    set_load = __ballot(load); set_mine = __ballot(own); set_full = __ballot(full);
+  };
+  struct Step { int t; int mine; int full; };
+  int win = 0;
+  if (n_win > 0) window(0);
+  auto next_step = [&]() -> Step {
+    while (set_load == 0) {
+      if (++win >= n_win) return Step{-1, 0, 0};
+      window(win);
+    }
+    const int bit = __builtin_ctzll(set_load);
+    set_load &= set_load - 1;
+    return Step{64 * win + bit, (int)((set_mine >> bit) & 1), (int)((set_full >> bit) & 1)};
+  };
+
+  Softmax<D, 2, BF> sm;
+  sm.init();
+
+  int next_id = 0;             // document of key `lane` of the tile whose loads are in flight
+  auto issue = [&](int t, lds_byte* kd, lds_byte* vd) {
+    const int valid = min(klen - t * kBlock, kBlock);
+    if (docs) next_id = doc_at(p.docs_k, (int64_t)b * p.Sk + t * kBlock + lane, lane < valid, -2);
+    TL::issue(rows_rsrc<D>(kb, p.ks[2], (int64_t)t * kBlock, valid), k_off, wave, kd);
+    TL::issue(rows_rsrc<D>(vb, p.vs[2], (int64_t)t * kBlock, valid), v_off, wave, vd);
+  };
+  auto step = [&](const Step cur, const Step nxt, lds_byte* kt, lds_byte* vt, lds_byte* kn, lds_byte* vn) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's share of the tile landed
+    const int cur_id = next_id;
+    if (docs) {
+      // keys of no document: whatever their values are, zeros take their place (0 times NaN is NaN)
+      const uint64_t valid = __ballot(cur_id >= 0);
+      if (~valid) TL::keep(valid, wave, lane, vt);
+    }
+    __syncthreads();
+    if (nxt.t >= 0) issue(nxt.t, kn, vn);
+    if (!cur.mine) return;
+    floatx16 s[2];
+    scores_product<D, 2, BF>(kt, rd, qf, s);
+    const int j0 = cur.t * kBlock + 4 * g;
+    if (p.k1 != 0.f) { cap_scores(p, s[0]); cap_scores(p, s[1]); }
+    if (p.bias_kind != kBiasNone) { bias_scores(p, L, j0, s[0]); bias_scores(p, L, j0 + 32, s[1]); }
+    if (!cur.full) {
+      limit_scores(L, j0, s[0]);
+      limit_scores(L, j0 + 32, s[1]);
+      if (docs) {
+        doc_ids[wave][lane] = cur_id;
+        __builtin_amdgcn_wave_barrier();
+        doc_scores(L, &doc_ids[wave][4 * g], s[0]);
+        doc_scores(L, &doc_ids[wave][32 + 4 * g], s[1]);
+      }
+    }
+    half8_t pf[2][2];
+    sm.step(p.cc, s, pf);
+    sm.accumulate(vt, tr, pf);
+  };
+  Step cur = next_step();
+  if (cur.t >= 0) issue(cur.t, (lds_byte*)k0, (lds_byte*)v0);
+  while (cur.t >= 0) {
+    Step nxt = next_step();
+    step(cur, nxt, (lds_byte*)k0, (lds_byte*)v0, (lds_byte*)k1, (lds_byte*)v1);
+    cur = nxt;
+    if (nxt.t >= 0) {
+      cur = next_step();
+      step(nxt, cur, (lds_byte*)k1, (lds_byte*)v1, (lds_byte*)k0, (lds_byte*)v0);
+    }
+  }
+
+  __syncthreads();             // every wave has left the walk: the tile buffers become output stages
+  if (rows <= 0) return;
+  const float l = pair_sum(sm.l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;              // no allowed key at all: zeros
+  if (p.lse && g == 0 && i < p.Sq) p.lse[(int64_t)bh * p.Sq + i] = l == 0.f ? -INFINITY : (sm.m + __builtin_amdgcn_logf(l)) * kLn2;
+  lds_byte* stage = (lds_byte*)(wave == 0 ? k0 : wave == 1 ? k1 : wave == 2 ? v0 : v1);
+  stage_rows<D, BF>(sm.o, inv, stage, j32, g);
+  half_t* ob = p.out + b * p.os[0] + h * p.os[1] + (int64_t)row0 * p.os[2];
+  const __amdgpu_buffer_rsrc_t o_rsrc = stof_wave_rsrc(ob);
+  constexpr int kC = D / 8;
+#pragma unroll
+  for (int n = 0; n < 32 * kC / 64; ++n) {
+    const int t = (64 / kC) * n + lane / kC, c = lane % kC;
+    const half8_t o = lds_frag(stage + t * (2 * D) + ((c ^ (t & (kC - 1))) << 4));
+    if (t < rows) stof_store16_through(o_rsrc, (uint32_t)t * (uint32_t)(p.os[2] * 2) + 16 * c, o);
+  }
+}
+
+// ---- row form.  Grid: B * Hkv * tiles (32 rows each) * splits.
+constexpr int kRowKeys = 32;
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(const ScoreParams p) {
+  typedef TileLoad<D, kRowKeys, 1> TL;
+  // (one object per buffer: the compiler orders LDS reads after in-flight loads per object)
+  __shared__ __attribute__((aligned(1024))) unsigned char k0[4 * TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char k1[4 * TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char v0[4 * TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char v1[4 * TL::kBytes];
+  __shared__ int doc_ids[4][kRowKeys];
+  __shared__ float stats[4][2][64];
+  extern __shared__ float tab[];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
+  const int G = p.group, n_rows = p.Sq * G;
+
+  const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
+  const int tile = p.tiles - 1 - rest % p.tiles, bk = rest / p.tiles;
+  const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
+  const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
+  const int r0 = tile * 32, rows = min(n_rows - r0, 32);
+  const int r = min(r0 + j32, n_rows - 1), i = r / G, hg = r - i * G, h = hk * G + hg;
+  const int i_lo = r0 / G, i_hi = (r0 + rows - 1) / G;
+  const bool docs = p.docs_q != nullptr;
+
+  // distance table of the heads in this tile: all G of them, or the rows' own when a tile has fewer rows
+  const int n_tab = 2 * p.radius + 1 + 2 * kTabPad;
+  LaneRow L;
+  L.pos = first + i;
+  L.limit = row_limit(p.causal, klen, prefix, L.pos);
+  L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, true, -1) : 0;
+  L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
+  L.tab = tab + hg * n_tab;
+  if (p.bias_kind == kBiasTable) {
+    for (int x = 0; x < G; ++x) load_table<BF>(p, hk * G + x, tab + x * n_tab, threadIdx.x, 256);
+    __syncthreads();
+  }
+
+  half8_t qf[D / 16];
+  {
+    const half_t* src = p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)i * p.qs[2];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const half8_t*>(src + 16 * ks + 8 * g);
+  }
+  const half_t* kb = p.k + b * p.ks[0] + hk * p.ks[1];
+  const half_t* vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  uint32_t k_off[TL::kN], v_off[TL::kN];
+  TL::offsets(k_off, 0, lane, p.ks[2]);
+  TL::offsets(v_off, 0, lane, p.vs[2]);
+  int rd[D / 16], tr[D / 32][2];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) rd[ks] = frag_off<D>(j32, g, ks);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) tr[dt][hh] = tr_off<D>(lane, dt, hh);
+
+  // this wave's stream of tiles: stream + n * streams; lane l decides the (64 w + l)-th of them
+  const int streams = 4 * p.splits, stream = 4 * split + wave;
+  const int hi = row_limit(p.causal, klen, prefix, first + i_hi), lo = row_limit(p.causal, klen, prefix, first + i_lo);
+  const int nqb = (p.Sq + kBlock - 1) / kBlock, nkb = (p.Sk + kBlock - 1) / kBlock;
+  DocRange qa = {0, 0, 1, 0}, qb = qa;                    // the at most two blocks that hold these queries
+  if (docs) {
+    qa = p.dr_q[(int64_t)b * nqb + i_lo / kBlock];
+    qb = p.dr_q[(int64_t)b * nqb + i_hi / kBlock];
+  }
+  const int n_tiles = (hi + kRowKeys - 1) / kRowKeys;
+  const int n_mine = stream < n_tiles ? (n_tiles - stream + streams - 1) / streams : 0;
+  const int n_win = (n_mine + 63) >> 6;
+  uint64_t set_load = 0, set_full = 0;
+  auto window = [&](int w) {
+    const int n = 64 * w + lane, t = stream + n * streams, j0 = t * kRowKeys;
+    bool load = n < n_mine, full = j0 + kRowKeys <= lo;
+    if (docs && load) {
+      const DocRange rk = p.dr_k[(int64_t)b * nkb + j0 / kBlock];
+      load = ranges_meet(rk, qa) || ranges_meet(rk, qb);
+      full = full && ranges_one(rk, qa) && ranges_one(rk, qb);
+    }
+    set_load = __ballot(load); set_full = __ballot(full);
+  };
+  struct Step { int t; int full; };
+  int win = 0;
+  if (n_win > 0) window(0);
+  auto next_step = [&]() -> Step {
+    while (set_load == 0) {
+      if (++win >= n_win) return Step{-1, 0};
+      window(win);
+    }
+    const int bit = __builtin_ctzll(set_load);
+    set_load &= set_load - 1;
+    return Step{stream + (64 * win + bit) * streams, (int)((set_full >> bit) & 1)};
+  };
+
+  Softmax<D, 1, BF> sm;
+  sm.init();
+  auto issue = [&](int t, lds_byte* kd, lds_byte* vd) {
+    const int valid = min(klen - t * kRowKeys, kRowKeys);
+    TL::issue(rows_rsrc<D>(kb, p.ks[2], (int64_t)t * kRowKeys, valid), k_off, 0, kd);
+    TL::issue(rows_rsrc<D>(vb, p.vs[2], (int64_t)t * kRowKeys, valid), v_off, 0, vd);
+  };
+  // one tile: wait for its loads (those of the tile after it stay in flight), use it, request the tile after the next into its buffers
+  auto step = [&](const Step cur, bool more, lds_byte* kt, lds_byte* vt) {
+    constexpr int kIn = 2 * TL::kN;       // load instructions of one tile
+    if (more) __builtin_amdgcn_s_waitcnt((kIn & 15) | ((kIn >> 4) << 14) | 0x0F70);
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
+    asm volatile("" ::: "memory");
+    if (docs) {
+      const int jj = cur.t * kRowKeys + j32;
+      const int id = doc_at(p.docs_k, (int64_t)b * p.Sk + jj, jj < klen, -2);
+      const uint64_t valid = __ballot(id >= 0);
+      if (~valid) TL::keep(valid, 0, lane, vt);
+      doc_ids[wave][j32] = id;
+      __builtin_amdgcn_wave_barrier();
+    }
+    floatx16 s[1];
+    scores_product<D, 1, BF>(kt, rd, qf, s);
+    const int j0 = cur.t * kRowKeys + 4 * g;
+    if (p.k1 != 0.f) cap_scores(p, s[0]);
+    if (p.bias_kind != kBiasNone) bias_scores(p, L, j0, s[0]);
+    if (!cur.full) {
+      limit_scores(L, j0, s[0]);
+      if (docs) doc_scores(L, &doc_ids[wave][4 * g], s[0]);
+    }
+    half8_t pf[1][2];
+    sm.step(p.cc, s, pf);
+    sm.accumulate(vt, tr, pf);
+  };
+  // every LDS read of the tile just used has returned, so loads may overwrite it
+  auto drained = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+  };
+  lds_byte* ka = (lds_byte*)k0 + wave * TL::kBytes; lds_byte* va = (lds_byte*)v0 + wave * TL::kBytes;
+  lds_byte* kz = (lds_byte*)k1 + wave * TL::kBytes; lds_byte* vz = (lds_byte*)v1 + wave * TL::kBytes;
+  Step cur = next_step();
+  Step nxt = cur.t >= 0 ? next_step() : cur;
+  if (cur.t >= 0) issue(cur.t, ka, va);
+  if (nxt.t >= 0) issue(nxt.t, kz, vz);
+  while (cur.t >= 0) {
+    step(cur, nxt.t >= 0, ka, va);
+    Step aft = nxt.t >= 0 ? next_step() : nxt;
+    drained();
+    if (aft.t >= 0) issue(aft.t, ka, va);
+    cur = nxt; nxt = aft;
+    if (cur.t >= 0) {
+      step(cur, nxt.t >= 0, kz, vz);
+      aft = nxt.t >= 0 ? next_step() : nxt;
+      drained();
+      if (aft.t >= 0) issue(aft.t, kz, vz);
+      cur = nxt; nxt = aft;
+    }
+  }
+
+  // ---- join the four waves: maxima and sums through `stats`, O (32 x D floats a wave) through the tile
+  // buffers, one object per wave (256 D bytes, half of it used), a quarter of the columns joined by each wave
+  stats[wave][0][lane] = sm.m;
+  stats[wave][1][lane] = sm.l;
+  __syncthreads();             // (also: every wave has left the walk)
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][0][lane]);
+  float l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float mw = stats[w][0][lane];
+    l += mw == -INFINITY ? 0.f : stats[w][1][lane] * __builtin_amdgcn_exp2f(mw - m);
+  }
+  // (a NaN maximum does not arise: fmaxf drops NaN; a NaN score makes the sum NaN)
+  const float f = sm.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm.m - m);
+  float* acc0 = reinterpret_cast<float*>(k0);
+  float* acc1 = reinterpret_cast<float*>(k1);
+  float* acc2 = reinterpret_cast<float*>(v0);
+  float* acc3 = reinterpret_cast<float*>(v1);
+  float* mine = wave == 0 ? acc0 : wave == 1 ? acc1 : wave == 2 ? acc2 : acc3;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) mine[(16 * dt + x) * 64 + lane] = sm.o[dt][x] * f;
+  __syncthreads();
+  l = pair_sum(l);
+  constexpr int kPer = D / 32 * 16 / 4;                 // register indices per wave
+  float part[kPer];
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) {
+    const int at = (kPer * wave + x) * 64 + lane;
+    part[x] = (acc0[at] + acc1[at]) + (acc2[at] + acc3[at]);
+  }
+  // register index n = kPer * wave + x of lane (j32, g): row j32, column 32 (n / 16) + 8 ((n % 16) / 4) + 4 g + n % 4
+  if (j32 >= rows) return;
+  if (p.splits > 1) {
+    const int64_t slot = ((int64_t)bk * p.tiles + tile) * p.splits + split;
+    float* po = p.part + slot * (32 * D + 64) + j32 * D;
+#pragma unroll
+    for (int x = 0; x < kPer; x += 4) {
+      const int n = kPer * wave + x, col = 32 * (n / 16) + 8 * ((n % 16) / 4) + 4 * g;
+      *reinterpret_cast<floatx4*>(po + col) = floatx4{part[x], part[x + 1], part[x + 2], part[x + 3]};
+    }
+    if (wave == 0 && g == 0) {
+      float* ps = p.part + slot * (32 * D + 64) + 32 * D;
+      ps[j32] = m;
+      ps[32 + j32] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  half_t* orow = p.out + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
+#pragma unroll
+  for (int x = 0; x < kPer; x += 4) {
+    const int n = kPer * wave + x, col = 32 * (n / 16) + 8 * ((n % 16) / 4) + 4 * g;
+    half4_t o4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o4[e] = to_elem<BF>(part[x + e] * inv);
+    *reinterpret_cast<half4_t*>(orow + col) = o4;
+  }
+  if (p.lse && wave == 0 && g == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Joins the splits of the row form: one wave per row, D / 64 columns per lane, in the order of the splits.
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int n_rows = p.Sq * p.group;
+  const int64_t bk = n / n_rows;
+  const int r = (int)(n - bk * n_rows);
+  if (bk >= (int64_t)p.B * p.Hkv) return;
+  const int tile = r / 32, j = r % 32;
+  const float* base = p.part + (bk * p.tiles + tile) * p.splits * (32 * D + 64);
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, base[s * (32 * D + 64) + 32 * D + j]);
+  float l = 0.f, o[D / 64] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float* q = base + s * (32 * D + 64);
+    const float ms = q[32 * D + j];
+    if (ms == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(ms - m);
+    l += f * q[32 * D + 32 + j];
+#pragma unroll
+    for (int x = 0; x < D / 64; ++x) o[x] += f * q[j * D + (D / 64) * lane + x];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int b = (int)(bk / p.Hkv), hk = (int)(bk - (int64_t)b * p.Hkv), i = r / p.group, h = hk * p.group + r % p.group;
+  half_t* orow = p.out + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
+#pragma unroll
+  for (int x = 0; x < D / 64; ++x) orow[(D / 64) * lane + x] = to_elem<BF>(o[x] * inv);
+  if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+}  // namespace
+
+// ---- host side
+
+// Form and number of key splits.  The row form takes calls whose rows fit one 32-row tile per key head
+// (single tokens: a token's heads read the cache once) and grids that give the wide form less than one
+// workgroup per compute unit; the keys are split until two workgroups per unit (one at head size 128,
+// whose tile buffers fill the LDS) have work, at least four tiles of 32 keys per wave's stream.
+namespace {
+
+struct Form { bool rows; int tiles, splits; };
+
+inline bool rows_fit(int group, int radius) { return radius < 0 || group * (2 * radius + 1 + 2 * kTabPad) * 4 <= 28 * 1024; }
+
+inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int form) {
+  const int group = Hq / Hkv, cus = 256;
+  const int64_t wide = (int64_t)B * Hq * ((Sq + 127) / 128);
+  const int64_t rows = (int64_t)Sq * group;
+  bool use_rows = form == 1 || (form < 0 && (rows <= 32 || wide < cus));
+  if (!rows_fit(group, radius)) use_rows = false;
+  if (!use_rows) return Form{false, (Sq + 127) / 128, 1};
+  const int tiles = (int)((rows + 31) / 32);
+  const int64_t wgs = (int64_t)B * Hkv * tiles;
+  const int64_t want = D == 64 ? 2 * cus : cus;
+  const int key_tiles = (Sk + kRowKeys - 1) / kRowKeys;
+  int64_t splits = (want + wgs - 1) / wgs;
+  const int most = (key_tiles + 15) / 16;
+  if (splits > most) splits = most;
+  if (splits < 1) splits = 1;
+  if (wgs >= want) splits = 1;
+  return Form{true, tiles, (int)splits};
+}
+
+inline int64_t ranges_bytes(int B, int Sq, int Sk) {
+  return (int64_t)B * ((Sq + kBlock - 1) / kBlock + (Sk + kBlock - 1) / kBlock) * (int64_t)sizeof(DocRange);
+}
+
+}  // namespace
+
+int score_attn_check(const void* const* req, int n_req, const int64_t* const* strides, int n_strides, int B, int Hq, int Hkv, int Sq, int Sk, int D,
+                     int dtype, float scale, float cap, int radius) {
+  for (int i = 0; i < n_req; ++i) {
+    if (!req[i]) return STOF_ERR_NULL_POINTER;
+    if (!stof_aligned16(req[i])) return STOF_ERR_MISALIGNED;
+  }
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Sk < 0 || Hq % Hkv != 0) return STOF_ERR_BAD_SHAPE;
+  if ((int64_t)B * Hq * ((Sq + 31) / 32) > 0x3fffffff || (int64_t)B * Hq * (int64_t)((Sk + 31) / 32) > 0x3fffffff || Sq > (1 << 29) || Sk > (1 << 29)) return STOF_ERR_BAD_SHAPE;
+  if (D != 64 && D != 128) return STOF_ERR_UNSUPPORTED;
+  if (dtype != STOF_DTYPE_F16 && dtype != STOF_DTYPE_BF16) return STOF_ERR_UNSUPPORTED;
+  if (!(scale > 0.f) || scale > 1e30f || !(cap >= 0.f) || cap > 1e30f || (cap > 0.f && cap < 1e-30f)) return STOF_ERR_UNSUPPORTED;
+  if (radius > STOF_SCORE_MAX_RADIUS) return STOF_ERR_UNSUPPORTED;
+  for (int i = 0; i < n_strides; ++i) {
+    if (!strides[i]) return STOF_ERR_NULL_POINTER;
+    for (int j = 0; j < 3; ++j)
+      if (strides[i][j] % 8 != 0 || strides[i][j] < 0) return STOF_ERR_MISALIGNED;
+    if (strides[i][2] > (1 << 23)) return STOF_ERR_BAD_SHAPE;   // 64 rows of a tile stay below 2^31 bytes
+  }
+  return STOF_OK;
+}
+
+void score_attn_params(ScoreParams& p, const void* q, const void* k, const void* v, const void* table, const void* slopes, const void* prefix,
+                       const void* kv_len, const void* docs_q, const void* docs_k, float scale, float cap, int radius, int causal, int q_start,
+                       int q_end, const int64_t* qs, const int64_t* ks, const int64_t* vs, int B, int Hq, int Hkv, int Sq, int Sk) {
+  p.q = (const half_t*)q; p.k = (const half_t*)k; p.v = (const half_t*)v;
+  for (int j = 0; j < 3; ++j) { p.qs[j] = qs[j]; p.ks[j] = ks[j]; p.vs[j] = vs[j]; }
+  p.table = (const half_t*)table; p.slopes = (const float*)slopes;
+  p.prefix = (const int*)prefix; p.kv_len = (const int*)kv_len;
+  p.docs_q = (const int*)docs_q; p.docs_k = (const int*)docs_k;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.group = Hq / Hkv;
+  p.radius = radius < 0 ? 0 : radius;
+  p.bias_kind = table ? kBiasTable : slopes ? kBiasSlopes : kBiasNone;
+  p.causal = causal != 0; p.q_start = q_start; p.q_end = q_end != 0;
+  p.c = scale * kLog2e;
+  p.k1 = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
+  p.capl = cap * kLog2e;
+  p.cc = (cap > 0.f || p.bias_kind != kBiasNone) ? 1.f : p.c;
+}
+
+void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st) {
+  const int nq = (p.Sq + kBlock - 1) / kBlock, nk = (p.Sk + kBlock - 1) / kBlock;
+  DocRange* dq = (DocRange*)ws;
+  DocRange* dk = dq + (int64_t)p.B * nq;
+  p.dr_q = dq; p.dr_k = dk;
+  doc_ranges_kernel<<<dim3((unsigned)(p.B * (nq + nk))), dim3(64), 0, st>>>(p.docs_q, p.docs_k, dq, dk, p.B, p.Sq, p.Sk);
+}
+
+template <int D, bool BF>
+static void launch_fwd(ScoreParams& p, const Form& f, hipStream_t st) {
+  const int n_tab = p.bias_kind == kBiasTable ? 2 * p.radius + 1 + 2 * kTabPad : 0;
+  if (f.rows) {
+    const unsigned grid = (unsigned)(p.B * p.Hkv) * (unsigned)p.tiles * (unsigned)p.splits;
+    score_attn_rows_kernel<D, BF><<<dim3(grid), dim3(256), (size_t)(p.group * n_tab) * 4, st>>>(p);
+    if (p.splits > 1) {
+      const int64_t n = (int64_t)p.B * p.Hkv * p.Sq * p.group;
+      score_attn_join_kernel<D, BF><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(p);
+    }
+  } else {
+    p.chunk = (p.B * p.Hq * p.tiles + 7) / 8;
+    score_attn_wide_kernel<D, BF><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
+  }
+}
+
+extern "C" int64_t stof_score_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int docs, int form) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Sk < 0 || Hq % Hkv != 0 || (D != 64 && D != 128)) return 0;
+  const Form f = pick_form(B, Hq, Hkv, Sq, Sk, D, radius, form);
+  int64_t n = docs ? ranges_bytes(B, Sq, Sk) : 0;
+  if (f.splits > 1) n += (int64_t)B * Hkv * f.tiles * f.splits * (32 * D + 64) * 4;
+  return n;
+}
+
+extern "C" int stof_score_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                                   const void* table, const float* slopes, const int32_t* prefix, const int32_t* kv_len,
+                                   const int32_t* docs_q, const int32_t* docs_k,
+                                   float scale, float cap, int radius, int causal, int q_start, int q_end,
+                                   const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
+                                   int B, int Hq, int Hkv, int Sq, int Sk, int D, int dtype, int form,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  const void* req[] = {q, k, v, out};
+  const int64_t* str[] = {q_strides, k_strides, v_strides, out_strides};
+  const int rc = score_attn_check(req, 4, str, 4, B, Hq, Hkv, Sq, Sk, D, dtype, scale, cap, table ? radius : -1);
+  if (rc) return rc;
+  if (table && slopes) return STOF_ERR_UNSUPPORTED;
+  if (table && radius < 0) return STOF_ERR_BAD_SHAPE;
+  if ((docs_q == nullptr) != (docs_k == nullptr)) return STOF_ERR_NULL_POINTER;
+  if (q_end && !kv_len) return STOF_ERR_NULL_POINTER;
+  if (q_start > (1 << 29) || q_start < -(1 << 29)) return STOF_ERR_BAD_SHAPE;
+  if (form < -1 || form > 1) return STOF_ERR_UNSUPPORTED;
+  const Form f = pick_form(B, Hq, Hkv, Sq, Sk, D, table ? radius : -1, form);
+  if (form == 1 && !f.rows) return STOF_ERR_UNSUPPORTED;
+  const int64_t need = stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, table ? radius : -1, docs_q != nullptr, form);
+  if (need > 0) {
+    if (!workspace) return STOF_ERR_NULL_POINTER;
+    if (!stof_aligned16(workspace)) return STOF_ERR_MISALIGNED;
+    if (workspace_bytes < need) return STOF_ERR_BAD_SHAPE;
+  }
+  ScoreParams p = {};
+  score_attn_params(p, q, k, v, table, slopes, prefix, kv_len, docs_q, docs_k, scale, cap, radius, causal, q_start, q_end,
+                    q_strides, k_strides, v_strides, B, Hq, Hkv, Sq, Sk);
+  p.out = (half_t*)out; p.lse = lse;
+  for (int j = 0; j < 3; ++j) p.os[j] = out_strides[j];
+  p.tiles = f.tiles; p.splits = f.splits;
+  hipStream_t st = (hipStream_t)stream;
+  if (docs_q) score_attn_ranges(p, workspace, st);
+  p.part = (float*)((char*)workspace + (docs_q ? ranges_bytes(B, Sq, Sk) : 0));
+  if (D == 64) { if (dtype == STOF_DTYPE_BF16) launch_fwd<64, true>(p, f, st); else launch_fwd<64, false>(p, f, st); }
+  else { if (dtype == STOF_DTYPE_BF16) launch_fwd<128, true>(p, f, st); else launch_fwd<128, false>(p, f, st); }
+  return stof_check_launch();
+}

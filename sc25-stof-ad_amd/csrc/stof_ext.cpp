@@ -79,4 +79,8 @@ PYBIND11_MODULE(_stof_ext, m) {
   STOF_BIND(stof_gemm_bias_res_ln_cluster_bounded);
   STOF_BIND(stof_gemm_bias_res_ln_cluster_workspace_bytes);
   STOF_BIND(stof_gemm_bias_res_ln_cluster);
+  STOF_BIND(stof_score_attn_workspace_bytes);
+  STOF_BIND(stof_score_attn_fwd);
+  STOF_BIND(stof_score_attn_bwd_workspace_bytes);
+  STOF_BIND(stof_score_attn_bwd);
 }
