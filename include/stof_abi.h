@@ -458,6 +458,25 @@ int stof_score_attn_bwd(const void* dout, const void* q, const void* k, const vo
                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * Linear operator in 8-bit integers (no counterpart in the reference).  x [M, K] in 16 bits (rows ldx apart):
+ *   sx_m = max_k |x_mk| / 127,  xq_mk = round(x_mk / sx_m) with the quotient taken exactly, ties to even
+ *   out_mn = act(sx_m * sw_n * sum_k xq_mk wq_nk + bias_n), the sum exact in int32
+ * wq [N, K] int8 (rows ldw apart) with fp32 scales sw [N], bias [N] and out [M, N] in x's format.  A row of zeros has
+ * scale 0; a row that is not finite has scale NaN.  K a multiple of 16 up to 131072, N a multiple of 8, ldx and
+ * ldo multiples of 8, ldw and ldq multiples of 16; pointers 16-byte aligned (sx: 4).
+ * stof_linear_i8 quantises and multiplies: one launch up to 16 tokens (workspace 0 bytes), else two through the
+ * workspace, which needs no initial contents.  stof_gemm_i8_bias_act takes rows already quantised, for
+ * several products on one x.
+ */
+int stof_quantize_rows_i8(const void* x, int8_t* xq, float* sx, int64_t M, int64_t K, int64_t ldx, int64_t ldq, int dtype, void* stream);
+int stof_gemm_i8_bias_act(const int8_t* xq, const float* sx, const int8_t* wq, const float* sw, const void* bias, void* out,
+                          int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw, int64_t ldo, int act, int dtype, void* stream);
+int64_t stof_linear_i8_workspace_bytes(int64_t M, int64_t K);
+int stof_linear_i8(const void* x, const int8_t* wq, const float* sw, const void* bias, void* out,
+                   int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int act, int dtype,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Measurement probes (no counterpart in the reference; used by bench.py, not by any operator).
  * stof_device_compute_units: compute units of the current device (hipDeviceAttributeMultiprocessorCount),
  * or a negative status.  stof_probe_clock: one wavefront spins for `iters` x 16 dependent adds between

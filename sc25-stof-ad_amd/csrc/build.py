@@ -30,7 +30,7 @@ def sources():
 
 def build(force=True, verbose=True):
     srcs = sources()
-    deps = srcs + [os.path.join(HERE, "stof_common.h"), os.path.join(ROOT, "include", "stof_abi.h")]
+    deps = srcs + [os.path.join(HERE, f) for f in os.listdir(HERE) if f.endswith(".h")] + [os.path.join(ROOT, "include", "stof_abi.h")]
     if not force and os.path.exists(OUT) and all(os.path.getmtime(OUT) >= os.path.getmtime(d) for d in deps):
         return OUT
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

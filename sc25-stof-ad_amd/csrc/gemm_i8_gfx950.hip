@@ -1,0 +1,427 @@
+// Linear operator in 8-bit integers for gfx950 (MI355X):
+//   stof_quantize_rows_i8   x [M,K] in 16 bits -> int8 with a scale for each row
+//   stof_gemm_i8_bias_act   C = act((xq wq^T) sx_m sw_n + bias)
+//   stof_linear_i8          both: the user's call on 16-bit activations
+//
+// A row's scale is a / 127 with a its largest magnitude, a value becomes round(127 x / a), ties to even.
+// That rounding is exact for 16-bit inputs: with a' = a 2^-e in [1, 2) and t = 127 x 2^-e (exact: 11 + 7 bits), the
+// quotient y = t / a' from one reciprocal and one residual step is within 2^-23 of the true quotient,
+// while a quotient of such numbers that is not k + 1/2 lies at least 2^-19 (relative) away from it.
+//
+// The products are exact: v_mfma_i32_32x32x32_i8 adds into int32, K <= 131072 keeps |sum| below 2^31.  The
+// only roundings are fp32 scaling, bias and activation, and the store.
+//
+// Large products use the tile form of the 16-bit GEMM (C^T = W X^T, both operands K-contiguous through LDS
+// rows of 128 bytes): a row of 128 bytes now holds 128 of K, so the loads, LDS reads and MFMAs of a tile
+// are those of the 16-bit kernel and do twice the arithmetic.  A few tokens use the token form: weights
+// go straight to registers, each exactly once, and every workgroup quantises the tokens itself, so a
+// single-token projection is one launch.
+#include "gemm_tile.h"
+
+namespace {
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
+typedef unsigned short ushort8_t __attribute__((ext_vector_type(8)));
+
+struct I8Params {
+  const half_t* x; const int8_t* xq; const float* sx; const int8_t* wq; const float* sw; const half_t* bias; half_t* out;
+  int M, N, K; int64_t ldx, ldq, ldw, ldo;
+  int tiles_m, tiles_n;
+};
+
+template <int ACT> __device__ __forceinline__ float act_i8(float x) {
+  if constexpr (ACT == STOF_ACT_RELU) return x < 0.f ? 0.f : x;    // (keeps the NaN of a row that was not finite)
+  else return activate<ACT>(x);
+}
+
+// Largest magnitude of 8 values as a bit pattern: the order of the patterns is the order of the magnitudes, with
+// infinity and NaN on top.
+__device__ __forceinline__ unsigned max_pattern(half8_t v, unsigned m) {
+  const ushort8_t u = __builtin_bit_cast(ushort8_t, v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, (unsigned)(u[e] & 0x7fff));
+  return m;
+}
+// One row's quantiser from its largest pattern.
+template <bool BF> struct RowQuant {
+  float a, inv, scale; int e; bool finite;
+  __device__ __forceinline__ RowQuant(unsigned pattern) {
+    finite = pattern < (BF ? 0x7f80u : 0x7c00u);
+    const float top = from_elem<BF>(__builtin_bit_cast(half_t, (unsigned short)pattern));
+    scale = finite ? top / 127.f : __builtin_nanf("");             // a row that is not finite: zeros times NaN
+    e = 0; a = 1.f;
+    if (finite && top > 0.f) {
+      e = ilogbf(top);
+      a = ldexpf(top, -e);
+    }
+    inv = 1.f / a;
+  }
+  __device__ __forceinline__ int operator()(half_t v) const {
+    const float t = 127.f * __builtin_amdgcn_ldexpf(from_elem<BF>(v), -e);
+    float y = t * inv;
+    y = __builtin_fmaf(__builtin_fmaf(-y, a, t), inv, y);
+    return finite ? (int)__builtin_rintf(y) : 0;
+  }
+  __device__ __forceinline__ uint64_t pack(half8_t v) const {
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const half_t a0 = v[i], a1 = v[i + 4];
+      lo |= (uint32_t)((*this)(a0) & 255) << (8 * i);
+      hi |= (uint32_t)((*this)(a1) & 255) << (8 * i);
+    }
+    return ((uint64_t)hi << 32) | lo;
+  }
+};
+__device__ __forceinline__ unsigned wave_max_u(unsigned m) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+  return m;
+}
+
+// One wave per row, 8 values per lane and pass; the second reading of the row comes from the caches.
+template <bool BF>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const half_t* x, int8_t* xq, float* sx, int M, int K, int64_t ldx, int64_t ldq) {
+  const int lane = threadIdx.x & 63;
+  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (m >= M) return;
+  const half_t* row = x + m * ldx;
+  unsigned top = 0;
+  for (int k = 8 * lane; k < K; k += 512) top = max_pattern(*reinterpret_cast<const half8_t*>(row + k), top);
+  const RowQuant<BF> q(wave_max_u(top));
+  for (int k = 8 * lane; k < K; k += 512)
+    *reinterpret_cast<uint64_t*>(xq + m * ldq + k) = q.pack(*reinterpret_cast<const half8_t*>(row + k));
+  if (lane == 0) sx[m] = q.scale;
+}
+
+__device__ __forceinline__ intx16 mfma_i8(int4_t a, int4_t b, intx16 c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ int4_t lds_frag_i8(const lds_byte* tile, int off) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) int4_t*>(tile + off);
+}
+
+// ---- tile form: T x T output tile, 4 waves as 2 x 2, each T/2 tokens x T/2 features; K tiles of 128, double buffered.
+constexpr int kI8K = 128;
+
+template <int ACT, bool BF, int T>
+__global__ __launch_bounds__(256, 2) void gemm_i8_kernel(const I8Params p) {
+  constexpr int kTile = T * kI8K;
+  constexpr int kLoads = T / 32;            // load instructions per wave and operand tile (8 rows each)
+  constexpr int kMT = T / 64;               // 32-wide MFMA tiles per wave and direction
+  __shared__ __attribute__((aligned(1024))) unsigned char a0[kTile];
+  __shared__ __attribute__((aligned(1024))) unsigned char a1[kTile];
+  __shared__ __attribute__((aligned(1024))) unsigned char w0[kTile];
+  __shared__ __attribute__((aligned(1024))) unsigned char w1[kTile];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
+  const int wm = wave >> 1, wn = wave & 1;
+  int tm, tn;
+  if (!raster_tile((int)blockIdx.x, p.tiles_m, p.tiles_n, tm, tn)) return;
+  const int m0 = tm * T, n0 = tn * T;
+
+  // rows past the edge re-read the last row; in the last K tile, chunks past K lie beyond the resource's
+  // extent and arrive as zeros
+  constexpr uint32_t kOut = 0x80000000u;
+  uint32_t a_off[kLoads], w_off[kLoads];
+  int chunk_k[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = 8 * (kLoads * wave + i) + (lane >> 3);
+    const int chunk = (lane & 7) ^ swz(r);
+    chunk_k[i] = 16 * chunk;
+    a_off[i] = (uint32_t)min(r, p.M - 1 - m0) * (uint32_t)p.ldq + 16 * chunk;
+    w_off[i] = (uint32_t)min(r, p.N - 1 - n0) * (uint32_t)p.ldw + 16 * chunk;
+  }
+  const __amdgpu_buffer_rsrc_t a_rs = stof_wave_rsrc(p.xq + (int64_t)m0 * p.ldq), w_rs = stof_wave_rsrc(p.wq + (int64_t)n0 * p.ldw);
+  auto issue = [&](int kt, lds_byte* ad, lds_byte* wd) {
+    const uint32_t koff = (uint32_t)kt * kI8K;
+    const int left = p.K - kt * kI8K;
+    if (left >= kI8K) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) dma16b(a_rs, a_off[i], koff, ad + (kLoads * wave + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) dma16b(w_rs, w_off[i], koff, wd + (kLoads * wave + i) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) dma16b(a_rs, chunk_k[i] < left ? a_off[i] : kOut, koff, ad + (kLoads * wave + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) dma16b(w_rs, chunk_k[i] < left ? w_off[i] : kOut, koff, wd + (kLoads * wave + i) * 1024);
+    }
+  };
+  int rd[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) rd[ks] = j32 * kI8K + (((2 * ks + g) ^ swz(j32)) << 4);
+
+  intx16 acc[kMT][kMT];                     // [feature tile][token tile]
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kMT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+  auto compute = [&](const lds_byte* at, const lds_byte* wt) {
+    int4_t xa[2][kMT], wb[2][kMT];
+    auto fetch = [&](int ks, int set) {
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) xa[set][i] = lds_frag_i8(at, (T / 2 * wm + 32 * i) * kI8K + rd[ks]);
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) wb[set][i] = lds_frag_i8(wt, (T / 2 * wn + 32 * i) * kI8K + rd[ks]);
+    };
+    fetch(0, 0);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks + 1 < 4) fetch(ks + 1, (ks + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ni = 0; ni < kMT; ++ni)
+#pragma unroll
+        for (int mi = 0; mi < kMT; ++mi) acc[ni][mi] = mfma_i8(wb[ks & 1][ni], xa[ks & 1][mi], acc[ni][mi]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const int nk = (p.K + kI8K - 1) / kI8K;
+  issue(0, (lds_byte*)a0, (lds_byte*)w0);
+  for (int kt = 0; kt < nk; kt += 2) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0): this wave's share of tile kt landed
+    __syncthreads();
+    if (kt + 1 < nk) issue(kt + 1, (lds_byte*)a1, (lds_byte*)w1);
+    compute((const lds_byte*)a0, (const lds_byte*)w0);
+    if (kt + 1 < nk) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+      __syncthreads();
+      if (kt + 2 < nk) issue(kt + 2, (lds_byte*)a0, (lds_byte*)w0);
+      compute((const lds_byte*)a1, (const lds_byte*)w1);
+    }
+  }
+  __syncthreads();                          // every wave is done with the operand tiles
+
+  // epilogue: 32 tokens x (T / 2) features at a time through the wave's own LDS rows (kMT * 64 bytes, 16-byte chunks
+  // XOR-ed by the row) and out in whole rows
+  constexpr int kRow = kMT * 64, kC = kRow / 16;
+  lds_byte* stage = (lds_byte*)a0 + wave * (32 * kRow);
+  const int m_base = m0 + T / 2 * wm, n_base = n0 + T / 2 * wn;
+  const __amdgpu_buffer_rsrc_t o_rs = stof_wave_rsrc(p.out + (int64_t)m_base * p.ldo + n_base);
+  floatx4 sw[kMT][4], bv[kMT][4];
+#pragma unroll
+  for (int ni = 0; ni < kMT; ++ni)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int n = n_base + 32 * ni + 8 * q4 + 4 * g;
+      sw[ni][q4] = bv[ni][q4] = floatx4{0.f, 0.f, 0.f, 0.f};
+      if (n < p.N) {                        // N % 8 == 0: four features are inside or outside together
+        sw[ni][q4] = *reinterpret_cast<const floatx4*>(p.sw + n);
+        if (p.bias) {
+          const half4_t b4 = *reinterpret_cast<const half4_t*>(p.bias + n);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { const half_t be = b4[e]; bv[ni][q4][e] = from_elem<BF>(be); }
+        }
+      }
+    }
+#pragma unroll
+  for (int mi = 0; mi < kMT; ++mi) {
+    const float sx = p.sx[min(m_base + 32 * mi + j32, p.M - 1)];
+#pragma unroll
+    for (int ni = 0; ni < kMT; ++ni)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        half4_t o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[e] = to_elem<BF>(act_i8<ACT>(__builtin_fmaf((float)acc[ni][mi][4 * q4 + e], sx * sw[ni][q4][e], bv[ni][q4][e])));
+        *reinterpret_cast<__attribute__((address_space(3))) half4_t*>(stage + j32 * kRow + (((4 * ni + q4) ^ (j32 & (kC - 1))) << 4) + 8 * g) = o;
+      }
+#pragma unroll
+    for (int i = 0; i < 32 * kC / 64; ++i) {
+      const int t = (64 / kC) * i + lane / kC, c = lane % kC;
+      const half8_t o = lds_frag(stage, t * kRow + ((c ^ (t & (kC - 1))) << 4));
+      if (m_base + 32 * mi + t < p.M && n_base + 8 * c < p.N)
+        stof_store16_through(o_rs, (uint32_t)(32 * mi + t) * (uint32_t)(p.ldo * 2) + 16 * c, o);
+    }
+  }
+}
+
+// ---- token form: up to 16 tokens, 16 features per workgroup, K split over the four waves.
+// v_mfma_i32_16x16x64_i8: A = 16 weight rows (lane & 15) x 64 of K (16 bytes per lane, group lane >> 4), B = the tokens from
+// LDS.  Result: token lane & 15, features 4 (lane >> 4) + r.  A wave's weights arrive in rounds of kTokLoads loads, the
+// next round requested before the products of the current one.
+constexpr int kTokMax = 16;
+constexpr int kTokLoads = 8;
+constexpr int kTokLds = 64 * 1024;
+
+template <int ACT, bool BF>
+__global__ __launch_bounds__(256) void linear_i8_token_kernel(const I8Params p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char xq_lds[];       // [M][Kp], Kp = K rounded up to 64, zeros beyond K
+  __shared__ unsigned tops[4][kTokMax];
+  __shared__ float sxs[kTokMax];
+  __shared__ int sums[4][16][17];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int steps = (p.K + 63) / 64, Kp = steps * 64;
+  const int8_t* wrow = p.wq + (int64_t)min(n0 + row, p.N - 1) * p.ldw;
+  // K step s of this wave: 64 (4 s + wave)
+  auto weights = [&](int s) -> int4_t {
+    const int k = 64 * (4 * s + wave) + 16 * kg;
+    return *reinterpret_cast<const int4_t*>(wrow + (k < p.K ? k : 0));          // (times zeros of x beyond K)
+  };
+  const int mine = (steps - wave + 3) / 4;
+  int4_t wa[kTokLoads];
+#pragma unroll
+  for (int i = 0; i < kTokLoads; ++i) wa[i] = i < mine ? weights(i) : int4_t{0, 0, 0, 0};
+
+  // the tokens: one or more passes of 256 threads x 8 values over each row
+  for (int m = 0; m < p.M; ++m) {
+    unsigned top = 0;
+    for (int k = 8 * threadIdx.x; k < p.K; k += 2048) top = max_pattern(*reinterpret_cast<const half8_t*>(p.x + m * p.ldx + k), top);
+    top = wave_max_u(top);
+    if (lane == 0) tops[wave][m] = top;
+  }
+  __syncthreads();
+  for (int m = 0; m < p.M; ++m) {
+    const RowQuant<BF> q(max(max(tops[0][m], tops[1][m]), max(tops[2][m], tops[3][m])));
+    for (int k = 8 * threadIdx.x; k < Kp; k += 2048)
+      *reinterpret_cast<uint64_t*>(xq_lds + m * Kp + k) = k < p.K ? q.pack(*reinterpret_cast<const half8_t*>(p.x + m * p.ldx + k)) : 0;
+    if (threadIdx.x == 0) sxs[m] = q.scale;
+  }
+  __syncthreads();
+
+  const unsigned char* xrow = xq_lds + min(row, p.M - 1) * Kp;
+  int4_t acc = {0, 0, 0, 0};
+  for (int s0 = 0; s0 < mine; s0 += kTokLoads) {
+    int4_t wn[kTokLoads];
+#pragma unroll
+    for (int i = 0; i < kTokLoads; ++i) wn[i] = s0 + kTokLoads + i < mine ? weights(s0 + kTokLoads + i) : int4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kTokLoads; ++i)
+      if (s0 + i < mine) {
+        const int4_t xb = *reinterpret_cast<const int4_t*>(xrow + 64 * (4 * (s0 + i) + wave) + 16 * kg);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wa[i], xb, acc, 0, 0, 0);
+      }
+#pragma unroll
+    for (int i = 0; i < kTokLoads; ++i) wa[i] = wn[i];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) sums[wave][row][4 * kg + r] = acc[r];
+  __syncthreads();
+  // thread (token t, feature f)
+  const int t = threadIdx.x >> 4, f = threadIdx.x & 15, n = n0 + f;
+  if (t < p.M && n < p.N) {
+    const int total = (sums[0][t][f] + sums[1][t][f]) + (sums[2][t][f] + sums[3][t][f]);
+    const float b = p.bias ? from_elem<BF>(p.bias[n]) : 0.f;
+    p.out[(int64_t)t * p.ldo + n] = to_elem<BF>(act_i8<ACT>(__builtin_fmaf((float)total, sxs[t] * p.sw[n], b)));
+  }
+}
+
+bool token_form(int64_t M, int64_t K) { return M <= kTokMax && M * ((K + 63) / 64 * 64) <= kTokLds; }
+int64_t padded(int64_t K) { return (K + 15) / 16 * 16; }
+
+// T = 128 while its tiles fill the device; else 64, four times the workgroups
+int tile_edge(int64_t M, int64_t N) { return ((M + 127) / 128) * ((N + 127) / 128) >= 256 ? 128 : 64; }
+
+template <int ACT, bool BF>
+void launch_gemm(I8Params& p, hipStream_t st) {
+  const int T = tile_edge(p.M, p.N);
+  p.tiles_m = (p.M + T - 1) / T;
+  p.tiles_n = (p.N + T - 1) / T;
+  const unsigned grid = raster_grid(p.tiles_m, p.tiles_n);
+  if (T == 128) gemm_i8_kernel<ACT, BF, 128><<<dim3(grid), dim3(256), 0, st>>>(p);
+  else gemm_i8_kernel<ACT, BF, 64><<<dim3(grid), dim3(256), 0, st>>>(p);
+}
+template <int ACT, bool BF>
+void launch_token(I8Params& p, hipStream_t st) {
+  const size_t lds = (size_t)p.M * ((p.K + 63) / 64 * 64);
+  linear_i8_token_kernel<ACT, BF><<<dim3((unsigned)((p.N + 15) / 16)), dim3(256), lds, st>>>(p);
+}
+template <bool BF>
+void launch_act(I8Params& p, int act, bool token, hipStream_t st) {
+  switch (act) {
+    case STOF_ACT_NONE: token ? launch_token<STOF_ACT_NONE, BF>(p, st) : launch_gemm<STOF_ACT_NONE, BF>(p, st); break;
+    case STOF_ACT_GELU_ERF: token ? launch_token<STOF_ACT_GELU_ERF, BF>(p, st) : launch_gemm<STOF_ACT_GELU_ERF, BF>(p, st); break;
+    case STOF_ACT_GELU_TANH: token ? launch_token<STOF_ACT_GELU_TANH, BF>(p, st) : launch_gemm<STOF_ACT_GELU_TANH, BF>(p, st); break;
+    default: token ? launch_token<STOF_ACT_RELU, BF>(p, st) : launch_gemm<STOF_ACT_RELU, BF>(p, st); break;
+  }
+}
+void launch_quantize(const void* x, int8_t* xq, float* sx, int M, int K, int64_t ldx, int64_t ldq, int dtype, hipStream_t st) {
+  const dim3 grid((unsigned)((M + 3) / 4));
+  if (dtype == STOF_DTYPE_BF16) quantize_rows_kernel<true><<<grid, dim3(256), 0, st>>>((const half_t*)x, xq, sx, M, K, ldx, ldq);
+  else quantize_rows_kernel<false><<<grid, dim3(256), 0, st>>>((const half_t*)x, xq, sx, M, K, ldx, ldq);
+}
+
+int check_sizes(int64_t M, int64_t N, int64_t K, int dtype) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || N % 8 != 0) return STOF_ERR_BAD_SHAPE;
+  if (M > (1 << 28) || N > (1 << 28) || K > 131072 || ((M + 63) / 64 + 8) * ((N + 63) / 64) > 0x0fffffff) return STOF_ERR_BAD_SHAPE;
+  if (dtype != STOF_DTYPE_F16 && dtype != STOF_DTYPE_BF16) return STOF_ERR_UNSUPPORTED;
+  return STOF_OK;
+}
+int check_common(const void* wq, const float* sw, const void* bias, const void* out, int64_t K, int64_t N, int64_t ldw, int64_t ldo, int act) {
+  if (!wq || !sw || !out) return STOF_ERR_NULL_POINTER;
+  if (!stof_aligned16(wq) || !stof_aligned16(sw) || !stof_aligned16(out) || (bias && !stof_aligned16(bias))) return STOF_ERR_MISALIGNED;
+  if (ldw < K || ldo < N || ldw > (1 << 23) || ldo > (1 << 22)) return STOF_ERR_BAD_SHAPE;    // 128 rows of a tile stay below 2^31 bytes
+  if (ldw % 16 != 0 || ldo % 8 != 0) return STOF_ERR_MISALIGNED;
+  if (act < STOF_ACT_NONE || act > STOF_ACT_RELU) return STOF_ERR_UNSUPPORTED;
+  return STOF_OK;
+}
+
+}  // namespace
+
+extern "C" int stof_quantize_rows_i8(const void* x, int8_t* xq, float* sx, int64_t M, int64_t K, int64_t ldx, int64_t ldq, int dtype, void* stream) {
+  const int rc = check_sizes(M, 8, K, dtype);
+  if (rc) return rc;
+  if (!x || !xq || !sx) return STOF_ERR_NULL_POINTER;
+  if (!stof_aligned16(x) || !stof_aligned16(xq) || ldx % 8 != 0 || ldq % 16 != 0) return STOF_ERR_MISALIGNED;
+  if (ldx < K || ldq < K) return STOF_ERR_BAD_SHAPE;
+  launch_quantize(x, xq, sx, (int)M, (int)K, ldx, ldq, dtype, (hipStream_t)stream);
+  return stof_check_launch();
+}
+
+extern "C" int stof_gemm_i8_bias_act(const int8_t* xq, const float* sx, const int8_t* wq, const float* sw, const void* bias, void* out,
+                                     int64_t M, int64_t N, int64_t K, int64_t ldq, int64_t ldw, int64_t ldo, int act, int dtype, void* stream) {
+  int rc = check_sizes(M, N, K, dtype);
+  if (rc) return rc;
+  rc = check_common(wq, sw, bias, out, K, N, ldw, ldo, act);
+  if (rc) return rc;
+  if (!xq || !sx) return STOF_ERR_NULL_POINTER;
+  if (!stof_aligned16(xq) || ldq % 16 != 0) return STOF_ERR_MISALIGNED;
+  if (ldq < K || ldq > (1 << 23)) return STOF_ERR_BAD_SHAPE;
+  I8Params p = {};
+  p.xq = xq; p.sx = sx; p.wq = wq; p.sw = sw; p.bias = (const half_t*)bias; p.out = (half_t*)out;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K; p.ldq = ldq; p.ldw = ldw; p.ldo = ldo;
+  if (dtype == STOF_DTYPE_BF16) launch_act<true>(p, act, false, (hipStream_t)stream);
+  else launch_act<false>(p, act, false, (hipStream_t)stream);
+  return stof_check_launch();
+}
+
+extern "C" int64_t stof_linear_i8_workspace_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || token_form(M, K)) return 0;
+  return M * padded(K) + (M * 4 + 15) / 16 * 16;
+}
+
+extern "C" int stof_linear_i8(const void* x, const int8_t* wq, const float* sw, const void* bias, void* out,
+                              int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldo, int act, int dtype,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_sizes(M, N, K, dtype);
+  if (rc) return rc;
+  rc = check_common(wq, sw, bias, out, K, N, ldw, ldo, act);
+  if (rc) return rc;
+  if (!x) return STOF_ERR_NULL_POINTER;
+  if (!stof_aligned16(x) || ldx % 8 != 0) return STOF_ERR_MISALIGNED;
+  if (ldx < K) return STOF_ERR_BAD_SHAPE;
+  const bool token = token_form(M, K);
+  I8Params p = {};
+  if (!token) {
+    if (!workspace) return STOF_ERR_NULL_POINTER;
+    if (!stof_aligned16(workspace)) return STOF_ERR_MISALIGNED;
+    if (workspace_bytes < stof_linear_i8_workspace_bytes(M, K)) return STOF_ERR_BAD_SHAPE;
+    p.ldq = padded(K);
+    p.xq = (int8_t*)workspace;
+    p.sx = (float*)((char*)workspace + M * p.ldq);
+    launch_quantize(x, (int8_t*)p.xq, (float*)p.sx, (int)M, (int)K, ldx, p.ldq, dtype, (hipStream_t)stream);
+  }
+  p.x = (const half_t*)x; p.wq = wq; p.sw = sw; p.bias = (const half_t*)bias; p.out = (half_t*)out;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K; p.ldx = ldx; p.ldw = ldw; p.ldo = ldo;
+  if (dtype == STOF_DTYPE_BF16) launch_act<true>(p, act, token, (hipStream_t)stream);
+  else launch_act<false>(p, act, token, (hipStream_t)stream);
+  return stof_check_launch();
+}

@@ -83,4 +83,8 @@ PYBIND11_MODULE(_stof_ext, m) {
   STOF_BIND(stof_score_attn_fwd);
   STOF_BIND(stof_score_attn_bwd_workspace_bytes);
   STOF_BIND(stof_score_attn_bwd);
+  STOF_BIND(stof_quantize_rows_i8);
+  STOF_BIND(stof_gemm_i8_bias_act);
+  STOF_BIND(stof_linear_i8_workspace_bytes);
+  STOF_BIND(stof_linear_i8);
 }

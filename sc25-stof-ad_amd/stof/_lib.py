@@ -80,6 +80,10 @@ _SIGNATURES = {
     "stof_score_attn_bwd_workspace_bytes": (c_int64, [c_int] * 8),
     "stof_score_attn_bwd": (c_int, [_P] * 16 + [c_float, c_float, c_int, c_int, c_int, c_int] + [POINTER(c_int64)] * 5 +
                             [c_int] * 7 + [_P, c_int64, _P]),
+    "stof_quantize_rows_i8": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
+    "stof_gemm_i8_bias_act": (c_int, [_P] * 6 + [c_int64] * 6 + [c_int, c_int, _P]),
+    "stof_linear_i8_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "stof_linear_i8": (c_int, [_P] * 5 + [c_int64] * 6 + [c_int, c_int, _P, c_int64, _P]),
 }
 
 
