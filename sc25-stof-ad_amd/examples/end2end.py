@@ -6,10 +6,13 @@ the stack with plain PyTorch ops ("TorchNative") and with this library's fused l
 QKV GEMM, block-masked attention, GEMM + bias + residual + LayerNorm, GEMM + bias + activation,
 GEMM + bias + residual + LayerNorm); print ms per iteration in the reference's format.  In
 addition the two outputs are compared.  T5 is run as its encoder stack (ReLU feed-forward,
-:154-210); the decoder's cross attention is not part of this library.
+:154-210); the decoder's cross attention is not part of this library.  --position_bias gives the layers a
+learned distance table (as T5 has; every key open, so the mask family is not used) and --linear int8 runs
+their linear operators in 8-bit integers.
 
     python sc25-stof-ad_amd/examples/end2end.py --model bert_base --batch_size 8 --seq_len 512 --method both
     python sc25-stof-ad_amd/examples/end2end.py --model gpt --batch_size 1 --seq_len 512 --graph
+    python sc25-stof-ad_amd/examples/end2end.py --model t5 --batch_size 8 --seq_len 512 --position_bias --linear int8
 """
 import argparse
 import math
@@ -25,6 +28,7 @@ from util.masks import (generate_bigbird_mask, generate_longformer_mask, generat
 from util.utils import time_stamp_cudasync, torch_cuda_identify                 # noqa: E402
 from stof import configs                                                        # noqa: E402
 from stof.layer import CapturedForward, EncoderStack, eager_layer               # noqa: E402
+from stof.scores import ScoreMask                                               # noqa: E402
 
 # model -> (heads, layers, feed-forward activation); head size 64, hidden = 64 * heads (src/benchmk_end2end.py:383-407)
 MODELS = {
@@ -60,6 +64,8 @@ def main():
     ap.add_argument("--batch_size", type=int, default=8)
     ap.add_argument("--seq_len", type=int, default=1024)
     ap.add_argument("--graph", action="store_true", help="STOF: record the stack into a HIP graph once and replay it (small batches are paced by issuing the launches)")
+    ap.add_argument("--position_bias", action="store_true", help="a learned table of the distances -128 .. 128 added to the scores; replaces the mask")
+    ap.add_argument("--linear", default="16bit", choices=["16bit", "int8"], help="STOF: the linear operators in the tensors' format or in 8-bit integers")
     ap.add_argument("--warmup_iters", type=int, default=20)
     ap.add_argument("--running_iters", type=int, default=100)
     args = ap.parse_args()
@@ -71,10 +77,19 @@ def main():
     hidden, ffn = 64 * heads, 256 * heads
     B, S = args.batch_size, args.seq_len
 
-    mask_name, mask = build_mask(args.mask_id, S, args.block_m, args.block_n, device)
-    mask = mask.to(device)
-    nnz, *lut = get_sparse_storage(mask, args.block_m, args.block_n)
-    print(f"{mask_name}: nnz figure {float(nnz):.1f}, {int(lut[5][-1])} of {math.ceil(S / args.block_m) * math.ceil(S / args.block_n)} blocks active")
+    scores, dense_bias = None, None
+    if args.position_bias:
+        radius = 128
+        table = (torch.randn(heads, 2 * radius + 1, generator=torch.Generator().manual_seed(7)) * 0.5).half().to(device)
+        at = torch.arange(S, device=device)
+        dense_bias = table[:, (at[None, :] - at[:, None]).clamp(-radius, radius) + radius]
+        scores, lut, mask = dict(bias=table), ScoreMask(), torch.ones(1, S, S, dtype=torch.float16, device=device)
+        print(f"Position table: distances up to {radius}, every key open")
+    else:
+        mask_name, mask = build_mask(args.mask_id, S, args.block_m, args.block_n, device)
+        mask = mask.to(device)
+        nnz, *lut = get_sparse_storage(mask, args.block_m, args.block_n)
+        print(f"{mask_name}: nnz figure {float(nnz):.1f}, {int(lut[5][-1])} of {math.ceil(S / args.block_m) * math.ceil(S / args.block_n)} blocks active")
 
     weights = [{k: v.to(device) for k, v in configs.layer_weights(hidden, ffn, seed=100 + i).items()} for i in range(layers)]
     x = configs.layer_input(configs.LayerConfig(args.model, B, S, hidden, heads, ffn, layers), seed=1, device=device)
@@ -83,10 +98,10 @@ def main():
         h = x
         with torch.no_grad():
             for w in weights:
-                h = eager_layer(h, w, mask, heads, 1e-12, gelu=act)
+                h = eager_layer(h, w, mask, heads, 1e-12, gelu=act, bias=dense_bias)
         return h
 
-    stack = EncoderStack(weights, heads, eps=1e-12, gelu=act)
+    stack = EncoderStack(weights, heads, eps=1e-12, gelu=act, scores=scores, linear=args.linear)
     fused = lambda: stack(x, lut, args.block_m)
     if args.graph:
         captured = CapturedForward(stack, x, lut, args.block_m)
