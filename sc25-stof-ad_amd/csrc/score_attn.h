@@ -113,15 +113,25 @@ __device__ __forceinline__ half8_t lds_frag_tr(const lds_byte* p0, const lds_byt
   return __builtin_bit_cast(half8_t, (short8_t)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// ROWS rows of a [rows, D] operand as a buffer resource: base in scalar registers, extent up to the last
-// valid row, so rows past it arrive as zeros whatever memory holds there.
-template <int D>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const half_t* base, int64_t stride, int64_t first, int valid) {
-  const uint64_t a = reinterpret_cast<uint64_t>(base + first * stride);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
-  const int bytes = valid > 0 ? ((valid - 1) * (int)stride + D) * 2 : 0;
-  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
-}
+// A [rows, D] operand whose tiles are loaded: base address, bytes of a row and of a tile of ROWS rows.  Tile t becomes a
+// buffer resource with its base in scalar registers and its extent up to the last of `valid` rows, so rows
+// past it arrive as zeros whatever memory holds there.  (The 64-bit base per tile keeps operands beyond
+// 2^32 bytes possible; strides are below 2^23 elements, so everything inside a tile fits 32 bits.)
+template <int D, int ROWS> struct TileSource {
+  uint64_t base; uint32_t row_bytes;
+  __device__ __forceinline__ void set(const half_t* p, int64_t stride) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    // (through uint32_t: readfirstlane returns a signed int, whose upper half would be its sign)
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+    base = ((uint64_t)hi << 32) | lo;
+    row_bytes = (uint32_t)stride * 2;
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(int t, int valid) const {
+    const uint64_t a = base + (uint64_t)(uint32_t)t * (uint64_t)(ROWS * row_bytes);
+    const uint32_t bytes = (uint32_t)(valid - 1) * row_bytes + 2 * D;
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(a), 0, (int)bytes, 0x00020000);
+  }
+};
 
 // Direct-to-LDS load of a tile of ROWS rows by WAVES waves: one instruction brings 1 KB (1024 / (2 D) rows).
 template <int D, int ROWS, int WAVES> struct TileLoad {
@@ -181,8 +191,9 @@ __device__ __forceinline__ void cap_scores(const ScoreParams& p, floatx16& s) {
     s[r] = __builtin_fmaf(u, -2.f * p.capl, p.capl);
   }
 }
+template <bool CAP>
 __device__ __forceinline__ void bias_scores(const ScoreParams& p, const LaneRow& L, int j0 /* jb + 4 g */, floatx16& s) {
-  const float mul = p.k1 != 0.f ? 1.f : p.c;
+  const float mul = CAP ? 1.f : p.c;
   if (p.bias_kind == kBiasTable) {
     const int x = min(max(j0 - L.pos, -p.radius - kTabPad), p.radius);
     const float* t = L.tab + (x + p.radius + kTabPad);
@@ -205,11 +216,9 @@ __device__ __forceinline__ void doc_scores(const LaneRow& L, const int* ids, flo
   for (int r = 0; r < 16; ++r) s[r] = ids[key_off(r)] == L.doc ? s[r] : -INFINITY;
 }
 
-// Document of position i of a sequence of n: -1 for none (queries), -2 for none (keys), so that they never match.
-__device__ __forceinline__ int doc_at(const int* docs, int64_t i, bool inside, int none) {
-  const int d = inside ? docs[i] : none;
-  return d < 0 ? none : d;
-}
+// Document of position i, -1 for none (queries) or -2 (keys), so that they never match.
+__device__ __forceinline__ int doc_or(int d, int none) { return d < 0 ? none : d; }
+__device__ __forceinline__ int doc_at(const int* docs, int64_t i, bool inside, int none) { return doc_or(inside ? docs[i] : none, none); }
 
 // Host helpers shared by the forward and backward entry points (score_attn_gfx950.hip).
 #pragma GCC visibility push(hidden)

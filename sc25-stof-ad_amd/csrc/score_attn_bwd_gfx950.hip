@@ -18,6 +18,8 @@
 // keeps 11 bits down to 2^-29 of the bound.  P is carried as 2^12 P.  bfloat16 needs neither.
 #include "score_attn.h"
 
+#include <type_traits>
+
 namespace {
 
 struct BwdParams {
@@ -123,26 +125,31 @@ __device__ __forceinline__ void cap_scores_grad(const ScoreParams& p, floatx16& 
   }
 }
 
-// A operand rows 32 x D of the tile times the lane's vector: 32 x 32 products
-template <int D, bool BF>
-__device__ __forceinline__ floatx16 product32(const lds_byte* t, const int (&rd)[D / 16], const half8_t (&f)[D / 16]) {
+// A step works on a tile's two pieces of 32 rows (pieces 0 and 1) in four phases of D / 16 slices with two
+// MFMAs each, scores and dP or sums.  Pipelined order (head size 128 without a table):
+//     0: scores and dP of piece 0      1: those of piece 1, and the softmax of piece 0
+//     2: sums of piece 0, and the softmax of piece 1      3: sums of piece 1
+// so that in phases 1 and 2 the vector arithmetic stands between MFMAs it does not depend on: one wave lives
+// on a SIMD there (its accumulators and operands fill more than 256 registers) and nothing else would fill
+// the matrix pipeline meanwhile.  Plain order (head size 64, where two waves share a SIMD and 256
+// registers do not hold both pieces; and with a table): piece 0, then piece 1.  The LDS fragments of a
+// slice are requested two slices ahead, in a ring of three; scheduling fences between slices keep that order.
+template <bool PIPE> struct Phases {
+  static __device__ __forceinline__ constexpr bool scores(int ph) { return PIPE ? ph < 2 : (ph & 1) == 0; }
+  static __device__ __forceinline__ constexpr int piece(int ph) { return PIPE ? ph & 1 : ph >> 1; }
+};
+#define STOF_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// fragment n = s2 * (D / 32) + dt of 32 transposed rows
+template <int D> __device__ __forceinline__ half8_t frag_tr(const lds_byte* t, int n, const int (&tr)[D / 32][2]) {
+  const int s2 = n / (D / 32), dt = n % (D / 32);
+  return lds_frag_tr(t + 16 * s2 * (2 * D) + tr[dt][0], t + 16 * s2 * (2 * D) + tr[dt][1]);
+}
+__device__ __forceinline__ floatx16 zero16() {
   floatx16 s;
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) s = mfma32<BF>(lds_frag(t + rd[ks]), f[ks], s);
   return s;
-}
-// acc^T += T^T X for 32 rows of the tile: X in the accumulator layout, as 16-bit values
-template <int D, bool BF>
-__device__ __forceinline__ void accumulate32(floatx16 (&acc)[D / 32], const lds_byte* t, const int (&tr)[D / 32][2], const half8_t (&x)[2]) {
-#pragma unroll
-  for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) {
-      const lds_byte* p = t + 16 * s2 * (2 * D);
-      acc[dt] = mfma32<BF>(lds_frag_tr(p + tr[dt][0], p + tr[dt][1]), x[s2], acc[dt]);
-    }
 }
 
 // 32 gradient rows of a wave through its LDS stage (rows of 2 D bytes) to contiguous rows at dst
@@ -177,7 +184,7 @@ __device__ __forceinline__ void store_rows(const floatx16 (&o)[D / 32], float mu
 // delta' = sum_j P_ij dP_ij is formed along the way in fp32, and with M = P (1 - tanh^2) K as one product more
 //     dQ = scale (dT(delta) K - (delta' - delta) M)
 // is exact in delta while the second term stays small.  delta' replaces delta for the kernel of the keys.
-template <int D, bool BF>
+template <int D, bool BF, bool CAP>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;
   typedef TileLoad<D, kBlock, 4> TL;
@@ -237,8 +244,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
     down = bp.scale * pow2(-k);
   }
 
-  const half_t* kb = p.k + b * p.ks[0] + hk * p.ks[1];
-  const half_t* vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  TileSource<D, kBlock> ksrc, vsrc;
+  ksrc.set(p.k + b * p.ks[0] + hk * p.ks[1], p.ks[2]);
+  vsrc.set(p.v + b * p.vs[0] + hk * p.vs[1], p.vs[2]);
   uint32_t k_off[TL::kN], v_off[TL::kN];
   TL::offsets(k_off, wave, lane, p.ks[2]);
   TL::offsets(v_off, wave, lane, p.vs[2]);
@@ -295,16 +303,18 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
     for (int r = 0; r < 16; ++r) { acc[x][r] = 0.f; mac[x][r] = 0.f; }
   float off = 0.f;                              // delta' - delta: sum_j P_ij (dP_ij - delta) (this lane's keys)
 
-  int next_id = 0;
+  int next_valid = 0, next_id = 0;
   auto issue = [&](int t, lds_byte* kd, lds_byte* vd) {
     const int valid = min(klen - t * kBlock, kBlock);
-    if (docs) next_id = doc_at(p.docs_k, (int64_t)b * p.Sk + t * kBlock + lane, lane < valid, -2);
-    TL::issue(rows_rsrc<D>(kb, p.ks[2], (int64_t)t * kBlock, valid), k_off, wave, kd);
-    TL::issue(rows_rsrc<D>(vb, p.vs[2], (int64_t)t * kBlock, valid), v_off, wave, vd);
+    // (the loaded id as it is: anything computed from it here would wait for the load)
+    if (docs) next_id = p.docs_k[(int64_t)b * p.Sk + t * kBlock + min(lane, valid - 1)];
+    next_valid = valid;
+    TL::issue(ksrc.tile(t, valid), k_off, wave, kd);
+    TL::issue(vsrc.tile(t, valid), v_off, wave, vd);
   };
   auto step = [&](const Step cur, const Step nxt, lds_byte* kt, lds_byte* vt, lds_byte* kn, lds_byte* vn) {
     __builtin_amdgcn_s_waitcnt(0x0F70);
-    const int cur_id = next_id;
+    const int cur_id = lane < next_valid ? doc_or(next_id, -2) : -2;
     if (docs) {
       const uint64_t valid = __ballot(cur_id >= 0);
       if (~valid) { TL::keep(valid, wave, lane, kt); TL::keep(valid, wave, lane, vt); }
@@ -316,30 +326,73 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
       doc_ids[wave][lane] = cur_id;
       __builtin_amdgcn_wave_barrier();
     }
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const int jb = cur.t * kBlock + 32 * mt, j0 = jb + 4 * g;
-      floatx16 s = product32<D, BF>(kt + 32 * mt * (2 * D), rd, qf), w;
-      const floatx16 dp = product32<D, BF>(vt + 32 * mt * (2 * D), rd, df);
-      if (p.k1 != 0.f) cap_scores_grad(p, s, w);
-      if (p.bias_kind != kBiasNone) bias_scores(p, L, j0, s);
+    constexpr bool PIPE = D == 128;
+    typedef Phases<PIPE> PH;
+    constexpr int NK = D / 16, kEl = 16 / NK;      // slices per phase, scores per slice of softmax
+    half8_t ring[3][2];
+    auto fetch = [&](int n) {
+      const int ph = n / NK, i = n % NK, off = 32 * PH::piece(ph) * (2 * D);
+      if (ph < 4 && PH::scores(ph)) {
+        ring[n % 3][0] = lds_frag(kt + off + rd[i]);
+        ring[n % 3][1] = lds_frag(vt + off + rd[i]);
+      } else if (ph < 4) {
+        ring[n % 3][0] = frag_tr<D>(kt + off, i, tr);
+      }
+    };
+    floatx16 s[2] = {zero16(), zero16()}, dp[2] = {zero16(), zero16()}, w[2];
+    half8_t x[2][2], y[2][2];
+    auto softmax = [&](int mt, int r) {
+      float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], p.cc, shift - lse));
+      float d = pr * (dp[mt][r] - delta);
+      off += d;
+      if constexpr (CAP) { d *= w[mt][r]; pr *= w[mt][r]; }
+      x[mt][r >> 3][r & 7] = to_elem<BF>(BF ? d : d * up);
+      y[mt][r >> 3][r & 7] = to_elem<BF>(pr);
+    };
+    auto rule = [&](int mt) {
+      const int j0 = cur.t * kBlock + 32 * mt + 4 * g;
+      if constexpr (CAP) cap_scores_grad(p, s[mt], w[mt]);
+      if (p.bias_kind != kBiasNone) bias_scores<CAP>(p, L, j0, s[mt]);
       if (!cur.full) {
-        limit_scores(L, j0, s);
-        if (docs) doc_scores(L, &doc_ids[wave][32 * mt + 4 * g], s);
+        limit_scores(L, j0, s[mt]);
+        if (docs) doc_scores(L, &doc_ids[wave][32 * mt + 4 * g], s[mt]);
       }
-      half8_t x[2], y[2];
+    };
+    fetch(0);
+    fetch(1);
+    auto phase = [&](auto number) {
+      constexpr int ph = decltype(number)::value, mt = PH::piece(ph);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.cc, shift - lse));
-        s[r] = pr * (dp[r] - delta);
-        off += s[r];
-        if (p.k1 != 0.f) { s[r] *= w[r]; pr *= w[r]; }
-        x[r >> 3][r & 7] = to_elem<BF>(BF ? s[r] : s[r] * up);
-        y[r >> 3][r & 7] = to_elem<BF>(pr);
+      for (int i = 0; i < NK; ++i) {
+        const int n = ph * NK + i;
+        fetch(n + 2);
+        STOF_FENCE();
+        if constexpr (PH::scores(ph)) {
+          s[mt] = mfma32<BF>(ring[n % 3][0], qf[i], s[mt]);
+          dp[mt] = mfma32<BF>(ring[n % 3][1], df[i], dp[mt]);
+        } else {
+          const int s2 = i / (D / 32), dt = i % (D / 32);
+          mac[dt] = mfma32<BF>(ring[n % 3][0], y[mt][s2], mac[dt]);
+          acc[dt] = mfma32<BF>(ring[n % 3][0], x[mt][s2], acc[dt]);
+        }
+        if constexpr (PIPE && (ph == 1 || ph == 2)) {
+#pragma unroll
+          for (int e = 0; e < kEl; ++e) softmax(ph - 1, kEl * i + e);
+        }
+        STOF_FENCE();
       }
-      accumulate32<D, BF>(mac, kt + 32 * mt * (2 * D), tr, y);
-      accumulate32<D, BF>(acc, kt + 32 * mt * (2 * D), tr, x);
-    }
+      if constexpr (PH::scores(ph)) {
+        rule(mt);
+        if constexpr (!PIPE) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) softmax(mt, r);
+        }
+      }
+    };
+    phase(std::integral_constant<int, 0>());
+    phase(std::integral_constant<int, 1>());
+    phase(std::integral_constant<int, 2>());
+    phase(std::integral_constant<int, 3>());
   };
   Step cur = next_step();
   if (cur.t >= 0) issue(cur.t, (lds_byte*)k0, (lds_byte*)v0);
@@ -396,7 +449,7 @@ __global__ __launch_bounds__(256) void score_attn_bwd_table_kernel(const BwdPara
 // the wave's own array; diagonals that clip, and pieces that lie beyond the radius as a whole, are
 // added in two registers per lane.  After each head the waves' arrays are joined and written to the
 // workspace, which a last kernel adds up over batch and key tiles.
-template <int D, bool BF, bool TAB>
+template <int D, bool BF, bool CAP, bool TAB>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;
   typedef TileLoad<D, kBlock, 4> TL;
@@ -407,7 +460,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
   __shared__ int doc_ids[4][kBlock];
   __shared__ __attribute__((aligned(16))) float st_lse[4][kBlock];
   __shared__ __attribute__((aligned(16))) float st_del[4][kBlock];
-  __shared__ float skew[TAB ? 4 : 1][TAB ? 32 * 33 + 32 : 1];
+  __shared__ float skew[TAB ? 4 : 1][TAB ? 32 + 32 * 33 + 32 : 1];
   extern __shared__ float tab[];                // kBiasTable: the head's table, then 2 R + 1 sums per wave
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -538,16 +591,26 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
   float slope = 0.f;
   int next_id = 0;
   floatx2_t next_st = {INFINITY, 0.f};
+  TileSource<D, kBlock> qsrc, dsrc;
+  const floatx2_t* stats = nullptr;
+  int issue_head = -1;
   auto issue = [&](const Step& s, lds_byte* qd, lds_byte* dd) {
-    const int h = hk * p.group + s.head, valid = min(p.Sq - s.t * kBlock, kBlock);
-    if (docs) next_id = doc_at(p.docs_q, (int64_t)b * p.Sq + s.t * kBlock + lane, lane < valid, -1);
-    next_st = bp.stats[((int64_t)b * p.Hq + h) * (64 * nqb) + s.t * kBlock + lane];
-    TL::issue(rows_rsrc<D>(p.q + b * p.qs[0] + h * p.qs[1], p.qs[2], (int64_t)s.t * kBlock, valid), q_off, wave, qd);
-    TL::issue(rows_rsrc<D>(bp.dout + b * bp.dos[0] + h * bp.dos[1], bp.dos[2], (int64_t)s.t * kBlock, valid), d_off, wave, dd);
+    const int valid = min(p.Sq - s.t * kBlock, kBlock);
+    if (s.head != issue_head) {
+      const int h = hk * p.group + s.head;
+      issue_head = s.head;
+      qsrc.set(p.q + b * p.qs[0] + h * p.qs[1], p.qs[2]);
+      dsrc.set(bp.dout + b * bp.dos[0] + h * bp.dos[1], bp.dos[2]);
+      stats = bp.stats + ((int64_t)b * p.Hq + h) * (64 * nqb);
+    }
+    if (docs) next_id = p.docs_q[(int64_t)b * p.Sq + s.t * kBlock + min(lane, valid - 1)];   // (as it is: see the query kernel)
+    next_st = stats[s.t * kBlock + lane];
+    TL::issue(qsrc.tile(s.t, valid), q_off, wave, qd);
+    TL::issue(dsrc.tile(s.t, valid), d_off, wave, dd);
   };
   auto step = [&](const Step cur, const Step nxt, lds_byte* qt, lds_byte* dt_, lds_byte* qn, lds_byte* dn) {
     __builtin_amdgcn_s_waitcnt(0x0F70);
-    const int cur_id = next_id;
+    const int cur_id = doc_or(next_id, -1);      // (rows past the end have no lse)
     const floatx2_t cur_st = next_st;
     // rows without keys: zeros, whatever the tensors hold there
     const uint64_t rows = __ballot(cur_st[0] != INFINITY);
@@ -563,85 +626,127 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
     __syncthreads();
     if (nxt.t >= 0) issue(nxt, qn, dn);
     if (!cur.mine) return;
-    st_lse[wave][lane] = cur_st[0];
+    st_lse[wave][lane] = cur_st[0] - (BF ? 0.f : (float)kPShift);   // fp16: P comes out times 2^kPShift
     st_del[wave][lane] = cur_st[1];
     if (docs && !cur.full) doc_ids[wave][lane] = cur_id;
     __builtin_amdgcn_wave_barrier();
-    const float mul = p.k1 != 0.f ? 1.f : p.c;
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+    constexpr bool PIPE = D == 128 && !TAB;
+    typedef Phases<PIPE> PH;
+    constexpr int NK = D / 16, kEl = 16 / NK;
+    half8_t ring[3][2];
+    auto fetch = [&](int n) {
+      const int ph = n / NK, i = n % NK, off = 32 * PH::piece(ph) * (2 * D);
+      if (ph < 4 && PH::scores(ph)) {
+        ring[n % 3][0] = lds_frag(qt + off + rd[i]);
+        ring[n % 3][1] = lds_frag(dt_ + off + rd[i]);
+      } else if (ph < 4) {
+        ring[n % 3][0] = frag_tr<D>(dt_ + off, i, tr);
+        ring[n % 3][1] = frag_tr<D>(qt + off, i, tr);
+      }
+    };
+    floatx16 s[2] = {zero16(), zero16()}, dp[2] = {zero16(), zero16()}, w[2];
+    half8_t x[2][2], y[2][2];                       // dT and P
+    floatx4 ls, de;
+    auto softmax = [&](int mt, int r) {
+      if (r % 4 == 0) {
+        ls = *reinterpret_cast<const floatx4*>(&st_lse[wave][32 * mt + 2 * r + 4 * g]);
+        de = *reinterpret_cast<const floatx4*>(&st_del[wave][32 * mt + 2 * r + 4 * g]);
+      }
+      const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], p.cc, -ls[r % 4]));
+      y[mt][r >> 3][r & 7] = to_elem<BF>(pr);
+      float d = pr * (dp[mt][r] - de[r % 4]);
+      if constexpr (TAB) s[mt][r] = d;
+      if constexpr (CAP) d *= w[mt][r];
+      x[mt][r >> 3][r & 7] = to_elem<BF>(BF ? d : d * up);
+    };
+    auto rule = [&](int mt) {
+      const float mul = CAP ? 1.f : p.c;
       const int pos0 = first + cur.t * kBlock + 32 * mt + 4 * g;    // position of the lane's score 0; score r: + key_off(r)
-      floatx16 s = product32<D, BF>(qt + 32 * mt * (2 * D), rd, kf), w;
-      floatx16 dp = product32<D, BF>(dt_ + 32 * mt * (2 * D), rd, vf);
-      if (p.k1 != 0.f) cap_scores_grad(p, s, w);
+      if constexpr (CAP) cap_scores_grad(p, s[mt], w[mt]);
       if constexpr (TAB) {
-        const int x = min(max(j - pos0, -p.radius), p.radius + kTabPad);   // distance j - p falls with the row
-        const float* t = tab + (x + p.radius + kTabPad);
+        const int at = min(max(j - pos0, -p.radius), p.radius + kTabPad);   // distance j - p falls with the row
+        const float* t = tab + (at + p.radius + kTabPad);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, t[-key_off(r)]);
+        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], mul, t[-key_off(r)]);
       } else if (p.bias_kind == kBiasSlopes) {
-        const float x = (float)(j - pos0);
+        const float at = (float)(j - pos0);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, -slope * __builtin_fabsf(x - (float)key_off(r)));
+        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], mul, -slope * __builtin_fabsf(at - (float)key_off(r)));
       }
       if (!cur.full) {
         const int rel = from - pos0;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = key_off(r) >= rel ? s[r] : -INFINITY;
-        if (docs) doc_scores(L, &doc_ids[wave][32 * mt + 4 * g], s);
+        for (int r = 0; r < 16; ++r) s[mt][r] = key_off(r) >= rel ? s[mt][r] : -INFINITY;
+        if (docs) doc_scores(L, &doc_ids[wave][32 * mt + 4 * g], s[mt]);
       }
-      half8_t x[2];
+    };
+    // TAB: piece mt's dS (in s) to the sums of the distances
+    auto distances = [&](int mt) {
+      const int d_lo = key0 - (first + cur.t * kBlock + 32 * mt) - 31, d_hi = d_lo + 62;   // distances of the piece
+      if (d_lo >= p.radius || d_hi <= -p.radius) {
+        float t = 0.f;
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const floatx4 ls = *reinterpret_cast<const floatx4*>(&st_lse[wave][32 * mt + 8 * q4 + 4 * g]);
-        const floatx4 de = *reinterpret_cast<const floatx4*>(&st_del[wave][32 * mt + 8 * q4 + 4 * g]);
+        for (int r = 0; r < 16; ++r) t += s[mt][r];
+        if (d_lo >= p.radius) far_hi += t; else far_lo += t;
+      } else {
+        float* sk = skew[wave] + 32;            // [query][key], row pitch 33, room on both sides
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * q4 + e;
-          const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.cc, (BF ? 0.f : (float)kPShift) - ls[e]));
-          x[r >> 3][r & 7] = to_elem<BF>(pr);
-          s[r] = pr * (dp[r] - de[e]);
+        for (int r = 0; r < 16; ++r) sk[(key_off(r) + 4 * g) * 33 + j32] = s[mt][r];
+        __builtin_amdgcn_wave_barrier();
+        int dg = lane - 31;                     // lane l sums the diagonal key - query = l - 31 of the piece
+        asm volatile("" : "+v"(dg));            // (or the 32 predicates below are kept across the walk, in spilled registers)
+        const float* at = sk + dg;
+        float t = 0.f;
+#pragma unroll
+        for (int q = 0; q < 32; ++q) {
+          const float e = at[34 * q];
+          t += (unsigned)(q + dg) < 32u ? e : 0.f;
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (lane < 63) {
+          const int d = d_lo + lane;
+          if (d >= p.radius) far_hi += t;
+          else if (d <= -p.radius) far_lo += t;
+          else sums[d + p.radius] += t;
         }
       }
-      accumulate32<D, BF>(dv, dt_ + 32 * mt * (2 * D), tr, x);
-      if constexpr (TAB) {
-        const int d_lo = key0 - (pos0 - 4 * g) - 31, d_hi = d_lo + 62;   // distances of the piece
-        if (d_lo >= p.radius || d_hi <= -p.radius) {
-          float t = 0.f;
+    };
+    fetch(0);
+    fetch(1);
+    auto phase = [&](auto number) {
+      constexpr int ph = decltype(number)::value, mt = PH::piece(ph);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) t += s[r];
-          if (d_lo >= p.radius) far_hi += t; else far_lo += t;
+      for (int i = 0; i < NK; ++i) {
+        const int n = ph * NK + i;
+        fetch(n + 2);
+        STOF_FENCE();
+        if constexpr (PH::scores(ph)) {
+          s[mt] = mfma32<BF>(ring[n % 3][0], kf[i], s[mt]);
+          dp[mt] = mfma32<BF>(ring[n % 3][1], vf[i], dp[mt]);
         } else {
-          float* sk = skew[wave];                 // [query][key]
+          const int s2 = i / (D / 32), dt = i % (D / 32);
+          dv[dt] = mfma32<BF>(ring[n % 3][0], y[mt][s2], dv[dt]);
+          dk[dt] = mfma32<BF>(ring[n % 3][1], x[mt][s2], dk[dt]);
+        }
+        if constexpr (PIPE && (ph == 1 || ph == 2)) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sk[(key_off(r) + 4 * g) * 33 + j32] = s[r];
-          __builtin_amdgcn_wave_barrier();
-          const int dg = lane - 31;               // lane l sums the diagonal key - query = l - 31 of the piece
-          float t = 0.f;
-#pragma unroll 8
-          for (int y = 0; y < 32; ++y) {
-            const int key = y + dg;
-            const bool in = key >= 0 && key < 32;
-            const float e = sk[y * 33 + (in ? key : 0)];
-            t += in ? e : 0.f;
-          }
-          __builtin_amdgcn_wave_barrier();
-          if (lane < 63) {
-            const int d = d_lo + lane;
-            if (d >= p.radius) far_hi += t;
-            else if (d <= -p.radius) far_lo += t;
-            else sums[d + p.radius] += t;
-          }
+          for (int e = 0; e < kEl; ++e) softmax(ph - 1, kEl * i + e);
+        }
+        STOF_FENCE();
+      }
+      if constexpr (PH::scores(ph)) {
+        rule(mt);
+        if constexpr (!PIPE) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) softmax(mt, r);
+          if constexpr (TAB) distances(mt);
         }
       }
-      if (p.k1 != 0.f) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= w[r];
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r >> 3][r & 7] = to_elem<BF>(BF ? s[r] : s[r] * up);
-      accumulate32<D, BF>(dk, qt + 32 * mt * (2 * D), tr, x);
-    }
+    };
+    phase(std::integral_constant<int, 0>());
+    phase(std::integral_constant<int, 1>());
+    phase(std::integral_constant<int, 2>());
+    phase(std::integral_constant<int, 3>());
   };
   Step cur = next_step();
   if (cur.t >= 0) issue(cur, (lds_byte*)q0, (lds_byte*)d0);
@@ -680,20 +785,23 @@ Layout layout(int B, int Hq, int Hkv, int Sq, int Sk, int radius, int docs) {
   return l;
 }
 
+template <int D, bool BF, bool CAP>
+void launch_main(BwdParams& p, hipStream_t st) {
+  const ScoreParams& s = p.s;
+  const int n_tab = s.bias_kind == kBiasTable ? 2 * s.radius + 1 + 2 * kTabPad : 0;
+  const unsigned gq = 8u * (unsigned)p.q_chunk, gk = 8u * (unsigned)p.k_chunk;
+  score_attn_bwd_q_kernel<D, BF, CAP><<<dim3(gq), dim3(256), (size_t)n_tab * 4, st>>>(p);
+  if (n_tab) score_attn_bwd_k_kernel<D, BF, CAP, true><<<dim3(gk), dim3(256), (size_t)(n_tab + 4 * (2 * s.radius + 1)) * 4, st>>>(p);
+  else score_attn_bwd_k_kernel<D, BF, CAP, false><<<dim3(gk), dim3(256), 0, st>>>(p);
+}
 template <int D, bool BF>
 void launch_bwd(BwdParams& p, hipStream_t st) {
   const ScoreParams& s = p.s;
   const int nq = (s.Sq + 63) / 64, nk = (s.Sk + 63) / 64;
-  const int n_tab = s.bias_kind == kBiasTable ? 2 * s.radius + 1 + 2 * kTabPad : 0;
   score_attn_bwd_prep_kernel<D, BF><<<dim3((unsigned)(s.B * s.Hq * nq + (BF ? 0 : s.B * s.Hkv * nk))), dim3(256), 0, st>>>(p);
-  const unsigned gq = 8u * (unsigned)p.q_chunk, gk = 8u * (unsigned)p.k_chunk;
-  score_attn_bwd_q_kernel<D, BF><<<dim3(gq), dim3(256), (size_t)n_tab * 4, st>>>(p);
-  if (n_tab) {
-    score_attn_bwd_k_kernel<D, BF, true><<<dim3(gk), dim3(256), (size_t)(n_tab + 4 * (2 * s.radius + 1)) * 4, st>>>(p);
+  s.k1 != 0.f ? launch_main<D, BF, true>(p, st) : launch_main<D, BF, false>(p, st);
+  if (s.bias_kind == kBiasTable)
     score_attn_bwd_table_kernel<BF><<<dim3((unsigned)((2 * s.radius + 64) / 64), (unsigned)s.Hq), dim3(256), 0, st>>>(p);
-  } else {
-    score_attn_bwd_k_kernel<D, BF, false><<<dim3(gk), dim3(256), 0, st>>>(p);
-  }
 }
 
 }  // namespace

@@ -125,7 +125,9 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
     }
 }
 
-template <int D, bool BF>
+// CAP is a template argument: with the cap behind a run-time branch the compiler computes it speculatively for every
+// tile (32 transcendental operations of 16 cycles per 64 keys and wave beside the 32 of the softmax).
+template <int D, bool BF, bool CAP>
 __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScoreParams p) {
   typedef TileLoad<D, kBlock, 4> TL;
   __shared__ __attribute__((aligned(1024))) unsigned char k0[TL::kBytes];
@@ -166,8 +168,9 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
     for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const half8_t*>(src + 16 * ks + 8 * g);
   }
 
-  const half_t* kb = p.k + b * p.ks[0] + hk * p.ks[1];
-  const half_t* vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  TileSource<D, kBlock> ksrc, vsrc;
+  ksrc.set(p.k + b * p.ks[0] + hk * p.ks[1], p.ks[2]);
+  vsrc.set(p.v + b * p.vs[0] + hk * p.vs[1], p.vs[2]);
   uint32_t k_off[TL::kN], v_off[TL::kN];
   TL::offsets(k_off, wave, lane, p.ks[2]);
   TL::offsets(v_off, wave, lane, p.vs[2]);
@@ -223,16 +226,18 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   Softmax<D, 2, BF> sm;
   sm.init();
 
-  int next_id = 0;             // document of key `lane` of the tile whose loads are in flight
+  int next_valid = 0, next_id = 0;   // document of key `lane` of the tile whose loads are in flight
   auto issue = [&](int t, lds_byte* kd, lds_byte* vd) {
     const int valid = min(klen - t * kBlock, kBlock);
-    if (docs) next_id = doc_at(p.docs_k, (int64_t)b * p.Sk + t * kBlock + lane, lane < valid, -2);
-    TL::issue(rows_rsrc<D>(kb, p.ks[2], (int64_t)t * kBlock, valid), k_off, wave, kd);
-    TL::issue(rows_rsrc<D>(vb, p.vs[2], (int64_t)t * kBlock, valid), v_off, wave, vd);
+    // (the loaded id as it is: anything computed from it here would wait for the load)
+    if (docs) next_id = p.docs_k[(int64_t)b * p.Sk + t * kBlock + min(lane, valid - 1)];
+    next_valid = valid;
+    TL::issue(ksrc.tile(t, valid), k_off, wave, kd);
+    TL::issue(vsrc.tile(t, valid), v_off, wave, vd);
   };
   auto step = [&](const Step cur, const Step nxt, lds_byte* kt, lds_byte* vt, lds_byte* kn, lds_byte* vn) {
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's share of the tile landed
-    const int cur_id = next_id;
+    const int cur_id = lane < next_valid ? doc_or(next_id, -2) : -2;
     if (docs) {
       // keys of no document: whatever their values are, zeros take their place (0 times NaN is NaN)
       const uint64_t valid = __ballot(cur_id >= 0);
@@ -244,8 +249,8 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
     floatx16 s[2];
     scores_product<D, 2, BF>(kt, rd, qf, s);
     const int j0 = cur.t * kBlock + 4 * g;
-    if (p.k1 != 0.f) { cap_scores(p, s[0]); cap_scores(p, s[1]); }
-    if (p.bias_kind != kBiasNone) { bias_scores(p, L, j0, s[0]); bias_scores(p, L, j0 + 32, s[1]); }
+    if constexpr (CAP) { cap_scores(p, s[0]); cap_scores(p, s[1]); }
+    if (p.bias_kind != kBiasNone) { bias_scores<CAP>(p, L, j0, s[0]); bias_scores<CAP>(p, L, j0 + 32, s[1]); }
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
       limit_scores(L, j0 + 32, s[1]);
@@ -293,7 +298,7 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
 // ---- row form.  Grid: B * Hkv * tiles (32 rows each) * splits.
 constexpr int kRowKeys = 32;
 
-template <int D, bool BF>
+template <int D, bool BF, bool CAP>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(const ScoreParams p) {
   typedef TileLoad<D, kRowKeys, 1> TL;
   // (one object per buffer: the compiler orders LDS reads after in-flight loads per object)
@@ -337,8 +342,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const half8_t*>(src + 16 * ks + 8 * g);
   }
-  const half_t* kb = p.k + b * p.ks[0] + hk * p.ks[1];
-  const half_t* vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  TileSource<D, kRowKeys> ksrc, vsrc;
+  ksrc.set(p.k + b * p.ks[0] + hk * p.ks[1], p.ks[2]);
+  vsrc.set(p.v + b * p.vs[0] + hk * p.vs[1], p.vs[2]);
   uint32_t k_off[TL::kN], v_off[TL::kN];
   TL::offsets(k_off, 0, lane, p.ks[2]);
   TL::offsets(v_off, 0, lane, p.vs[2]);
@@ -390,8 +396,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
   sm.init();
   auto issue = [&](int t, lds_byte* kd, lds_byte* vd) {
     const int valid = min(klen - t * kRowKeys, kRowKeys);
-    TL::issue(rows_rsrc<D>(kb, p.ks[2], (int64_t)t * kRowKeys, valid), k_off, 0, kd);
-    TL::issue(rows_rsrc<D>(vb, p.vs[2], (int64_t)t * kRowKeys, valid), v_off, 0, vd);
+    TL::issue(ksrc.tile(t, valid), k_off, 0, kd);
+    TL::issue(vsrc.tile(t, valid), v_off, 0, vd);
   };
   // one tile: wait for its loads (those of the tile after it stay in flight), use it, request the tile after the next into its buffers
   auto step = [&](const Step cur, bool more, lds_byte* kt, lds_byte* vt) {
@@ -410,8 +416,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
     floatx16 s[1];
     scores_product<D, 1, BF>(kt, rd, qf, s);
     const int j0 = cur.t * kRowKeys + 4 * g;
-    if (p.k1 != 0.f) cap_scores(p, s[0]);
-    if (p.bias_kind != kBiasNone) bias_scores(p, L, j0, s[0]);
+    if constexpr (CAP) cap_scores(p, s[0]);
+    if (p.bias_kind != kBiasNone) bias_scores<CAP>(p, L, j0, s[0]);
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
       if (docs) doc_scores(L, &doc_ids[wave][4 * g], s[0]);
@@ -628,19 +634,23 @@ void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st) {
   doc_ranges_kernel<<<dim3((unsigned)(p.B * (nq + nk))), dim3(64), 0, st>>>(p.docs_q, p.docs_k, dq, dk, p.B, p.Sq, p.Sk);
 }
 
-template <int D, bool BF>
-static void launch_fwd(ScoreParams& p, const Form& f, hipStream_t st) {
+template <int D, bool BF, bool CAP>
+static void launch_form(ScoreParams& p, const Form& f, hipStream_t st) {
   const int n_tab = p.bias_kind == kBiasTable ? 2 * p.radius + 1 + 2 * kTabPad : 0;
   if (f.rows) {
     const unsigned grid = (unsigned)(p.B * p.Hkv) * (unsigned)p.tiles * (unsigned)p.splits;
-    score_attn_rows_kernel<D, BF><<<dim3(grid), dim3(256), (size_t)(p.group * n_tab) * 4, st>>>(p);
-    if (p.splits > 1) {
-      const int64_t n = (int64_t)p.B * p.Hkv * p.Sq * p.group;
-      score_attn_join_kernel<D, BF><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(p);
-    }
+    score_attn_rows_kernel<D, BF, CAP><<<dim3(grid), dim3(256), (size_t)(p.group * n_tab) * 4, st>>>(p);
   } else {
     p.chunk = (p.B * p.Hq * p.tiles + 7) / 8;
-    score_attn_wide_kernel<D, BF><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
+    score_attn_wide_kernel<D, BF, CAP><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
+  }
+}
+template <int D, bool BF>
+static void launch_fwd(ScoreParams& p, const Form& f, hipStream_t st) {
+  p.k1 != 0.f ? launch_form<D, BF, true>(p, f, st) : launch_form<D, BF, false>(p, f, st);
+  if (p.splits > 1) {
+    const int64_t n = (int64_t)p.B * p.Hkv * p.Sq * p.group;
+    score_attn_join_kernel<D, BF><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(p);
   }
 }
 

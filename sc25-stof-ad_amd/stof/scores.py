@@ -226,11 +226,14 @@ class _ScoreAttn(Function):
         ctx.save_for_backward(q, k, v, out, lse, bias, slopes, mask.prefix, mask.kv_len, mask.docs_q, mask.docs_k)
         ctx.rule = (mask, scale, cap, out_layout)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)          # no zeros for lse
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _dlse):
+        if dout is None:
+            return (None,) * 10
         q, k, v, out, lse, bias, slopes = ctx.saved_tensors[:7]
         mask, scale, cap, out_layout = ctx.rule
         if out_layout == "bshd":
