@@ -140,10 +140,9 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
 
-  // XCD x takes a contiguous range of (batch, head, query tile); the tiles with most keys go first
-  const int id = (blockIdx.x & 7) * p.chunk + (blockIdx.x >> 3);
-  if (id >= p.B * p.Hq * p.tiles) return;
-  const int bh = id / p.tiles, tile = p.tiles - 1 - (id - bh * p.tiles);
+  Placed at;
+  if (!place(blockIdx.x, p.B * p.Hq, p.tiles, p.chunk, p.cus_per_xcd, 2, p.causal, at)) return;
+  const int bh = at.head, tile = p.tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
 
   const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
@@ -623,6 +622,8 @@ void score_attn_params(ScoreParams& p, const void* q, const void* k, const void*
   p.c = scale * kLog2e;
   p.k1 = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
   p.capl = cap * kLog2e;
+  int cus = stof_device_compute_units();
+  p.cus_per_xcd = cus >= 8 ? cus / 8 : 32;
   p.cc = (cap > 0.f || p.bias_kind != kBiasNone) ? 1.f : p.c;
 }
 
