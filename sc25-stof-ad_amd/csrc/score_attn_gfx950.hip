@@ -12,7 +12,7 @@
 //    ranges become three 64-bit sets that the walk takes bit by bit.
 //  * row form, for few rows and long keys (single tokens) and for small grids: one workgroup owns 32
 //    rows, row r = (query r / G, head r % G of the G heads that share a key head), so a token's heads
-//    read the cache once; its four waves take every fourth tile of 32 keys through buffers of their own
+//    read the cache once; its eight waves take every eighth tile of 32 keys through a buffer of their own
 //    without barriers, and the keys can be split further over workgroups, joined by a second kernel.
 #include "score_attn.h"
 
@@ -295,18 +295,21 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
 }
 
 // ---- row form.  Grid: B * Hkv * tiles (32 rows each) * splits.
+//
+// Bound: the reading of K and V, or for short caches the chain of dependent loads.  Each wave keeps one K and one V
+// tile of 32 keys: the next K tile is requested as soon as the scores of the current one are formed, the next V
+// tile after the second product, so one of the two is always on its way while the wave computes, and
+// eight waves with 128 KB of requests (head size 128) per compute unit cover the memory's latency.
 constexpr int kRowKeys = 32;
+constexpr int kRowWaves = 8;
 
 template <int D, bool BF, bool CAP>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(const ScoreParams p) {
+__global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(const ScoreParams p) {
   typedef TileLoad<D, kRowKeys, 1> TL;
-  // (one object per buffer: the compiler orders LDS reads after in-flight loads per object)
-  __shared__ __attribute__((aligned(1024))) unsigned char k0[4 * TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) unsigned char k1[4 * TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) unsigned char v0[4 * TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) unsigned char v1[4 * TL::kBytes];
-  __shared__ int doc_ids[4][kRowKeys];
-  __shared__ float stats[4][2][64];
+  __shared__ __attribute__((aligned(1024))) unsigned char k_lds[kRowWaves * TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char v_lds[kRowWaves * TL::kBytes];
+  __shared__ int doc_ids[kRowWaves][kRowKeys];
+  __shared__ float stats[kRowWaves][2][64];
   extern __shared__ float tab[];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -331,7 +334,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
   L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
   L.tab = tab + hg * n_tab;
   if (p.bias_kind == kBiasTable) {
-    for (int x = 0; x < G; ++x) load_table<BF>(p, hk * G + x, tab + x * n_tab, threadIdx.x, 256);
+    for (int x = 0; x < G; ++x) load_table<BF>(p, hk * G + x, tab + x * n_tab, threadIdx.x, 64 * kRowWaves);
     __syncthreads();
   }
 
@@ -356,7 +359,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
     for (int hh = 0; hh < 2; ++hh) tr[dt][hh] = tr_off<D>(lane, dt, hh);
 
   // this wave's stream of tiles: stream + n * streams; lane l decides the (64 w + l)-th of them
-  const int streams = 4 * p.splits, stream = 4 * split + wave;
+  const int streams = kRowWaves * p.splits, stream = kRowWaves * split + wave;
   const int hi = row_limit(p.causal, klen, prefix, first + i_hi), lo = row_limit(p.causal, klen, prefix, first + i_lo);
   const int nqb = (p.Sq + kBlock - 1) / kBlock, nkb = (p.Sk + kBlock - 1) / kBlock;
   DocRange qa = {0, 0, 1, 0}, qb = qa;                    // the at most two blocks that hold these queries
@@ -393,27 +396,34 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
 
   Softmax<D, 1, BF> sm;
   sm.init();
-  auto issue = [&](int t, lds_byte* kd, lds_byte* vd) {
-    const int valid = min(klen - t * kRowKeys, kRowKeys);
-    TL::issue(ksrc.tile(t, valid), k_off, 0, kd);
-    TL::issue(vsrc.tile(t, valid), v_off, 0, vd);
-  };
-  // one tile: wait for its loads (those of the tile after it stay in flight), use it, request the tile after the next into its buffers
-  auto step = [&](const Step cur, bool more, lds_byte* kt, lds_byte* vt) {
-    constexpr int kIn = 2 * TL::kN;       // load instructions of one tile
-    if (more) __builtin_amdgcn_s_waitcnt((kIn & 15) | ((kIn >> 4) << 14) | 0x0F70);
-    else __builtin_amdgcn_s_waitcnt(0x0F70);
+  lds_byte* kt = (lds_byte*)k_lds + wave * TL::kBytes;
+  lds_byte* vt = (lds_byte*)v_lds + wave * TL::kBytes;
+  auto issue_k = [&](int t) { TL::issue(ksrc.tile(t, min(klen - t * kRowKeys, kRowKeys)), k_off, 0, kt); };
+  auto issue_v = [&](int t) { TL::issue(vsrc.tile(t, min(klen - t * kRowKeys, kRowKeys)), v_off, 0, vt); };
+  // every LDS read so far has returned, so loads may overwrite what was read
+  auto drained = [&]() {
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+  };
+  constexpr int kAllButOne = (TL::kN & 15) | ((TL::kN >> 4) << 14) | 0x0F70;   // vmcnt: the loads of one tile may be out
+  Step cur = next_step();
+  if (cur.t >= 0) { issue_k(cur.t); issue_v(cur.t); }
+  while (cur.t >= 0) {
+    const Step nxt = next_step();
+    int id = 0;
     if (docs) {
       const int jj = cur.t * kRowKeys + j32;
-      const int id = doc_at(p.docs_k, (int64_t)b * p.Sk + jj, jj < klen, -2);
-      const uint64_t valid = __ballot(id >= 0);
-      if (~valid) TL::keep(valid, 0, lane, vt);
+      id = doc_at(p.docs_k, (int64_t)b * p.Sk + jj, jj < klen, -2);     // (its wait covers both tiles)
       doc_ids[wave][j32] = id;
       __builtin_amdgcn_wave_barrier();
     }
+    __builtin_amdgcn_s_waitcnt(kAllButOne);       // K has landed (V, requested after it, may be out)
+    asm volatile("" ::: "memory");
     floatx16 s[1];
     scores_product<D, 1, BF>(kt, rd, qf, s);
+    drained();
+    if (nxt.t >= 0) issue_k(nxt.t);
     const int j0 = cur.t * kRowKeys + 4 * g;
     if constexpr (CAP) cap_scores(p, s[0]);
     if (p.bias_kind != kBiasNone) bias_scores<CAP>(p, L, j0, s[0]);
@@ -423,68 +433,57 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
     }
     half8_t pf[1][2];
     sm.step(p.cc, s, pf);
-    sm.accumulate(vt, tr, pf);
-  };
-  // every LDS read of the tile just used has returned, so loads may overwrite it
-  auto drained = [&]() {
+    if (nxt.t >= 0) __builtin_amdgcn_s_waitcnt(kAllButOne);             // V has landed (the next K may be out)
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
-    asm volatile("" ::: "memory");
-  };
-  lds_byte* ka = (lds_byte*)k0 + wave * TL::kBytes; lds_byte* va = (lds_byte*)v0 + wave * TL::kBytes;
-  lds_byte* kz = (lds_byte*)k1 + wave * TL::kBytes; lds_byte* vz = (lds_byte*)v1 + wave * TL::kBytes;
-  Step cur = next_step();
-  Step nxt = cur.t >= 0 ? next_step() : cur;
-  if (cur.t >= 0) issue(cur.t, ka, va);
-  if (nxt.t >= 0) issue(nxt.t, kz, vz);
-  while (cur.t >= 0) {
-    step(cur, nxt.t >= 0, ka, va);
-    Step aft = nxt.t >= 0 ? next_step() : nxt;
-    drained();
-    if (aft.t >= 0) issue(aft.t, ka, va);
-    cur = nxt; nxt = aft;
-    if (cur.t >= 0) {
-      step(cur, nxt.t >= 0, kz, vz);
-      aft = nxt.t >= 0 ? next_step() : nxt;
-      drained();
-      if (aft.t >= 0) issue(aft.t, kz, vz);
-      cur = nxt; nxt = aft;
+    if (docs) {
+      const uint64_t valid = __ballot(id >= 0);
+      if (~valid) TL::keep(valid, 0, lane, vt);
     }
+    sm.accumulate(vt, tr, pf);
+    drained();
+    if (nxt.t >= 0) issue_v(nxt.t);
+    cur = nxt;
   }
 
-  // ---- join the four waves: maxima and sums through `stats`, O (32 x D floats a wave) through the tile
-  // buffers, one object per wave (256 D bytes, half of it used), a quarter of the columns joined by each wave
+  // ---- join the waves: maxima and sums through `stats`, O (32 x D floats a wave) through the tile buffers
+  // (a wave's K and V tiles hold just that: registers below D / 4 in the K tiles, the rest in the V tiles), a
+  // share of the columns joined by each wave
   stats[wave][0][lane] = sm.m;
   stats[wave][1][lane] = sm.l;
   __syncthreads();             // (also: every wave has left the walk)
   float m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][0][lane]);
+  for (int w = 0; w < kRowWaves; ++w) m = fmaxf(m, stats[w][0][lane]);
   float l = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kRowWaves; ++w) {
     const float mw = stats[w][0][lane];
     l += mw == -INFINITY ? 0.f : stats[w][1][lane] * __builtin_amdgcn_exp2f(mw - m);
   }
   // (a NaN maximum does not arise: fmaxf drops NaN; a NaN score makes the sum NaN)
   const float f = sm.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm.m - m);
-  float* acc0 = reinterpret_cast<float*>(k0);
-  float* acc1 = reinterpret_cast<float*>(k1);
-  float* acc2 = reinterpret_cast<float*>(v0);
-  float* acc3 = reinterpret_cast<float*>(v1);
-  float* mine = wave == 0 ? acc0 : wave == 1 ? acc1 : wave == 2 ? acc2 : acc3;
+  constexpr int kRegs = D / 2;                          // registers of O: index 16 dt + x
+  constexpr int kHalf = kRegs / 2;
+  float* klo = reinterpret_cast<float*>(k_lds);
+  float* vhi = reinterpret_cast<float*>(v_lds);
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int x = 0; x < 16; ++x) mine[(16 * dt + x) * 64 + lane] = sm.o[dt][x] * f;
+    for (int x = 0; x < 16; ++x) {
+      const int n = 16 * dt + x;
+      (n < kHalf ? klo : vhi)[wave * (TL::kBytes / 4) + (n % kHalf) * 64 + lane] = sm.o[dt][x] * f;
+    }
   __syncthreads();
   l = pair_sum(l);
-  constexpr int kPer = D / 32 * 16 / 4;                 // register indices per wave
+  constexpr int kPer = kRegs / kRowWaves;               // register indices per wave
   float part[kPer];
+  const float* from = (kPer * wave < kHalf ? klo : vhi) + (kPer * wave % kHalf) * 64 + lane;
 #pragma unroll
   for (int x = 0; x < kPer; ++x) {
-    const int at = (kPer * wave + x) * 64 + lane;
-    part[x] = (acc0[at] + acc1[at]) + (acc2[at] + acc3[at]);
+    part[x] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) part[x] += from[w * (TL::kBytes / 4) + x * 64];
   }
   // register index n = kPer * wave + x of lane (j32, g): row j32, column 32 (n / 16) + 8 ((n % 16) / 4) + 4 g + n % 4
   if (j32 >= rows) return;
@@ -516,34 +515,50 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_rows_kernel(c
   if (p.lse && wave == 0 && g == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Joins the splits of the row form: one wave per row, D / 64 columns per lane, in the order of the splits.
+// Joins the splits of the row form: one workgroup per row, every fourth split to a wave, D / 64 columns per lane; the
+// waves' sums are added in their order.
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int kC = D / 64, kSlot = 32 * D + 64;
+  __shared__ float sums[4][D];
+  __shared__ float factor[64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int n_rows = p.Sq * p.group;
-  const int64_t bk = n / n_rows;
-  const int r = (int)(n - bk * n_rows);
-  if (bk >= (int64_t)p.B * p.Hkv) return;
-  const int tile = r / 32, j = r % 32;
-  const float* base = p.part + (bk * p.tiles + tile) * p.splits * (32 * D + 64);
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, base[s * (32 * D + 64) + 32 * D + j]);
-  float l = 0.f, o[D / 64] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float* q = base + s * (32 * D + 64);
-    const float ms = q[32 * D + j];
-    if (ms == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(ms - m);
-    l += f * q[32 * D + 32 + j];
+  const int64_t bk = blockIdx.x / n_rows;
+  const int r = blockIdx.x - (int)bk * n_rows, tile = r / 32, j = r % 32;
+  const float* base = p.part + (bk * p.tiles + tile) * p.splits * kSlot;
+  // lane s: maximum and sum of split s (at most 64)
+  const float ms = lane < p.splits ? base[lane * kSlot + 32 * D + j] : -INFINITY;
+  const float ls = lane < p.splits ? base[lane * kSlot + 32 * D + 32 + j] : 0.f;
+  float m = ms;
 #pragma unroll
-    for (int x = 0; x < D / 64; ++x) o[x] += f * q[j * D + (D / 64) * lane + x];
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float fs = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+  const float l = wave_sum(fs * ls);
+  factor[lane] = fs;                                    // (every wave the same)
+  __syncthreads();
+  float o[kC] = {};
+#pragma unroll 4
+  for (int s = wave; s < p.splits; s += 4) {
+    const float f = factor[s];
+#pragma unroll
+    for (int x = 0; x < kC; ++x) {
+      const float v = base[s * kSlot + j * D + kC * lane + x];
+      o[x] += f == 0.f ? 0.f : f * v;                   // (a split that saw no key wrote zeros; its maximum is -inf)
+    }
   }
+#pragma unroll
+  for (int x = 0; x < kC; ++x) sums[wave][kC * lane + x] = o[x];
+  __syncthreads();
+  if (wave != 0) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int b = (int)(bk / p.Hkv), hk = (int)(bk - (int64_t)b * p.Hkv), i = r / p.group, h = hk * p.group + r % p.group;
   half_t* orow = p.out + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
 #pragma unroll
-  for (int x = 0; x < D / 64; ++x) orow[(D / 64) * lane + x] = to_elem<BF>(o[x] * inv);
+  for (int x = 0; x < kC; ++x) {
+    const int c = kC * lane + x;
+    orow[c] = to_elem<BF>(((sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c])) * inv);
+  }
   if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
@@ -559,7 +574,7 @@ namespace {
 
 struct Form { bool rows; int tiles, splits; };
 
-inline bool rows_fit(int group, int radius) { return radius < 0 || group * (2 * radius + 1 + 2 * kTabPad) * 4 <= 28 * 1024; }
+inline bool rows_fit(int group, int radius) { return radius < 0 || group * (2 * radius + 1 + 2 * kTabPad) * 4 <= 26 * 1024; }   // (beside 133 KB of tiles)
 
 inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int form) {
   const int group = Hq / Hkv, cus = 256;
@@ -570,13 +585,13 @@ inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius,
   if (!use_rows) return Form{false, (Sq + 127) / 128, 1};
   const int tiles = (int)((rows + 31) / 32);
   const int64_t wgs = (int64_t)B * Hkv * tiles;
-  const int64_t want = D == 64 ? 2 * cus : cus;
+  const int64_t want = 4 * cus;
   const int key_tiles = (Sk + kRowKeys - 1) / kRowKeys;
   int64_t splits = (want + wgs - 1) / wgs;
-  const int most = (key_tiles + 15) / 16;
+  const int most = (key_tiles + 2 * kRowWaves - 1) / (2 * kRowWaves);      // two tiles per wave
   if (splits > most) splits = most;
+  if (splits > 64) splits = 64;                                            // one lane each in the join
   if (splits < 1) splits = 1;
-  if (wgs >= want) splits = 1;
   return Form{true, tiles, (int)splits};
 }
 
@@ -640,7 +655,7 @@ static void launch_form(ScoreParams& p, const Form& f, hipStream_t st) {
   const int n_tab = p.bias_kind == kBiasTable ? 2 * p.radius + 1 + 2 * kTabPad : 0;
   if (f.rows) {
     const unsigned grid = (unsigned)(p.B * p.Hkv) * (unsigned)p.tiles * (unsigned)p.splits;
-    score_attn_rows_kernel<D, BF, CAP><<<dim3(grid), dim3(256), (size_t)(p.group * n_tab) * 4, st>>>(p);
+    score_attn_rows_kernel<D, BF, CAP><<<dim3(grid), dim3(64 * kRowWaves), (size_t)(p.group * n_tab) * 4, st>>>(p);
   } else {
     p.chunk = (p.B * p.Hq * p.tiles + 7) / 8;
     score_attn_wide_kernel<D, BF, CAP><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
@@ -651,7 +666,7 @@ static void launch_fwd(ScoreParams& p, const Form& f, hipStream_t st) {
   p.k1 != 0.f ? launch_form<D, BF, true>(p, f, st) : launch_form<D, BF, false>(p, f, st);
   if (p.splits > 1) {
     const int64_t n = (int64_t)p.B * p.Hkv * p.Sq * p.group;
-    score_attn_join_kernel<D, BF><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(p);
+    score_attn_join_kernel<D, BF><<<dim3((unsigned)n), dim3(256), 0, st>>>(p);
   }
 }
 
