@@ -13,7 +13,9 @@
 //
 // Large products use the tile form of the 16-bit GEMM (C^T = W X^T, both operands K-contiguous through LDS
 // rows of 128 bytes): a row of 128 bytes now holds 128 of K, so the loads, LDS reads and MFMAs of a tile
-// are those of the 16-bit kernel and do twice the arithmetic.  A few tokens use the token form: weights
+// are those of the 16-bit kernel and do twice the arithmetic.  Bound at long K by the LDS reads beside the MFMAs
+// (8192^3: 2.25 POP/s, a library's product 2.08), at K ~ 1024 by what a tile pays beside its products: scales and
+// bias are therefore requested ahead of the operands and wait in LDS for the epilogue (8192 x 1024 -> 4096 60 -> 53 us).  A few tokens use the token form: weights
 // go straight to registers, each exactly once, and every workgroup quantises the tokens itself, so a
 // single-token projection is one launch.
 #include "gemm_tile.h"
@@ -80,19 +82,39 @@ __device__ __forceinline__ unsigned wave_max_u(unsigned m) {
   return m;
 }
 
-// One wave per row, 8 values per lane and pass; the second reading of the row comes from the caches.
-template <bool BF>
+// One wave per row, 8 values per lane and chunk of 512.  Rows of up to NV chunks stay in registers between the search
+// for the maximum and the rounding; longer ones (NV = 0) are read again, from the caches.
+template <bool BF, int NV>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const half_t* x, int8_t* xq, float* sx, int M, int K, int64_t ldx, int64_t ldq) {
   const int lane = threadIdx.x & 63;
   const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= M) return;
   const half_t* row = x + m * ldx;
+  int8_t* out = xq + m * ldq;
   unsigned top = 0;
-  for (int k = 8 * lane; k < K; k += 512) top = max_pattern(*reinterpret_cast<const half8_t*>(row + k), top);
-  const RowQuant<BF> q(wave_max_u(top));
-  for (int k = 8 * lane; k < K; k += 512)
-    *reinterpret_cast<uint64_t*>(xq + m * ldq + k) = q.pack(*reinterpret_cast<const half8_t*>(row + k));
-  if (lane == 0) sx[m] = q.scale;
+  if constexpr (NV > 0) {
+    half8_t v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = 512 * i + 8 * lane;
+      const half8_t z = {};
+      v[i] = k < K ? *reinterpret_cast<const half8_t*>(row + k) : z;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) top = max_pattern(v[i], top);
+    const RowQuant<BF> q(wave_max_u(top));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = 512 * i + 8 * lane;
+      if (k < K) *reinterpret_cast<uint64_t*>(out + k) = q.pack(v[i]);
+    }
+    if (lane == 0) sx[m] = q.scale;
+  } else {
+    for (int k = 8 * lane; k < K; k += 512) top = max_pattern(*reinterpret_cast<const half8_t*>(row + k), top);
+    const RowQuant<BF> q(wave_max_u(top));
+    for (int k = 8 * lane; k < K; k += 512) *reinterpret_cast<uint64_t*>(out + k) = q.pack(*reinterpret_cast<const half8_t*>(row + k));
+    if (lane == 0) sx[m] = q.scale;
+  }
 }
 
 __device__ __forceinline__ intx16 mfma_i8(int4_t a, int4_t b, intx16 c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
@@ -100,25 +122,40 @@ __device__ __forceinline__ int4_t lds_frag_i8(const lds_byte* tile, int off) {
   return *reinterpret_cast<const __attribute__((address_space(3))) int4_t*>(tile + off);
 }
 
-// ---- tile form: T x T output tile, 4 waves as 2 x 2, each T/2 tokens x T/2 features; K tiles of 128, double buffered.
+// ---- tile form: T x T output tile, WM x WN waves, each T/WM tokens x T/WN features; K tiles of 128 through ST buffers.
+// KG > 1: KG groups of WM x WN waves take every KG-th K tile each, through buffers of their own, and their integer
+// sums are added at the end (exact, so their order does not matter).
 constexpr int kI8K = 128;
 
-template <int ACT, bool BF, int T>
-__global__ __launch_bounds__(256, 2) void gemm_i8_kernel(const I8Params p) {
+template <int ACT, bool BF, int T, int WM, int WN, int ST, int KG, int OCC>
+__global__ __launch_bounds__(64 * WM * WN * KG, OCC) void gemm_i8_kernel(const I8Params p) {
   constexpr int kTile = T * kI8K;
-  constexpr int kLoads = T / 32;            // load instructions per wave and operand tile (8 rows each)
-  constexpr int kMT = T / 64;               // 32-wide MFMA tiles per wave and direction
-  __shared__ __attribute__((aligned(1024))) unsigned char a0[kTile];
-  __shared__ __attribute__((aligned(1024))) unsigned char a1[kTile];
-  __shared__ __attribute__((aligned(1024))) unsigned char w0[kTile];
-  __shared__ __attribute__((aligned(1024))) unsigned char w1[kTile];
+  constexpr int kLoads = T / 8 / (WM * WN); // load instructions per wave and operand tile (8 rows each)
+  constexpr int kTok = T / WM / 32, kFeat = T / WN / 32;   // 32-wide MFMA tiles per wave and direction
+  __shared__ __attribute__((aligned(1024))) unsigned char a0_all[KG * kTile];
+  __shared__ __attribute__((aligned(1024))) unsigned char w0_all[KG * kTile];
+  __shared__ __attribute__((aligned(1024))) unsigned char a1_all[ST == 2 ? KG * kTile : 16];
+  __shared__ __attribute__((aligned(1024))) unsigned char w1_all[ST == 2 ? KG * kTile : 16];
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / (64 * WM * WN)));
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) % (WM * WN));
+  lds_byte* a0 = (lds_byte*)a0_all + group * kTile; lds_byte* w0 = (lds_byte*)w0_all + group * kTile;
+  lds_byte* a1 = (lds_byte*)a1_all + (ST == 2 ? group * kTile : 0); lds_byte* w1 = (lds_byte*)w1_all + (ST == 2 ? group * kTile : 0);
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
+  __shared__ __attribute__((aligned(16))) float sx_lds[T], sw_lds[T], b_lds[T];
   int tm, tn;
-  if (!raster_tile((int)blockIdx.x, p.tiles_m, p.tiles_n, tm, tn)) return;
+  if (p.tiles_m < 8) {                      // (the raster gives token tile tm to XCD tm % 8: fewer would leave XCDs empty)
+    tn = blockIdx.x / p.tiles_m;
+    tm = blockIdx.x - tn * p.tiles_m;
+  } else if (!raster_tile((int)blockIdx.x, p.tiles_m, p.tiles_n, tm, tn)) {
+    return;
+  }
   const int m0 = tm * T, n0 = tn * T;
+  // the epilogue's scales and bias: requested ahead of the operands, into LDS once the products are done
+  const int et = threadIdx.x % T;
+  const float e_sx = p.sx[min(m0 + et, p.M - 1)], e_sw = p.sw[min(n0 + et, p.N - 1)];
+  const float e_b = p.bias ? from_elem<BF>(p.bias[min(n0 + et, p.N - 1)]) : 0.f;
 
   // rows past the edge re-read the last row; in the last K tile, chunks past K lie beyond the resource's
   // extent and arrive as zeros
@@ -153,21 +190,21 @@ __global__ __launch_bounds__(256, 2) void gemm_i8_kernel(const I8Params p) {
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) rd[ks] = j32 * kI8K + (((2 * ks + g) ^ swz(j32)) << 4);
 
-  intx16 acc[kMT][kMT];                     // [feature tile][token tile]
+  intx16 acc[kFeat][kTok];                  // [feature tile][token tile]
 #pragma unroll
-  for (int i = 0; i < kMT; ++i)
+  for (int i = 0; i < kFeat; ++i)
 #pragma unroll
-    for (int j = 0; j < kMT; ++j)
+    for (int j = 0; j < kTok; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
   auto compute = [&](const lds_byte* at, const lds_byte* wt) {
-    int4_t xa[2][kMT], wb[2][kMT];
+    int4_t xa[2][kTok], wb[2][kFeat];
     auto fetch = [&](int ks, int set) {
 #pragma unroll
-      for (int i = 0; i < kMT; ++i) xa[set][i] = lds_frag_i8(at, (T / 2 * wm + 32 * i) * kI8K + rd[ks]);
+      for (int i = 0; i < kTok; ++i) xa[set][i] = lds_frag_i8(at, (T / WM * wm + 32 * i) * kI8K + rd[ks]);
 #pragma unroll
-      for (int i = 0; i < kMT; ++i) wb[set][i] = lds_frag_i8(wt, (T / 2 * wn + 32 * i) * kI8K + rd[ks]);
+      for (int i = 0; i < kFeat; ++i) wb[set][i] = lds_frag_i8(wt, (T / WN * wn + 32 * i) * kI8K + rd[ks]);
     };
     fetch(0, 0);
 #pragma unroll
@@ -175,61 +212,78 @@ __global__ __launch_bounds__(256, 2) void gemm_i8_kernel(const I8Params p) {
       if (ks + 1 < 4) fetch(ks + 1, (ks + 1) & 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ni = 0; ni < kMT; ++ni)
+      for (int ni = 0; ni < kFeat; ++ni)
 #pragma unroll
-        for (int mi = 0; mi < kMT; ++mi) acc[ni][mi] = mfma_i8(wb[ks & 1][ni], xa[ks & 1][mi], acc[ni][mi]);
+        for (int mi = 0; mi < kTok; ++mi) acc[ni][mi] = mfma_i8(wb[ks & 1][ni], xa[ks & 1][mi], acc[ni][mi]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const int nk = (p.K + kI8K - 1) / kI8K;
-  issue(0, (lds_byte*)a0, (lds_byte*)w0);
-  for (int kt = 0; kt < nk; kt += 2) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0): this wave's share of tile kt landed
-    __syncthreads();
-    if (kt + 1 < nk) issue(kt + 1, (lds_byte*)a1, (lds_byte*)w1);
-    compute((const lds_byte*)a0, (const lds_byte*)w0);
-    if (kt + 1 < nk) {
+  // group's K tiles: group, group + KG, ...; every group passes every barrier
+  const int nk = (p.K + kI8K - 1) / kI8K, steps = (nk + KG - 1) / KG;
+  auto tile = [&](int i) { return i * KG + group; };
+  if (tile(0) < nk) issue(tile(0), a0, w0);
+  if constexpr (ST == 1) {
+    for (int i = 0; i < steps; ++i) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0): this wave's share of the tile landed
+      __syncthreads();
+      if (tile(i) < nk) compute(a0, w0);
+      __syncthreads();
+      if (i + 1 < steps && tile(i + 1) < nk) issue(tile(i + 1), a0, w0);
+    }
+  } else {
+    for (int i = 0; i < steps; i += 2) {
       __builtin_amdgcn_s_waitcnt(0x0F70);
       __syncthreads();
-      if (kt + 2 < nk) issue(kt + 2, (lds_byte*)a0, (lds_byte*)w0);
-      compute((const lds_byte*)a1, (const lds_byte*)w1);
-    }
-  }
-  __syncthreads();                          // every wave is done with the operand tiles
-
-  // epilogue: 32 tokens x (T / 2) features at a time through the wave's own LDS rows (kMT * 64 bytes, 16-byte chunks
-  // XOR-ed by the row) and out in whole rows
-  constexpr int kRow = kMT * 64, kC = kRow / 16;
-  lds_byte* stage = (lds_byte*)a0 + wave * (32 * kRow);
-  const int m_base = m0 + T / 2 * wm, n_base = n0 + T / 2 * wn;
-  const __amdgpu_buffer_rsrc_t o_rs = stof_wave_rsrc(p.out + (int64_t)m_base * p.ldo + n_base);
-  floatx4 sw[kMT][4], bv[kMT][4];
-#pragma unroll
-  for (int ni = 0; ni < kMT; ++ni)
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const int n = n_base + 32 * ni + 8 * q4 + 4 * g;
-      sw[ni][q4] = bv[ni][q4] = floatx4{0.f, 0.f, 0.f, 0.f};
-      if (n < p.N) {                        // N % 8 == 0: four features are inside or outside together
-        sw[ni][q4] = *reinterpret_cast<const floatx4*>(p.sw + n);
-        if (p.bias) {
-          const half4_t b4 = *reinterpret_cast<const half4_t*>(p.bias + n);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { const half_t be = b4[e]; bv[ni][q4][e] = from_elem<BF>(be); }
-        }
+      if (tile(i + 1) < nk) issue(tile(i + 1), a1, w1);
+      if (tile(i) < nk) compute(a0, w0);
+      if (i + 1 < steps) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        __syncthreads();
+        if (tile(i + 2) < nk) issue(tile(i + 2), a0, w0);
+        if (tile(i + 1) < nk) compute(a1, w1);
       }
     }
+  }
+  if ((int)threadIdx.x < T) { sx_lds[et] = e_sx; sw_lds[et] = e_sw; b_lds[et] = e_b; }
+  __syncthreads();                          // every wave is done with the operand tiles
+  if constexpr (KG > 1) {
+    // the other groups' sums to group 0, T T / (64 WM WN) integers per lane through the operand tiles
+    constexpr int kInts = kFeat * kTok * 16;
+    static_assert(64 * WM * WN * kInts * 4 <= 2 * kTile, "a group's sums fit its two operand buffers");
 #pragma unroll
-  for (int mi = 0; mi < kMT; ++mi) {
-    const float sx = p.sx[min(m_base + 32 * mi + j32, p.M - 1)];
+    for (int n = 0; n < kInts; ++n) {
+      lds_byte* at = ((n < kInts / 2) ? a0 : w0) + ((n % (kInts / 2)) * (WM * WN) + wave) * 256 + 4 * lane;
+      if (group > 0) *reinterpret_cast<__attribute__((address_space(3))) int*>(at) = acc[n / (16 * kTok)][(n / 16) % kTok][n % 16];
+    }
+    __syncthreads();
+    if (group > 0) return;
 #pragma unroll
-    for (int ni = 0; ni < kMT; ++ni)
+    for (int n = 0; n < kInts; ++n)
+#pragma unroll
+      for (int o = 1; o < KG; ++o)
+        acc[n / (16 * kTok)][(n / 16) % kTok][n % 16] += *reinterpret_cast<const __attribute__((address_space(3))) int*>(
+            ((n < kInts / 2) ? a0 : w0) + o * kTile + ((n % (kInts / 2)) * (WM * WN) + wave) * 256 + 4 * lane);
+  }
+
+  // epilogue: 32 tokens x (T / WN) features at a time through the wave's own LDS rows (kFeat * 64 bytes, 16-byte chunks
+  // XOR-ed by the row) and out in whole rows
+  constexpr int kRow = kFeat * 64, kC = kRow / 16;
+  lds_byte* stage = a0 + wave * (32 * kRow);   // (group 0's own)
+  const int m_base = m0 + T / WM * wm, n_base = n0 + T / WN * wn;
+  const __amdgpu_buffer_rsrc_t o_rs = stof_wave_rsrc(p.out + (int64_t)m_base * p.ldo + n_base);
+#pragma unroll
+  for (int mi = 0; mi < kTok; ++mi) {
+    const float sx = sx_lds[T / WM * wm + 32 * mi + j32];
+#pragma unroll
+    for (int ni = 0; ni < kFeat; ++ni)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
+        const int n = T / WN * wn + 32 * ni + 8 * q4 + 4 * g;
+        const floatx4 sw = *reinterpret_cast<const floatx4*>(sw_lds + n), bv = *reinterpret_cast<const floatx4*>(b_lds + n);
         half4_t o;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          o[e] = to_elem<BF>(act_i8<ACT>(__builtin_fmaf((float)acc[ni][mi][4 * q4 + e], sx * sw[ni][q4][e], bv[ni][q4][e])));
+          o[e] = to_elem<BF>(act_i8<ACT>(__builtin_fmaf((float)acc[ni][mi][4 * q4 + e], sx * sw[e], bv[e])));
         *reinterpret_cast<__attribute__((address_space(3))) half4_t*>(stage + j32 * kRow + (((4 * ni + q4) ^ (j32 & (kC - 1))) << 4) + 8 * g) = o;
       }
 #pragma unroll
@@ -317,17 +371,37 @@ __global__ __launch_bounds__(256) void linear_i8_token_kernel(const I8Params p) 
 bool token_form(int64_t M, int64_t K) { return M <= kTokMax && M * ((K + 63) / 64 * 64) <= kTokLds; }
 int64_t padded(int64_t K) { return (K + 15) / 16 * 16; }
 
-// T = 128 while its tiles fill the device; else 64, four times the workgroups
-int tile_edge(int64_t M, int64_t N) { return ((M + 127) / 128) * ((N + 127) / 128) >= 256 ? 128 : 64; }
+// Which tile form, by the number of tiles and the length of K (us, form taken | its neighbour):
+//  * 128 x 128 tiles that leave half the device empty -> 64 x 64, and with few of those and a long K four groups of
+//    waves along K: 777 x 768 -> 2304 7.6 | 9.1 (128), 512 x 4096 -> 1024 12.3 | 18.3 (64 without groups),
+//    100 x 4096 -> 4096 11.6 | 17.5, 2048 x 4096 -> 1024 (512 tiles of 64) 19.9 | 23.3 (groups), K 1024 even;
+//  * 256 x 256 (0.75 KB of LDS reads per MFMA instead of 1 KB, one workgroup per unit) needs every unit busy and a K
+//    that outweighs its unoverlapped epilogue: 8192^3 489 | 530, 4096^3 66.6 | 72.4, 8192 x 1024 -> 4096 50 | 46;
+//  * 128 x 128 with two buffers while all tiles are resident (two per unit): 8192 x 4096 -> 1024 38 | 46; with one
+//    buffer, four workgroups per unit whose epilogues and products overlap, beyond: 8192 x 1024 -> 4096 46 | 53,
+//    65536 x 1024 -> 1024 94 | 103.
+enum { kTile64, kTile64Groups, kTile128, kTile128Single, kTile256 };
+int tile_form(int64_t M, int64_t N, int64_t K) {
+  const int64_t t64 = ((M + 63) / 64) * ((N + 63) / 64), t128 = ((M + 127) / 128) * ((N + 127) / 128), t256 = ((M + 255) / 256) * ((N + 255) / 256);
+  if (t128 < 256) return t64 <= 256 && K >= 2048 ? kTile64Groups : kTile64;
+  if (K >= 2048 && t256 >= 256) return kTile256;
+  return t128 <= 512 ? kTile128 : kTile128Single;
+}
 
 template <int ACT, bool BF>
 void launch_gemm(I8Params& p, hipStream_t st) {
-  const int T = tile_edge(p.M, p.N);
+  const int form = tile_form(p.M, p.N, p.K);
+  const int T = form == kTile256 ? 256 : form >= kTile128 ? 128 : 64;
   p.tiles_m = (p.M + T - 1) / T;
   p.tiles_n = (p.N + T - 1) / T;
-  const unsigned grid = raster_grid(p.tiles_m, p.tiles_n);
-  if (T == 128) gemm_i8_kernel<ACT, BF, 128><<<dim3(grid), dim3(256), 0, st>>>(p);
-  else gemm_i8_kernel<ACT, BF, 64><<<dim3(grid), dim3(256), 0, st>>>(p);
+  const dim3 grid(p.tiles_m < 8 ? (unsigned)(p.tiles_m * p.tiles_n) : raster_grid(p.tiles_m, p.tiles_n));
+  switch (form) {
+    case kTile64: gemm_i8_kernel<ACT, BF, 64, 2, 2, 2, 1, 4><<<grid, dim3(256), 0, st>>>(p); break;
+    case kTile64Groups: gemm_i8_kernel<ACT, BF, 64, 2, 2, 2, 4, 1><<<grid, dim3(1024), 0, st>>>(p); break;
+    case kTile128: gemm_i8_kernel<ACT, BF, 128, 2, 2, 2, 1, 2><<<grid, dim3(256), 0, st>>>(p); break;
+    case kTile128Single: gemm_i8_kernel<ACT, BF, 128, 2, 2, 1, 1, 4><<<grid, dim3(256), 0, st>>>(p); break;
+    default: gemm_i8_kernel<ACT, BF, 256, 2, 4, 2, 1, 1><<<grid, dim3(512), 0, st>>>(p); break;
+  }
 }
 template <int ACT, bool BF>
 void launch_token(I8Params& p, hipStream_t st) {
@@ -343,10 +417,16 @@ void launch_act(I8Params& p, int act, bool token, hipStream_t st) {
     default: token ? launch_token<STOF_ACT_RELU, BF>(p, st) : launch_gemm<STOF_ACT_RELU, BF>(p, st); break;
   }
 }
+template <bool BF>
+void launch_quantize_nv(const half_t* x, int8_t* xq, float* sx, int M, int K, int64_t ldx, int64_t ldq, hipStream_t st) {
+  const dim3 grid((unsigned)((M + 3) / 4)), block(256);
+  if (K <= 1024) quantize_rows_kernel<BF, 2><<<grid, block, 0, st>>>(x, xq, sx, M, K, ldx, ldq);
+  else if (K <= 4096) quantize_rows_kernel<BF, 8><<<grid, block, 0, st>>>(x, xq, sx, M, K, ldx, ldq);
+  else quantize_rows_kernel<BF, 0><<<grid, block, 0, st>>>(x, xq, sx, M, K, ldx, ldq);
+}
 void launch_quantize(const void* x, int8_t* xq, float* sx, int M, int K, int64_t ldx, int64_t ldq, int dtype, hipStream_t st) {
-  const dim3 grid((unsigned)((M + 3) / 4));
-  if (dtype == STOF_DTYPE_BF16) quantize_rows_kernel<true><<<grid, dim3(256), 0, st>>>((const half_t*)x, xq, sx, M, K, ldx, ldq);
-  else quantize_rows_kernel<false><<<grid, dim3(256), 0, st>>>((const half_t*)x, xq, sx, M, K, ldx, ldq);
+  if (dtype == STOF_DTYPE_BF16) launch_quantize_nv<true>((const half_t*)x, xq, sx, M, K, ldx, ldq, st);
+  else launch_quantize_nv<false>((const half_t*)x, xq, sx, M, K, ldx, ldq, st);
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K, int dtype) {

@@ -122,8 +122,9 @@ def test_linear_and_product(M, N, K, dtype, act, bias):
     _close(gemm_i8(q, s, w.cuda(), ws.cuda(), cu(b), act=act, dtype=dt), want, "gemm_i8")
 
 
-def test_tile_edge_of_128():
-    M, N, K = 2048, 2056, 272
+@pytest.mark.parametrize("M,N,K", [(2048, 2056, 272), (2300, 4104, 144), (200, 264, 2064), (4096, 4104, 2064), (40, 8, 4096)])
+def test_every_tile_form_at_its_edges(M, N, K):
+    """128 x 128 tiles with two buffers and with one, 64 x 64 with groups along K, 256 x 256: sizes that end inside a tile."""
     x = torch.randn(M, K, generator=_gen(1)).half()
     w, ws, b = _weights(N, K, torch.float16, 2)
     _close(linear_i8(x.cuda(), w.cuda(), ws.cuda(), b.cuda()), _want(*_quant64(x), w, ws, b, "none", torch.float16))
