@@ -22,7 +22,9 @@ __all__ = ["quantize_rows_i8", "gemm_i8", "linear_i8"]
 
 def _call(dev, fn, what, *args):
     if dev.index == torch.cuda.current_device():
-        check(fn(*args), what)
+        rc = fn(*args)
+        if rc:
+            check(rc, what)
     else:
         with torch.cuda.device(dev):
             check(fn(*args), what)
@@ -123,7 +125,8 @@ def linear_i8(x, wq, w_scale, bias=None, act="none", out=None):
     N, ldw = _weights(wq, w_scale, bias, K, x.device, x.dtype, act)
     x2, ldx = _rows2d("x", x, 8)
     M = x2.shape[0]
-    y = _output(out, x.shape[:-1] + (N,), x.dtype, x.device)
+    shape = (M, N) if x.dim() == 2 else x.shape[:-1] + (N,)
+    y = x.new_empty(shape) if out is None else _output(out, shape, x.dtype, x.device)
     if M:
         lib = _lib.lib()
         nbytes = lib.stof_linear_i8_workspace_bytes(M, K)

@@ -24,7 +24,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import StofError, check
-from .ops import _DTYPES, _ptr, _require, _stream
+from .ops import _DTYPES, _require, _stream
 
 __all__ = ["ScoreMask", "score_attn", "score_attn_backward", "MAX_RADIUS"]
 
@@ -53,35 +53,43 @@ class ScoreMask:
 
     def __init__(self, causal=False, prefix=None, kv_len=None, docs=None, q_start=None):
         for name, t in (("prefix", prefix), ("kv_len", kv_len)):
-            _require(t is None or (torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()),
-                     f"{name} must be a contiguous int32 tensor [B]")
+            if t is not None:
+                _require(torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(),
+                         f"{name} must be a contiguous int32 tensor [B]")
         _require(prefix is None or causal, "a prefix opens keys that a causal rule closes: it needs causal=True")
-        dq, dk = docs if isinstance(docs, (tuple, list)) else (docs, docs)
-        for t in (dq, dk):
-            _require(docs is None or (torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 2 and t.is_contiguous()),
-                     "docs must be a contiguous int32 tensor [B,S] or a pair of them")
-        _require(q_start is None or q_start == "end" or (type(q_start) is int and abs(q_start) <= 1 << 29),
-                 f"q_start must be None, an int or 'end', got {q_start!r}")
-        _require(q_start != "end" or kv_len is not None, "q_start='end' needs kv_len")
-        self.causal, self.prefix, self.kv_len, self.q_start = bool(causal), prefix, kv_len, q_start
+        dq = dk = None
+        if docs is not None:
+            dq, dk = docs if isinstance(docs, (tuple, list)) else (docs, docs)
+            for t in (dq, dk):
+                _require(torch.is_tensor(t) and t.dtype == torch.int32 and t.dim() == 2 and t.is_contiguous(),
+                         "docs must be a contiguous int32 tensor [B,S] or a pair of them")
+        if q_start is not None:
+            _require(q_start == "end" or (type(q_start) is int and abs(q_start) <= 1 << 29), "q_start must be None, an int or 'end'")
+            _require(q_start != "end" or kv_len is not None, "q_start='end' needs kv_len")
+        self.causal, self.prefix, self.kv_len, self.q_start = 1 if causal else 0, prefix, kv_len, q_start
         self.docs_q, self.docs_k = dq, dk
 
     def _check(self, B, Sq, Sk, dev):
-        for name, t, shape in (("prefix", self.prefix, (B,)), ("kv_len", self.kv_len, (B,)),
-                               ("docs", self.docs_q, (B, Sq)), ("docs", self.docs_k, (B, Sk))):
-            if t is not None and (t.shape != shape or t.device != dev):
+        def fits(name, t, *shape):
+            if t.shape != shape or t.device != dev:
                 raise StofError(f"{name} must be {list(shape)} on q's device, got {list(t.shape)} on {t.device}")
+        if self.prefix is not None:
+            fits("prefix", self.prefix, B)
+        if self.kv_len is not None:
+            fits("kv_len", self.kv_len, B)
+        if self.docs_q is not None:
+            fits("docs", self.docs_q, B, Sq)
+            fits("docs", self.docs_k, B, Sk)
 
 
 _NO_MASK = ScoreMask()
 
 
-def _checked(q, k, v, mask, cap, scale, bias, slopes):
-    """The argument checks of forward and backward; the rule's numbers as the C ABI takes them."""
+def _refuse(q, k, v, mask, scale, cap, bias, slopes):
+    """The refusal of a call that ``_rule`` found wanting, by name."""
     if not q.is_cuda:
         raise StofError("q must be a CUDA tensor (this path has no CPU implementation)")
-    dt = _DTYPES.get(q.dtype)
-    if dt is None:
+    if q.dtype not in _DTYPES:
         raise StofError(f"q must be float16 or bfloat16, got {q.dtype}")
     dev = q.device
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -97,57 +105,87 @@ def _checked(q, k, v, mask, cap, scale, bias, slopes):
         raise StofError(f"the number of query heads ({Hq}) must be a multiple of the number of key heads ({Hkv})")
     if D not in (64, 128):
         raise StofError(f"head size must be 64 or 128, got {D}")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise StofError(f"scale must be positive, got {scale}")
-    cap = 0.0 if cap is None else float(cap)
     if cap != 0.0 and not 1e-30 < cap < 1e30:
         raise StofError(f"cap must be positive, got {cap}")
-    radius = -1
+    if bias is not None and slopes is not None:
+        raise StofError("bias and slopes exclude each other")
     if bias is not None:
-        if slopes is not None:
-            raise StofError("bias and slopes exclude each other")
         if not (bias.dim() == 2 and bias.shape[0] == Hq and bias.shape[1] % 2 == 1 and bias.is_contiguous()
                 and bias.dtype == q.dtype and bias.device == dev):
             raise StofError(f"bias must be a contiguous [{Hq}, 2 R + 1] tensor of q's dtype and device")
-        radius = bias.shape[1] // 2
-        if radius > MAX_RADIUS:
-            raise StofError(f"bias must tell apart at most {MAX_RADIUS} distances to each side, got {radius}")
-    elif slopes is not None:
+        raise StofError(f"bias must tell apart at most {MAX_RADIUS} distances to each side, got {bias.shape[1] // 2}")
+    if slopes is not None:
         if not (slopes.shape == (Hq,) and slopes.dtype == torch.float32 and slopes.is_contiguous() and slopes.device == dev):
             raise StofError(f"slopes must be a contiguous float32 [{Hq}] tensor on q's device")
-        if slopes.requires_grad:
-            raise StofError("slopes are constants of the rule: there is no gradient for them")
-    mask._check(B, Sq, Sk, dev)
-    q_end = 1 if mask.q_start == "end" else 0
-    q_start = 0 if q_end else (Sk - Sq if mask.q_start is None else mask.q_start)
-    return dt, scale, cap, radius, q_start, q_end
+        raise StofError("slopes are constants of the rule: there is no gradient for them")
+    raise StofError("these tensors cannot be used together")
 
 
-def _forward(q, k, v, mask, scale, cap, bias, slopes, out, out_layout, want_lse, launch_form):
-    dt, scale, cap, radius, q_start, q_end = _checked(q, k, v, mask, cap, scale, bias, slopes)
+class _Rule:
+    """A call's checked numbers, as the C ABI takes them; what the backward pass keeps of the forward pass."""
+
+    __slots__ = ("mask", "dt", "dev", "sizes", "scale", "cap", "radius", "q_start", "q_end", "strides")
+
+    def __init__(self, q, k, v, mask, scale, cap, bias, slopes):
+        # (one pass over the conditions: this runs on every call; which of them failed is found out by _refuse)
+        dtype, dev = q.dtype, q.device
+        qs, ks, vs = q.shape, k.shape, v.shape
+        scale = (0.0 if len(qs) != 4 or qs[3] == 0 else 1.0 / math.sqrt(qs[3])) if scale is None else float(scale)
+        cap = 0.0 if cap is None else float(cap)
+        qt, kt, vt = q.stride(), k.stride(), v.stride()
+        ok = (q.is_cuda and dtype in _DTYPES and len(qs) == 4 and len(ks) == 4 and vs == ks and qt[3] == 1 and kt[3] == 1 and vt[3] == 1
+              and k.dtype == dtype and v.dtype == dtype and k.device == dev and v.device == dev and ks[0] == qs[0] and ks[3] == qs[3]
+              and ks[1] > 0 and qs[1] % ks[1] == 0 and (qs[3] == 64 or qs[3] == 128) and 0.0 < scale < 1e30
+              and (cap == 0.0 or 1e-30 < cap < 1e30))
+        radius = -1
+        if ok and bias is not None:
+            n = bias.shape
+            ok = (slopes is None and len(n) == 2 and n[0] == qs[1] and n[1] % 2 == 1 and n[1] <= 2 * MAX_RADIUS + 1 and bias.is_contiguous()
+                  and bias.dtype == dtype and bias.device == dev)
+            radius = n[-1] // 2
+        elif ok and slopes is not None:
+            ok = (slopes.shape == qs[1:2] and slopes.dtype == torch.float32 and slopes.is_contiguous() and slopes.device == dev
+                  and not slopes.requires_grad)
+        if not ok:
+            _refuse(q, k, v, mask, scale, cap, bias, slopes)
+        B, Hq, Sq, D = qs
+        Hkv, Sk = ks[1], ks[2]
+        mask._check(B, Sq, Sk, dev)
+        start = mask.q_start
+        self.mask, self.dt, self.dev, self.sizes = mask, _DTYPES[dtype], dev, (B, Hq, Hkv, Sq, Sk, D)
+        self.scale, self.cap, self.radius = scale, cap, radius
+        self.q_end = 1 if start == "end" else 0
+        self.q_start = 0 if self.q_end else (Sk - Sq if start is None else start)
+        i64x3 = _lib.i64x3
+        self.strides = (i64x3(qt[0], qt[1], qt[2]), i64x3(kt[0], kt[1], kt[2]), i64x3(vt[0], vt[1], vt[2]))
+
+
+def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
     if launch_form not in _FORMS:
         raise StofError(f"launch form must be one of None, 'auto', 'wide', 'rows', got {launch_form!r}")
     form = _FORMS[launch_form]
-    B, Hq, Sq, D = q.shape
-    Hkv, Sk = k.shape[1], k.shape[2]
-    dev = q.device
+    B, Hq, Hkv, Sq, Sk, D = sizes = r.sizes
+    dev, mask = r.dev, r.mask
     if out_layout == "bhsd":
         if out is None:
-            out = torch.empty((B, Hq, Sq, D), dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.stride(3) != 1:
-            raise StofError("out must be [B,H,S,D] with contiguous D")
-        ostr = (out.stride(0), out.stride(1), out.stride(2))
+            out = q.new_empty((B, Hq, Sq, D))
+            ostr = (Hq * Sq * D, Sq * D, D)
+        elif out.shape != q.shape or out.stride(3) != 1 or out.dtype != q.dtype or out.device != dev:
+            raise StofError("out must be [B,H,S,D] with contiguous D, of q's dtype and device")
+        else:
+            ostr = out.stride()
     elif out_layout == "bshd":
         if out is None:
-            out = torch.empty((B, Sq, Hq * D), dtype=q.dtype, device=dev)
-        elif out.shape != (B, Sq, Hq * D) or out.stride(2) != 1:
-            raise StofError("out must be [B,S,H*D] with contiguous last dim")
-        ostr = (out.stride(0), D, out.stride(1))
+            out = q.new_empty((B, Sq, Hq * D))
+            ostr = (Sq * Hq * D, D, Hq * D)
+        elif out.shape != (B, Sq, Hq * D) or out.stride(2) != 1 or out.dtype != q.dtype or out.device != dev:
+            raise StofError("out must be [B,S,H*D] with contiguous last dim, of q's dtype and device")
+        else:
+            ostr = (out.stride(0), D, out.stride(1))
     else:
         raise StofError(f"unknown out_layout {out_layout!r}")
-    if out.dtype != q.dtype or out.device != dev:
-        raise StofError("out must have q's dtype and device")
     lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=dev) if want_lse else None
     if B == 0 or Hq == 0 or Sq == 0 or Sk == 0:
         out.zero_()
@@ -155,19 +193,24 @@ def _forward(q, k, v, mask, scale, cap, bias, slopes, out, out_layout, want_lse,
             lse.fill_(-math.inf)
         return out, lse
     lib = _lib.lib()
-    nbytes = lib.stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, radius, mask.docs_q is not None, form)
+    docs_q = mask.docs_q
+    nbytes = lib.stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, r.radius, docs_q is not None, form)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None   # this call's own: calls may overlap on other streams and graphs
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(bias), _ptr(slopes), _ptr(mask.prefix),
-            _ptr(mask.kv_len), _ptr(mask.docs_q), _ptr(mask.docs_k), scale, cap, radius, int(mask.causal), q_start, q_end,
-            _lib.i64x3(qs[0], qs[1], qs[2]), _lib.i64x3(ks[0], ks[1], ks[2]), _lib.i64x3(vs[0], vs[1], vs[2]), _lib.i64x3(*ostr),
-            B, Hq, Hkv, Sq, Sk, D, dt, form, _ptr(ws), nbytes, _stream(dev))
+    qs, ks, vs = r.strides
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(lse), _at(bias), _at(slopes), _at(mask.prefix),
+            _at(mask.kv_len), _at(docs_q), _at(mask.docs_k), r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end,
+            qs, ks, vs, _lib.i64x3(ostr[0], ostr[1], ostr[2]),
+            *sizes, r.dt, form, _at(ws), nbytes, _stream(dev))
     if dev.index == torch.cuda.current_device():
         check(lib.stof_score_attn_fwd(*args), "stof_score_attn_fwd")
     else:
         with torch.cuda.device(dev):
             check(lib.stof_score_attn_fwd(*args), "stof_score_attn_fwd")
     return out, lse
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t):
@@ -183,19 +226,20 @@ def score_attn_backward(dout, q, k, v, out, lse, mask=None, scale=None, cap=None
     contiguous, ``dbias`` None without a table.  What autograd calls; on its own
     it is for training loops that keep their own graph of calls, a captured one among them.  ``dout`` and ``out``
     are ``[B,Hq,Sq,D]`` views; the rule must be the forward pass's."""
-    mask = _NO_MASK if mask is None else mask
-    dt, scale, cap, radius, q_start, q_end = _checked(q, k, v, mask, cap, scale, bias, slopes)
-    B, Hq, Sq, D = q.shape
-    Hkv, Sk = k.shape[1], k.shape[2]
-    dev = q.device
+    r = _Rule(q, k, v, _NO_MASK if mask is None else mask, scale, cap, bias, slopes)
     for name, t in (("dout", dout), ("out", out)):
-        if t.shape != q.shape or t.dtype != q.dtype or t.device != dev:
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != r.dev:
             raise StofError(f"{name} must have q's shape, dtype and device")
-    if lse.shape != (B, Hq, Sq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
-        raise StofError(f"lse must be the float32 [{B}, {Hq}, {Sq}] tensor of the forward pass")
-    new = lambda like: torch.empty(like.shape, dtype=q.dtype, device=dev)
-    dq, dk, dv = new(q), new(k), new(v)
-    db = new(bias) if bias is not None else None
+    if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != r.dev:
+        raise StofError(f"lse must be the float32 {list(q.shape[:3])} tensor of the forward pass")
+    return _backward(dout, q, k, v, out, lse, r, bias, slopes)
+
+
+def _backward(dout, q, k, v, out, lse, r, bias, slopes):
+    B, Hq, Hkv, Sq, Sk, D = sizes = r.sizes
+    dev, mask = r.dev, r.mask
+    dq, dk, dv = q.new_empty((B, Hq, Sq, D)), q.new_empty((B, Hkv, Sk, D)), q.new_empty((B, Hkv, Sk, D))
+    db = torch.empty_like(bias) if bias is not None else None
     if B == 0 or Hq == 0 or Sq == 0 or Sk == 0:
         for t in (dq, dk, dv, db):
             if t is not None:
@@ -203,13 +247,14 @@ def score_attn_backward(dout, q, k, v, out, lse, mask=None, scale=None, cap=None
         return dq, dk, dv, db
     dout, out = _rows(dout), _rows(out)
     lib = _lib.lib()
-    nbytes = lib.stof_score_attn_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, radius, mask.docs_q is not None)
+    nbytes = lib.stof_score_attn_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, r.radius, mask.docs_q is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    s3 = lambda t: _lib.i64x3(*t.stride()[:3])
-    args = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(db),
-            _ptr(bias), _ptr(slopes), _ptr(mask.prefix), _ptr(mask.kv_len), _ptr(mask.docs_q), _ptr(mask.docs_k),
-            scale, cap, radius, int(mask.causal), q_start, q_end, s3(dout), s3(q), s3(k), s3(v), s3(out),
-            B, Hq, Hkv, Sq, Sk, D, dt, ws.data_ptr(), nbytes, _stream(dev))
+    ds, os_ = dout.stride(), out.stride()
+    i64x3 = _lib.i64x3
+    args = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), _at(db), _at(bias), _at(slopes), _at(mask.prefix), _at(mask.kv_len), _at(mask.docs_q), _at(mask.docs_k),
+            r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end, i64x3(ds[0], ds[1], ds[2]), *r.strides,
+            i64x3(os_[0], os_[1], os_[2]), *sizes, r.dt, ws.data_ptr(), nbytes, _stream(dev))
     if dev.index == torch.cuda.current_device():
         check(lib.stof_score_attn_bwd(*args), "stof_score_attn_bwd")
     else:
@@ -220,11 +265,12 @@ def score_attn_backward(dout, q, k, v, out, lse, mask=None, scale=None, cap=None
 
 class _ScoreAttn(Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, slopes, mask, scale, cap, out_layout, launch_form):
-        out, lse = _forward(q, k, v, mask, scale, cap, bias, slopes, None, out_layout, True, launch_form)
+    def forward(ctx, q, k, v, bias, slopes, rule, out_layout, launch_form):
+        out, lse = _forward(q, k, v, rule, bias, slopes, None, out_layout, True, launch_form)
+        mask = rule.mask
         # the rule's tensors are saved too, so that one changed in place before the backward pass is noticed
         ctx.save_for_backward(q, k, v, out, lse, bias, slopes, mask.prefix, mask.kv_len, mask.docs_q, mask.docs_k)
-        ctx.rule = (mask, scale, cap, out_layout)
+        ctx.rule, ctx.out_layout = rule, out_layout
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)          # no zeros for lse
         return out, lse
@@ -233,16 +279,15 @@ class _ScoreAttn(Function):
     @once_differentiable
     def backward(ctx, dout, _dlse):
         if dout is None:
-            return (None,) * 10
+            return (None,) * 8
         q, k, v, out, lse, bias, slopes = ctx.saved_tensors[:7]
-        mask, scale, cap, out_layout = ctx.rule
-        if out_layout == "bshd":
+        if ctx.out_layout == "bshd":
             B, H, S, D = q.shape
             out, dout = (t.reshape(B, S, H, D).permute(0, 2, 1, 3) for t in (out, dout))
         need = ctx.needs_input_grad
-        dq, dk, dv, db = score_attn_backward(dout, q, k, v, out, lse, mask, scale, cap, bias, slopes)
+        dq, dk, dv, db = _backward(dout, q, k, v, out, lse, ctx.rule, bias, slopes)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, db if need[3] else None,
-                None, None, None, None, None, None)
+                None, None, None, None)
 
 
 def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None, out=None, out_layout="bhsd",
@@ -255,11 +300,11 @@ def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None,
     logarithm of the softmax's denominator, fp32 ``[B,Hq,Sq]``.  Differentiable in q, k, v and bias (through the
     output, not through lse).  ``launch_form``: None, "wide" (128-query tiles) or "rows" (32-row tiles with the
     keys split; single tokens and small grids) - the rule by sizes is in the library."""
-    mask = _NO_MASK if mask is None else mask
+    r = _Rule(q, k, v, _NO_MASK if mask is None else mask, scale, cap, bias, slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         if out is not None:
             raise StofError("out= has no gradient: leave it out, or call under torch.no_grad()")
-        o, lse = _ScoreAttn.apply(q, k, v, bias, slopes, mask, scale, cap, out_layout, launch_form)
-        return (o, lse) if return_lse else o
-    o, lse = _forward(q, k, v, mask, scale, cap, bias, slopes, out, out_layout, return_lse, launch_form)
+        o, lse = _ScoreAttn.apply(q, k, v, bias, slopes, r, out_layout, launch_form)
+    else:
+        o, lse = _forward(q, k, v, r, bias, slopes, out, out_layout, return_lse, launch_form)
     return (o, lse) if return_lse else o
