@@ -84,30 +84,40 @@ __device__ __forceinline__ float pair_sum(float x) {
 }
 
 // Workgroup -> (head, tile).  The dispatcher hands workgroups to the 8 XCDs in turn and, inside an XCD, to its compute
-// units in turn; an XCD takes whole heads, so that a head's K and V pass through one L2.  Causal work grows along the
+// units in turn; an XCD takes whole key heads (with the `group` query heads that share each), so that a head's K and V
+// pass through one L2, and every eighth of them, so that samples of uneven length spread over the XCDs (B8 H12 S1024
+// with uneven key lengths: a sample per XCD before, the longest set the time).  Causal work grows along the
 // tiles: the heads of a set that fills the XCD (`resident` workgroups per unit) are then ordered together, longest
 // tiles first.  The passes over the units that become resident at once are dealt in boustrophedon order, so that a
 // unit that starts with a long tile gets a short one beside it; what follows goes to whichever unit is free.
 // rank counts tiles from the longest; the order is a bijection for any sizes.  Head by head, longest first, before:
 // B2 H16 S2048 causal, D128: forward 65 -> 52 us, backward 113 -> 83 (queries) and 132 -> 97 (keys).
 struct Placed { int head, rank; };
-__device__ __forceinline__ bool place(const int index, const int heads, const int tiles, const int chunk, const int cus_per_xcd,
-                                      const int resident, const bool graded, Placed& out) {
+__device__ __forceinline__ bool place(const int index, const int heads, const int group, const int tiles, const int chunk,
+                                      const int cus_per_xcd, const int resident, const bool graded, Placed& out) {
   const int x = index & 7, i = index >> 3;
-  if (!graded || heads % 8 != 0) {
+  if ((heads / group) % 8 != 0) {          // key heads do not divide over the XCDs: contiguous shares, head by head
     const int id = x * chunk + i;
     out.head = id / tiles;
     out.rank = id - out.head * tiles;
     return id < heads * tiles;
   }
-  const int hx = heads / 8;
-  const int hs = min(hx, max(1, (resident * cus_per_xcd + tiles - 1) / tiles));
-  const int set = i / (hs * tiles), h0 = set * hs, hn = min(hs, hx - h0), il = i - set * hs * tiles;
-  const int pass = il / cus_per_xcd, pos = il - pass * cus_per_xcd;
-  const int len = min(cus_per_xcd, hn * tiles - pass * cus_per_xcd);
-  const int j = pass * cus_per_xcd + (pass < resident && (pass & 1) ? len - 1 - pos : pos);
-  out.rank = j / hn;
-  out.head = x * hx + h0 + (j - out.rank * hn);
+  const int hx = heads / 8;                // (the grid is exact: chunk = hx * tiles)
+  int local;                               // of this XCD's heads
+  if (!graded) {
+    local = i / tiles;
+    out.rank = i - local * tiles;
+  } else {
+    const int hs = min(hx, max(1, (resident * cus_per_xcd + tiles - 1) / tiles));
+    const int set = i / (hs * tiles), h0 = set * hs, hn = min(hs, hx - h0), il = i - set * hs * tiles;
+    const int pass = il / cus_per_xcd, pos = il - pass * cus_per_xcd;
+    const int len = min(cus_per_xcd, hn * tiles - pass * cus_per_xcd);
+    const int j = pass * cus_per_xcd + (pass < resident && (pass & 1) ? len - 1 - pos : pos);
+    out.rank = j / hn;
+    local = h0 + (j - out.rank * hn);
+  }
+  const int key_head = local / group;
+  out.head = (key_head * 8 + x) * group + (local - key_head * group);
   return true;
 }
 

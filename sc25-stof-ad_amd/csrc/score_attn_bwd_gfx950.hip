@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
   Placed at;
-  if (!place(blockIdx.x, p.B * p.Hq, bp.q_tiles, bp.q_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, at)) return;
+  if (!place(blockIdx.x, p.B * p.Hq, p.group, bp.q_tiles, bp.q_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, at)) return;
   const int bh = at.head, tile = bp.q_tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
   const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
@@ -213,8 +213,6 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, i < p.Sq, -1) : 0;
   L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
   L.tab = tab;
-  if (p.bias_kind == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);
-
   floatx2_t st = {INFINITY, 0.f};
   if (i < p.Sq) st = bp.stats[(int64_t)bh * (64 * nqb) + i];
   const float lse = st[0], delta = st[1];
@@ -397,6 +395,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   };
   Step cur = next_step();
   if (cur.t >= 0) issue(cur.t, (lds_byte*)k0, (lds_byte*)v0);
+  if (p.bias_kind == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);   // (the walk's first barrier covers it)
   while (cur.t >= 0) {
     Step nxt = next_step();
     step(cur, nxt, (lds_byte*)k0, (lds_byte*)v0, (lds_byte*)k1, (lds_byte*)v1);
@@ -420,25 +419,29 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   store_rows<D, BF>(acc, 1.f, stage, bp.dq + ((int64_t)bh * p.Sq + row0) * D, rows, lane);
 }
 
-// d table[h][x]: the workgroups' sums over batch and key tiles, in order.  Four slices of them per entry.
+// d table[h][x]: the workgroups' sums over batch and key tiles, in order.  Sixteen slices of them per entry.
 template <bool BF>
-__global__ __launch_bounds__(256) void score_attn_bwd_table_kernel(const BwdParams bp) {
+__global__ __launch_bounds__(1024) void score_attn_bwd_table_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;
-  __shared__ float part[4][64];
+  __shared__ float part[16][64];
   const int n_dist = 2 * p.radius + 1;
   const int h = blockIdx.y, x = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
-  const int tiles = bp.k_tiles * bp.splits, n = p.B * tiles, per = (n + 3) / 4;
+  const int tiles = bp.k_tiles * bp.splits, n = p.B * tiles, per = (n + 15) / 16;
   float t = 0.f;                   // (fp16: carried times 2^kPShift)
-  if (x < n_dist)
+  if (x < n_dist) {
+#pragma unroll 4
     for (int y = slice * per; y < min(n, (slice + 1) * per); ++y) {
       const int b = y / tiles, tile = y - b * tiles;
       t += bp.tab_part[(((int64_t)b * p.Hq + h) * tiles + tile) * n_dist + x];
     }
+  }
   part[slice][threadIdx.x & 63] = t;
   __syncthreads();
   if (slice == 0 && x < n_dist) {
-    const int y = threadIdx.x;
-    bp.dtable[(int64_t)h * n_dist + x] = to_elem<BF>((BF ? 1.f : pow2(-kPShift)) * ((part[0][y] + part[1][y]) + (part[2][y] + part[3][y])));
+    float sum = 0.f;
+#pragma unroll
+    for (int y = 0; y < 16; ++y) sum += part[y][threadIdx.x];
+    bp.dtable[(int64_t)h * n_dist + x] = to_elem<BF>((BF ? 1.f : pow2(-kPShift)) * sum);
   }
 }
 
@@ -467,7 +470,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
   Placed at;
-  if (!place(blockIdx.x, p.B * p.Hkv, bp.k_tiles * bp.splits, bp.k_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, at)) return;
+  if (!place(blockIdx.x, p.B * p.Hkv, 1, bp.k_tiles * bp.splits, bp.k_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, at)) return;
   const int bk = at.head, slot = at.rank;
   const int tile = slot / bp.splits, split = slot - tile * bp.splits;   // (causal: the first keys have most queries)
   const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
@@ -811,14 +814,15 @@ __global__ __launch_bounds__(256) void score_attn_bwd_join_kernel(const float* p
 // ---- host side
 
 // Workgroups per key tile: few key heads (shared by many query heads) and short sequences leave the device
-// empty while each workgroup walks all their query tiles.  Split s takes every splits-th query tile, until 512
-// workgroups (two per compute unit) have work of at least four tiles each; their fp32 sums are joined by one more
-// kernel.  B2 H16/4 S2048 D128 causal, 128 workgroups: 246 us unsplit, 103 + 12 us with four splits.
+// empty while each workgroup walks all their query tiles.  Up to 256 workgroups, split s takes every splits-th query
+// tile, until 512 workgroups (two per compute unit) have work of at least four tiles each; their fp32 sums are
+// joined by one more kernel.  B2 H16/4 S2048 D128 causal, 128 workgroups: 246 us unsplit, 103 + 12 us with four
+// splits; B8 H12 S512 D64 with a table, 384 workgroups: 51 + 4 us unsplit, 44 + 18 us with two.
 int key_splits(int B, int Hkv, int Sq, int Sk, int group, int D) {
   const int64_t wgs = (int64_t)B * Hkv * ((Sk + 127) / 128);
   const int64_t want = 512;
   const int most = ((Sq + 63) / 64 * group + 3) / 4;
-  int64_t n = wgs >= want ? 1 : (want + wgs - 1) / wgs;
+  int64_t n = wgs > want / 2 ? 1 : (want + wgs - 1) / wgs;
   if (n > (Sq + 63) / 64) n = (Sq + 63) / 64;
   if (n > most) n = most;
   return n > 8 ? 8 : (int)n;
@@ -860,7 +864,7 @@ void launch_bwd(BwdParams& p, hipStream_t st) {
     score_attn_bwd_join_kernel<BF><<<dim3((unsigned)((2 * n / 8 + 255) / 256)), dim3(256), 0, st>>>(p.kv_part, p.dk, p.dv, n, p.splits);
   }
   if (s.bias_kind == kBiasTable)
-    score_attn_bwd_table_kernel<BF><<<dim3((unsigned)((2 * s.radius + 64) / 64), (unsigned)s.Hq), dim3(256), 0, st>>>(p);
+    score_attn_bwd_table_kernel<BF><<<dim3((unsigned)((2 * s.radius + 64) / 64), (unsigned)s.Hq), dim3(1024), 0, st>>>(p);
 }
 
 }  // namespace

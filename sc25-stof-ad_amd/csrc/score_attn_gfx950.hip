@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
 
   Placed at;
-  if (!place(blockIdx.x, p.B * p.Hq, p.tiles, p.chunk, p.cus_per_xcd, 2, p.causal, at)) return;
+  if (!place(blockIdx.x, p.B * p.Hq, p.group, p.tiles, p.chunk, p.cus_per_xcd, D == 64 ? 3 : 2, p.causal, at)) return;
   const int bh = at.head, tile = p.tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
 
@@ -157,7 +157,6 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, i < p.Sq, -1) : 0;
   L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
   L.tab = tab;
-  if (p.bias_kind == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);   // (the walk's first barrier covers it)
 
   // Q^T as the B operand: lane (query j32, group g) holds 8 consecutive d per step; rows past the end re-read the last
   half8_t qf[D / 16];
@@ -245,8 +244,31 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
     __syncthreads();
     if (nxt.t >= 0) issue(nxt.t, kn, vn);
     if (!cur.mine) return;
+    // fragments two ahead of their MFMA, in a ring of three: K's for the scores, then V's (transposed), the first two of
+    // which arrive during the softmax
+    constexpr int NS = D / 8, NV = D / 8;          // MFMAs of the scores and of P V
+    half8_t ring[3];
+    auto fetch = [&](int n) {
+      if (n < NS) {
+        ring[n % 3] = lds_frag(kt + 32 * (n & 1) * (2 * D) + rd[n >> 1]);
+      } else if (n < NS + NV) {
+        const int m = n - NS, dt = m % (D / 32);
+        const lds_byte* vp = vt + 16 * (m / (D / 32)) * (2 * D);
+        ring[n % 3] = lds_frag_tr(vp + tr[dt][0], vp + tr[dt][1]);
+      }
+    };
     floatx16 s[2];
-    scores_product<D, 2, BF>(kt, rd, qf, s);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
+    fetch(0);
+    fetch(1);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      fetch(n + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      s[n & 1] = mfma32<BF>(ring[n % 3], qf[n >> 1], s[n & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     const int j0 = cur.t * kBlock + 4 * g;
     if constexpr (CAP) { cap_scores(p, s[0]); cap_scores(p, s[1]); }
     if (p.bias_kind != kBiasNone) { bias_scores<CAP>(p, L, j0, s[0]); bias_scores<CAP>(p, L, j0 + 32, s[1]); }
@@ -262,10 +284,19 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
     }
     half8_t pf[2][2];
     sm.step(p.cc, s, pf);
-    sm.accumulate(vt, tr, pf);
+#pragma unroll
+    for (int n = NS; n < NS + NV; ++n) {
+      const int m = n - NS, u = m / (D / 32), dt = m % (D / 32);
+      fetch(n + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      sm.o[dt] = mfma32<BF>(ring[n % 3], pf[u >> 1][u & 1], sm.o[dt]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   Step cur = next_step();
   if (cur.t >= 0) issue(cur.t, (lds_byte*)k0, (lds_byte*)v0);
+  // (behind the first tile's loads, whose latency it shares; the walk's first barrier covers it)
+  if (p.bias_kind == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);
   while (cur.t >= 0) {
     Step nxt = next_step();
     step(cur, nxt, (lds_byte*)k0, (lds_byte*)v0, (lds_byte*)k1, (lds_byte*)v1);
@@ -333,11 +364,6 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, true, -1) : 0;
   L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
   L.tab = tab + hg * n_tab;
-  if (p.bias_kind == kBiasTable) {
-    for (int x = 0; x < G; ++x) load_table<BF>(p, hk * G + x, tab + x * n_tab, threadIdx.x, 64 * kRowWaves);
-    __syncthreads();
-  }
-
   half8_t qf[D / 16];
   {
     const half_t* src = p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)i * p.qs[2];
@@ -409,6 +435,10 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   constexpr int kAllButOne = (TL::kN & 15) | ((TL::kN >> 4) << 14) | 0x0F70;   // vmcnt: the loads of one tile may be out
   Step cur = next_step();
   if (cur.t >= 0) { issue_k(cur.t); issue_v(cur.t); }
+  if (p.bias_kind == kBiasTable) {      // (behind the first loads, whose latency it shares)
+    for (int x = 0; x < G; ++x) load_table<BF>(p, hk * G + x, tab + x * n_tab, threadIdx.x, 64 * kRowWaves);
+    __syncthreads();
+  }
   while (cur.t >= 0) {
     const Step nxt = next_step();
     int id = 0;
