@@ -596,10 +596,13 @@ __global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams 
 
 // ---- host side
 
-// Form and number of key splits.  The row form takes calls whose rows fit one 32-row tile per key head
-// (single tokens: a token's heads read the cache once) and grids that give the wide form less than one
-// workgroup per compute unit; the keys are split until two workgroups per unit (one at head size 128,
-// whose tile buffers fill the LDS) have work, at least four tiles of 32 keys per wave's stream.
+// Form and number of key splits.  The row form takes calls whose rows fit one 32-row tile per key head (single tokens: a
+// token's heads read the cache once), and grids that leave most of the device to a few workgroups of the wide form,
+// each of which then walks all keys alone (us, wide | rows): B1 H8 S1024 D64 (64 workgroups) 16.8 | 8.6, B2 H12
+// S512 (96) 10.5 | 12.3, B1 H8 S2048 (128) 31.1 | 23.0, B2 H8 S1024 D128 (128) 23.3 | 25.6, B3 H8 S1000 (192) 18.0 |
+// 23.3, B8 H32 4 queries over 1024 keys 16.7 | 14.0.  With less than a workgroup per compute unit the keys are
+// split further until four per unit have work (of two tiles for each wave at least), which also evens out
+// caches of different length: B16 H32/8 up to 16384 keys D128, two splits 146 us, eight 128.
 namespace {
 
 struct Form { bool rows; int tiles, splits; };
@@ -610,14 +613,14 @@ inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius,
   const int group = Hq / Hkv, cus = 256;
   const int64_t wide = (int64_t)B * Hq * ((Sq + 127) / 128);
   const int64_t rows = (int64_t)Sq * group;
-  bool use_rows = form == 1 || (form < 0 && (rows <= 32 || wide < cus));
+  bool use_rows = form == 1 || (form < 0 && (rows <= 32 || wide < 96 || (wide <= 128 && Sk >= 2048)));
   if (!rows_fit(group, radius)) use_rows = false;
   if (!use_rows) return Form{false, (Sq + 127) / 128, 1};
   const int tiles = (int)((rows + 31) / 32);
   const int64_t wgs = (int64_t)B * Hkv * tiles;
   const int64_t want = 4 * cus;
   const int key_tiles = (Sk + kRowKeys - 1) / kRowKeys;
-  int64_t splits = (want + wgs - 1) / wgs;
+  int64_t splits = wgs >= cus ? 1 : (want + wgs - 1) / wgs;
   const int most = (key_tiles + 2 * kRowWaves - 1) / (2 * kRowWaves);      // two tiles per wave
   if (splits > most) splits = most;
   if (splits > 64) splits = 64;                                            // one lane each in the join
