@@ -8,7 +8,7 @@
 // quotient y = t / a' from one reciprocal and one residual step is within 2^-23 of the true quotient,
 // while a quotient of such numbers that is not k + 1/2 lies at least 2^-19 (relative) away from it.
 //
-// The products are exact: v_mfma_i32_32x32x32_i8 adds into int32, K <= 131072 keeps |sum| below 2^31.  The
+// The products are exact: v_mfma_i32_32x32x32_i8 adds into int32, K <= 131056 keeps |sum| below 2^31 for any int8 operands.  The
 // only roundings are fp32 scaling, bias and activation, and the store.
 //
 // Large products use the tile form of the 16-bit GEMM (C^T = W X^T, both operands K-contiguous through LDS
@@ -431,7 +431,7 @@ void launch_quantize(const void* x, int8_t* xq, float* sx, int M, int K, int64_t
 
 int check_sizes(int64_t M, int64_t N, int64_t K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || N % 8 != 0) return STOF_ERR_BAD_SHAPE;
-  if (M > (1 << 28) || N > (1 << 28) || K > 131072 || ((M + 63) / 64 + 8) * ((N + 63) / 64) > 0x0fffffff) return STOF_ERR_BAD_SHAPE;
+  if (M > (1 << 28) || N > (1 << 28) || K > 131056 || ((M + 63) / 64 + 8) * ((N + 63) / 64) > 0x0fffffff) return STOF_ERR_BAD_SHAPE;
   if (dtype != STOF_DTYPE_F16 && dtype != STOF_DTYPE_BF16) return STOF_ERR_UNSUPPORTED;
   return STOF_OK;
 }

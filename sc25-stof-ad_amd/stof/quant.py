@@ -57,8 +57,8 @@ def quantize_rows_i8(x):
     """``x`` ``[..., K]`` (fp16 or bfloat16, K a multiple of 16) -> int8 ``[..., K]`` and its scales, fp32 ``[...]``."""
     dt = _elems("x", x)
     K = x.shape[-1] if x.dim() else 0
-    if K % 16 or K == 0 or K > 131072:
-        raise StofError(f"K must be a multiple of 16 up to 131072, got {K}")
+    if K % 16 or K == 0 or K > 131056:
+        raise StofError(f"K must be a multiple of 16 up to 131056, got {K}")
     x2, ldx = _rows2d("x", x, 8)
     M = x2.shape[0]
     xq = torch.empty(x.shape, dtype=torch.int8, device=x.device)
@@ -75,8 +75,8 @@ def _weights(wq, w_scale, bias, K, dev, dtype, act):
     N = wq.shape[0]
     if N == 0 or N % 8:
         raise StofError(f"N must be a multiple of 8, got {N}")
-    if K % 16 or K == 0 or K > 131072:
-        raise StofError(f"K must be a multiple of 16 up to 131072, got {K}")
+    if K % 16 or K == 0 or K > 131056:
+        raise StofError(f"K must be a multiple of 16 up to 131056, got {K}")
     ldw = wq.stride(0) if N > 1 else K
     if not (w_scale.dtype == torch.float32 and w_scale.shape == (N,) and w_scale.is_contiguous() and w_scale.device == dev):
         raise StofError(f"w_scale must be a contiguous float32 [{N}] tensor on x's device")

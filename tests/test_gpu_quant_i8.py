@@ -131,8 +131,8 @@ def test_every_tile_form_at_its_edges(M, N, K):
 
 
 def test_sums_at_the_largest_k():
-    """Every product 127 x 127 at K = 131072: the sum 2114060288 is the largest an int32 has to hold here."""
-    K = 131072
+    """Every product 127 x 127 at the largest K, and -128 x -128, whose sum 2147221504 is the largest there is below 2^31."""
+    K = 131056
     x = torch.full((20, K), 3.0).bfloat16()
     w = torch.full((8, K), 127, dtype=torch.int8)
     w[1] = -127
@@ -141,6 +141,17 @@ def test_sums_at_the_largest_k():
         y = linear_i8(rows.cuda(), w.cuda(), ws.cuda()).cpu().double()
         want = 3.0 * 127 * K * 1e-9
         assert bool(((y[:, 0] - want).abs() <= 2.0 ** -7 * want).all()) and bool((y[:, 1] == -y[:, 0]).all())
+    low = torch.full((20, K), -128, dtype=torch.int8)
+    y = gemm_i8(low.cuda(), torch.ones(20).cuda(), low[:8].cuda(), ws.cuda(), dtype=torch.bfloat16).cpu().double()
+    assert bool(((y - 2147221504e-9).abs() <= 2.0 ** -8 * 2.15).all())
+
+
+@pytest.mark.parametrize("M,K", [(16, 4096), (1, 65536), (16, 4112), (2, 32768), (2, 32784)])
+def test_token_form_at_the_limit_of_its_lds(M, K):
+    """64 KB of quantised rows in LDS, and the first sizes beyond, which take the other form."""
+    x = torch.randn(M, K, generator=_gen(M)).bfloat16()
+    w, ws, b = _weights(24, K, torch.bfloat16, 3)
+    _close(linear_i8(x.cuda(), w.cuda(), ws.cuda(), b.cuda()), _want(*_quant64(x), w, ws, b, "none", torch.bfloat16))
 
 
 def test_batch_dims_strides_and_guard_rows():

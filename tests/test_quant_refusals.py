@@ -28,7 +28,7 @@ def test_argument_checks(lib):
     q = lambda x=P, xq=P, sx=P, M=4, K=64, ldx=64, ldq=64, dt=0: lib.stof_quantize_rows_i8(x, xq, sx, M, K, ldx, ldq, dt, None)
     assert q(x=None) == -1 and q(xq=None) == -1 and q(sx=None) == -1
     assert q(x=P + 2) == -4 and q(ldx=65) == -4 and q(ldq=72) == -4
-    assert q(M=0) == -2 and q(K=40) == -2 and q(K=131088) == -2 and q(ldx=56) == -2 and q(ldq=48) == -2
+    assert q(M=0) == -2 and q(K=40) == -2 and q(K=131072) == -2 and q(ldx=56) == -2 and q(ldq=48) == -2
     assert q(dt=2) == -3
     g = lambda xq=P, sx=P, wq=P, sw=P, b=None, o=P, M=4, N=16, K=64, ldq=64, ldw=64, ldo=16, act=0, dt=0: \
         lib.stof_gemm_i8_bias_act(xq, sx, wq, sw, b, o, M, N, K, ldq, ldw, ldo, act, dt, None)
