@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define STOF_ABI_VERSION 4   /* 4: attention plan entry points, stof_retile_lut and the cluster form with a wait limit added, the two process-wide setters (attention launch form, cluster spin limit) removed - both are per-call arguments, the library keeps no mutable state; 3: split-K and element-format entry points (nothing removed or changed) */
+#define STOF_ABI_VERSION 4   /* entry points added since (score attention, 8-bit linear) change none of these and keep the number; 4: attention plan entry points, stof_retile_lut and the cluster form with a wait limit added, the two process-wide setters (attention launch form, cluster spin limit) removed - both are per-call arguments, the library keeps no mutable state; 3: split-K and element-format entry points (nothing removed or changed) */
 
 enum {
   STOF_OK = 0,
@@ -426,15 +426,17 @@ int stof_gemm_bias_res_ln_cluster_dt(const void* A, const void* Wt, const void* 
  *                  docs_q[b][i] == docs_k[b][j] >= 0
  *   out_i = softmax over the allowed j, times v;  lse_i = log of the softmax's denominator
  * A row without allowed keys gives zeros and lse = -inf.  prefix, kv_len (clamped to [0, Sk]), docs_*:
- * int32, each may be NULL; they are read by the launch, not before.  Keys at or past kv_len and keys of a
- * negative document are not used as values, whatever they hold (NaN included).
+ * int32, each may be NULL; they are read by the launch, not before.  Keys at or past kv_len, keys that causality
+ * closes to every query of the sample and keys of a negative document are not used as values, whatever they hold
+ * (NaN included).  scale in (0, 1e6], cap 0 or in [1e-3, 1024].
  * Strides: (batch, head, row) in elements, multiples of 8, rows at most 2^23; pointers 16-byte aligned.
  * lse [B, Hq, Sq] fp32 may be NULL.  form: -1 the library's choice, 0 128-query tiles, 1 32-row tiles with
  * the keys split over waves and workgroups.  The workspace (bytes below, 0 = none) needs no initial
  * contents and belongs to this call until its work is done.
  */
 #define STOF_SCORE_MAX_RADIUS 1024
-int64_t stof_score_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int docs, int form);
+#define STOF_SCORE_MAX_CAP 1024.0f   /* the cap's error is 2^-22 of it: beyond, scores would lose what 16-bit outputs keep */
+int64_t stof_score_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs, int form);
 int stof_score_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
                         const void* table, const float* slopes, const int32_t* prefix, const int32_t* kv_len,
                         const int32_t* docs_q, const int32_t* docs_k,
@@ -462,8 +464,8 @@ int stof_score_attn_bwd(const void* dout, const void* q, const void* k, const vo
  *   sx_m = max_k |x_mk| / 127,  xq_mk = round(x_mk / sx_m) with the quotient taken exactly, ties to even
  *   out_mn = act(sx_m * sw_n * sum_k xq_mk wq_nk + bias_n), the sum exact in int32
  * wq [N, K] int8 (rows ldw apart) with fp32 scales sw [N], bias [N] and out [M, N] in x's format.  A row of zeros has
- * scale 0; a row that is not finite has scale NaN.  K a multiple of 16 up to 131072, N a multiple of 8, ldx and
- * ldo multiples of 8, ldw and ldq multiples of 16; pointers 16-byte aligned (sx: 4).
+ * scale 0; a row that is not finite has scale NaN.  K a multiple of 16 up to 131056 (sums stay in int32 for any
+ * bytes), N a multiple of 8, ldx and ldo multiples of 8, ldw and ldq multiples of 16; pointers 16-byte aligned (sx: 4).
  * stof_linear_i8 quantises and multiplies: one launch up to 16 tokens (workspace 0 bytes), else two through the
  * workspace, which needs no initial contents.  stof_gemm_i8_bias_act takes rows already quantised, for
  * several products on one x.

@@ -54,22 +54,23 @@ struct ScoreParams {
   float c, k1, capl;                       // scale log2e; 2 scale log2e / cap (0: no cap); cap log2e
   float cc;                                // what turns a rule's result into log2 units: c when it is the raw product, else 1
   // form for few rows
-  int splits, group; float* part;
+  int splits, group, table_in_lds; float* part;
 };
 
-// Per-sample scalars: number of keys and position of query 0.
-__device__ __forceinline__ int sample_keys(const ScoreParams& p, int b) {
-  int n = p.Sk;
-  if (p.kv_len) n = min(max(__builtin_amdgcn_readfirstlane(p.kv_len[b]), 0), p.Sk);
-  return n;
-}
-__device__ __forceinline__ int sample_first(const ScoreParams& p, int klen) { return p.q_end ? klen - p.Sq : p.q_start; }
-__device__ __forceinline__ int sample_prefix(const ScoreParams& p, int b) {
-  return p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[b]) : 0;
-}
 // Keys j < row_limit are allowed for a query at position `pos` (documents aside).
 __device__ __forceinline__ int row_limit(int causal, int klen, int prefix, int pos) {
   return causal ? min(klen, max(pos + 1, prefix)) : klen;
+}
+// A sample's scalars: number of keys that any of its queries may see (those past it are never loaded), position of
+// query 0, prefix.
+struct Sample { int keys, first, prefix; };
+__device__ __forceinline__ Sample sample_of(const ScoreParams& p, int b) {
+  Sample s;
+  s.keys = p.kv_len ? min(max(__builtin_amdgcn_readfirstlane(p.kv_len[b]), 0), p.Sk) : p.Sk;
+  s.first = p.q_end ? s.keys - p.Sq : p.q_start;
+  s.prefix = p.prefix ? __builtin_amdgcn_readfirstlane(p.prefix[b]) : 0;
+  s.keys = max(row_limit(p.causal, s.keys, s.prefix, s.first + p.Sq - 1), 0);
+  return s;
 }
 
 __device__ __forceinline__ float pair_max(float x) {
@@ -203,20 +204,22 @@ template <int D, int ROWS, int WAVES> struct TileLoad {
   }
 };
 
+// A table entry in log2 units.
+template <bool BF> __device__ __forceinline__ float table_entry(half_t v) {
+  const float e = from_elem<BF>(v), s = e * kLog2e;
+  return __builtin_fabsf(e) < INFINITY ? fminf(fmaxf(s, -kTabMax), kTabMax) : s;    // (infinities and NaN as they are)
+}
 // A head's distance table in LDS: entry x + kTabPad + R holds table[clip(x)] * log2(e), x from -R - kTabPad to R + kTabPad.
 template <bool BF>
 __device__ __forceinline__ void load_table(const ScoreParams& p, int head, float* tab, int tid, int threads) {
   const int n = 2 * p.radius + 1;
   for (int x = tid; x < n + 2 * kTabPad; x += threads) {
-    const float e = from_elem<BF>(p.table[(int64_t)head * n + min(max(x - kTabPad, 0), n - 1)]);
-    const float s = e * kLog2e;
-    tab[x] = (e == -INFINITY || e == INFINITY) ? s : fminf(fmaxf(s, -kTabMax), kTabMax);   // (NaN: fminf / fmaxf would drop it)
-    if (e != e) tab[x] = e;
+    tab[x] = table_entry<BF>(p.table[(int64_t)head * n + min(max(x - kTabPad, 0), n - 1)]);
   }
 }
 
 // What one lane knows of its query.
-struct LaneRow { int pos, limit, doc; float slope; const float* tab; };
+struct LaneRow { int pos, limit, doc; float slope; const float* tab; const half_t* gtab; };
 
 // The rule on 16 scores of the lane's query: s[r] belongs to key jb + 4 g + 8 (r / 4) + r % 4.  Raw products
 // in, what p.cc turns into log2 units out.

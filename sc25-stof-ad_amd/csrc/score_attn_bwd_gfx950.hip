@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256) void score_attn_bwd_prep_kernel(const BwdParam
   } else {
     const int idx = blockIdx.x - s.B * s.Hq * nq, bh = idx / nk, t = idx - bh * nk;
     const int b = bh / s.Hkv, h = bh - b * s.Hkv;
-    const int klen = sample_keys(s, b);
+    const int klen = sample_of(s, b).keys;
     for (int x = 0; x < 64 / (4 * kR); ++x) {
       const int r = 64 * t + (4 * x + wave) * kR + lane / kC;
       if (r < klen && (!s.docs_k || s.docs_k[(int64_t)b * s.Sk + r] >= 0)) {
@@ -202,7 +202,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   if (!place(blockIdx.x, p.B * p.Hq, p.group, bp.q_tiles, bp.q_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, at)) return;
   const int bh = at.head, tile = bp.q_tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
-  const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
+  const Sample sample = sample_of(p, b);
+  const int klen = sample.keys, first = sample.first, prefix = sample.prefix;
   const int row0 = tile * 128 + 32 * wave, rows = min(p.Sq - row0, 32), i = row0 + j32;
   const bool docs = p.docs_q != nullptr;
   const int nqb = (p.Sq + kBlock - 1) / kBlock, nkb = (p.Sk + kBlock - 1) / kBlock;
@@ -474,7 +475,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
   const int bk = at.head, slot = at.rank;
   const int tile = slot / bp.splits, split = slot - tile * bp.splits;   // (causal: the first keys have most queries)
   const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
-  const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
+  const Sample sample = sample_of(p, b);
+  const int klen = sample.keys, first = sample.first, prefix = sample.prefix;
   const int key0 = tile * 128 + 32 * wave, keys = min(p.Sk - key0, 32), j = key0 + j32;
   const bool docs = p.docs_q != nullptr;
   const int nqb = (p.Sq + kBlock - 1) / kBlock, nkb = (p.Sk + kBlock - 1) / kBlock;

@@ -145,7 +145,8 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   const int bh = at.head, tile = p.tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
 
-  const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
+  const Sample sample = sample_of(p, b);
+  const int klen = sample.keys, first = sample.first, prefix = sample.prefix;
   const int row0 = tile * 128 + 32 * wave;               // this wave's first query
   const int rows = min(p.Sq - row0, 32);                 // (<= 0: none)
   const int i = row0 + j32;
@@ -350,7 +351,8 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
   const int tile = p.tiles - 1 - rest % p.tiles, bk = rest / p.tiles;
   const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
-  const int klen = sample_keys(p, b), first = sample_first(p, klen), prefix = sample_prefix(p, b);
+  const Sample sample = sample_of(p, b);
+  const int klen = sample.keys, first = sample.first, prefix = sample.prefix;
   const int r0 = tile * 32, rows = min(n_rows - r0, 32);
   const int r = min(r0 + j32, n_rows - 1), i = r / G, hg = r - i * G, h = hk * G + hg;
   const int i_lo = r0 / G, i_hi = (r0 + rows - 1) / G;
@@ -364,6 +366,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, true, -1) : 0;
   L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
   L.tab = tab + hg * n_tab;
+  L.gtab = p.table + (int64_t)h * (2 * p.radius + 1);
   half8_t qf[D / 16];
   {
     const half_t* src = p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)i * p.qs[2];
@@ -435,7 +438,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   constexpr int kAllButOne = (TL::kN & 15) | ((TL::kN >> 4) << 14) | 0x0F70;   // vmcnt: the loads of one tile may be out
   Step cur = next_step();
   if (cur.t >= 0) { issue_k(cur.t); issue_v(cur.t); }
-  if (p.bias_kind == kBiasTable) {      // (behind the first loads, whose latency it shares)
+  if (p.bias_kind == kBiasTable && p.table_in_lds) {      // (behind the first loads, whose latency it shares)
     for (int x = 0; x < G; ++x) load_table<BF>(p, hk * G + x, tab + x * n_tab, threadIdx.x, 64 * kRowWaves);
     __syncthreads();
   }
@@ -456,7 +459,16 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
     if (nxt.t >= 0) issue_k(nxt.t);
     const int j0 = cur.t * kRowKeys + 4 * g;
     if constexpr (CAP) cap_scores(p, s[0]);
-    if (p.bias_kind != kBiasNone) bias_scores<CAP>(p, L, j0, s[0]);
+    if (p.bias_kind == kBiasTable && !p.table_in_lds) {
+      // more heads share the cache than tables fit: entries straight from memory
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int x = min(max(j0 + key_off(r) - L.pos, -p.radius), p.radius) + p.radius;
+        s[0][r] = __builtin_fmaf(s[0][r], CAP ? 1.f : p.c, table_entry<BF>(L.gtab[x]));
+      }
+    } else if (p.bias_kind != kBiasNone) {
+      bias_scores<CAP>(p, L, j0, s[0]);
+    }
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
       if (docs) doc_scores(L, &doc_ids[wave][4 * g], s[0]);
@@ -607,14 +619,14 @@ namespace {
 
 struct Form { bool rows; int tiles, splits; };
 
-inline bool rows_fit(int group, int radius) { return radius < 0 || group * (2 * radius + 1 + 2 * kTabPad) * 4 <= 26 * 1024; }   // (beside 133 KB of tiles)
+// whether the tables of the heads that share a key head fit into LDS (beside 133 KB of tiles)
+inline bool tables_fit(int group, int radius) { return group * (2 * radius + 1 + 2 * kTabPad) * 4 <= 26 * 1024; }
 
-inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int form) {
+inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int form) {
   const int group = Hq / Hkv, cus = 256;
   const int64_t wide = (int64_t)B * Hq * ((Sq + 127) / 128);
   const int64_t rows = (int64_t)Sq * group;
   bool use_rows = form == 1 || (form < 0 && (rows <= 32 || wide < 96 || (wide <= 128 && Sk >= 2048)));
-  if (!rows_fit(group, radius)) use_rows = false;
   if (!use_rows) return Form{false, (Sq + 127) / 128, 1};
   const int tiles = (int)((rows + 31) / 32);
   const int64_t wgs = (int64_t)B * Hkv * tiles;
@@ -644,7 +656,7 @@ int score_attn_check(const void* const* req, int n_req, const int64_t* const* st
   if ((int64_t)B * Hq * ((Sq + 31) / 32) > 0x3fffffff || (int64_t)B * Hq * (int64_t)((Sk + 31) / 32) > 0x3fffffff || Sq > (1 << 29) || Sk > (1 << 29)) return STOF_ERR_BAD_SHAPE;
   if (D != 64 && D != 128) return STOF_ERR_UNSUPPORTED;
   if (dtype != STOF_DTYPE_F16 && dtype != STOF_DTYPE_BF16) return STOF_ERR_UNSUPPORTED;
-  if (!(scale > 0.f) || scale > 1e30f || !(cap >= 0.f) || cap > 1e30f || (cap > 0.f && cap < 1e-30f)) return STOF_ERR_UNSUPPORTED;
+  if (!(scale > 0.f) || scale > 1e6f || !(cap >= 0.f) || cap > STOF_SCORE_MAX_CAP || (cap > 0.f && cap < 1e-3f)) return STOF_ERR_UNSUPPORTED;
   if (radius > STOF_SCORE_MAX_RADIUS) return STOF_ERR_UNSUPPORTED;
   for (int i = 0; i < n_strides; ++i) {
     if (!strides[i]) return STOF_ERR_NULL_POINTER;
@@ -688,7 +700,7 @@ static void launch_form(ScoreParams& p, const Form& f, hipStream_t st) {
   const int n_tab = p.bias_kind == kBiasTable ? 2 * p.radius + 1 + 2 * kTabPad : 0;
   if (f.rows) {
     const unsigned grid = (unsigned)(p.B * p.Hkv) * (unsigned)p.tiles * (unsigned)p.splits;
-    score_attn_rows_kernel<D, BF, CAP><<<dim3(grid), dim3(64 * kRowWaves), (size_t)(p.group * n_tab) * 4, st>>>(p);
+    score_attn_rows_kernel<D, BF, CAP><<<dim3(grid), dim3(64 * kRowWaves), (size_t)(p.table_in_lds ? p.group * n_tab : 0) * 4, st>>>(p);
   } else {
     p.chunk = (p.B * p.Hq * p.tiles + 7) / 8;
     score_attn_wide_kernel<D, BF, CAP><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
@@ -703,9 +715,9 @@ static void launch_fwd(ScoreParams& p, const Form& f, hipStream_t st) {
   }
 }
 
-extern "C" int64_t stof_score_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int docs, int form) {
+extern "C" int64_t stof_score_attn_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs, int form) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Sk < 0 || Hq % Hkv != 0 || (D != 64 && D != 128)) return 0;
-  const Form f = pick_form(B, Hq, Hkv, Sq, Sk, D, radius, form);
+  const Form f = pick_form(B, Hq, Hkv, Sq, Sk, form);
   int64_t n = docs ? ranges_bytes(B, Sq, Sk) : 0;
   if (f.splits > 1) n += (int64_t)B * Hkv * f.tiles * f.splits * (32 * D + 64) * 4;
   return n;
@@ -728,9 +740,8 @@ extern "C" int stof_score_attn_fwd(const void* q, const void* k, const void* v, 
   if (q_end && !kv_len) return STOF_ERR_NULL_POINTER;
   if (q_start > (1 << 29) || q_start < -(1 << 29)) return STOF_ERR_BAD_SHAPE;
   if (form < -1 || form > 1) return STOF_ERR_UNSUPPORTED;
-  const Form f = pick_form(B, Hq, Hkv, Sq, Sk, D, table ? radius : -1, form);
-  if (form == 1 && !f.rows) return STOF_ERR_UNSUPPORTED;
-  const int64_t need = stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, table ? radius : -1, docs_q != nullptr, form);
+  const Form f = pick_form(B, Hq, Hkv, Sq, Sk, form);
+  const int64_t need = stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, docs_q != nullptr, form);
   if (need > 0) {
     if (!workspace) return STOF_ERR_NULL_POINTER;
     if (!stof_aligned16(workspace)) return STOF_ERR_MISALIGNED;
@@ -742,6 +753,7 @@ extern "C" int stof_score_attn_fwd(const void* q, const void* k, const void* v, 
   p.out = (half_t*)out; p.lse = lse;
   for (int j = 0; j < 3; ++j) p.os[j] = out_strides[j];
   p.tiles = f.tiles; p.splits = f.splits;
+  p.table_in_lds = table && tables_fit(p.group, radius);
   hipStream_t st = (hipStream_t)stream;
   if (docs_q) score_attn_ranges(p, workspace, st);
   p.part = (float*)((char*)workspace + (docs_q ? ranges_bytes(B, Sq, Sk) : 0));

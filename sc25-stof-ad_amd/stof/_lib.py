@@ -74,7 +74,7 @@ _SIGNATURES = {
                                                       c_float, _P, c_int64, c_int, c_int, _P]),
     "stof_gemm_bias_res_ln_cluster": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                                               c_float, _P, c_int64, _P]),
-    "stof_score_attn_workspace_bytes": (c_int64, [c_int] * 9),
+    "stof_score_attn_workspace_bytes": (c_int64, [c_int] * 8),
     "stof_score_attn_fwd": (c_int, [_P] * 11 + [c_float, c_float, c_int, c_int, c_int, c_int] + [POINTER(c_int64)] * 4 +
                             [c_int] * 8 + [_P, c_int64, _P]),
     "stof_score_attn_bwd_workspace_bytes": (c_int64, [c_int] * 8),

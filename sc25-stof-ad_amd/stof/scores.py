@@ -26,9 +26,10 @@ from . import _lib
 from ._lib import StofError, check
 from .ops import _DTYPES, _require, _stream
 
-__all__ = ["ScoreMask", "score_attn", "score_attn_backward", "MAX_RADIUS"]
+__all__ = ["ScoreMask", "score_attn", "score_attn_backward", "MAX_RADIUS", "MAX_CAP"]
 
 MAX_RADIUS = 1024
+MAX_CAP = 1024.0        # the cap is formed to 2^-22 of its size: a larger one would take more from the scores than 16-bit outputs show
 _FORMS = {None: -1, "auto": -1, "wide": 0, "rows": 1}
 
 
@@ -45,9 +46,9 @@ class ScoreMask:
 
     The tensors are read by the launches, not here: a serving loop keeps one object and writes new lengths
     into ``kv_len``.  Contents are not checked (that would synchronise); lengths are clamped to [0, Sk].
-    Keys past ``kv_len`` and keys without a document are never used as values, whatever they hold.  A
-    non-finite key or value that SOME query of a sample may attend to can reach other rows of its
-    64 x 64 tile, as it does in a dense product."""
+    Keys past ``kv_len``, keys that causality closes to every query of the sample and keys without a document are
+    never used as values, whatever they hold (the free part of a cache).  A non-finite key or value that SOME
+    query of a sample may attend to can reach other rows of its 64 x 64 tile, as it does in a dense product."""
 
     __slots__ = ("causal", "prefix", "kv_len", "docs_q", "docs_k", "q_start")
 
@@ -105,10 +106,10 @@ def _refuse(q, k, v, mask, scale, cap, bias, slopes):
         raise StofError(f"the number of query heads ({Hq}) must be a multiple of the number of key heads ({Hkv})")
     if D not in (64, 128):
         raise StofError(f"head size must be 64 or 128, got {D}")
-    if not 0.0 < scale < 1e30:
-        raise StofError(f"scale must be positive, got {scale}")
-    if cap != 0.0 and not 1e-30 < cap < 1e30:
-        raise StofError(f"cap must be positive, got {cap}")
+    if not 0.0 < scale <= 1e6:
+        raise StofError(f"scale must be positive and at most 1e6, got {scale}")
+    if cap != 0.0 and not 1e-3 <= cap <= MAX_CAP:
+        raise StofError(f"cap must be between 1e-3 and {MAX_CAP}, got {cap}")
     if bias is not None and slopes is not None:
         raise StofError("bias and slopes exclude each other")
     if bias is not None:
@@ -137,8 +138,8 @@ class _Rule:
         qt, kt, vt = q.stride(), k.stride(), v.stride()
         ok = (q.is_cuda and dtype in _DTYPES and len(qs) == 4 and len(ks) == 4 and vs == ks and qt[3] == 1 and kt[3] == 1 and vt[3] == 1
               and k.dtype == dtype and v.dtype == dtype and k.device == dev and v.device == dev and ks[0] == qs[0] and ks[3] == qs[3]
-              and ks[1] > 0 and qs[1] % ks[1] == 0 and (qs[3] == 64 or qs[3] == 128) and 0.0 < scale < 1e30
-              and (cap == 0.0 or 1e-30 < cap < 1e30))
+              and ks[1] > 0 and qs[1] % ks[1] == 0 and (qs[3] == 64 or qs[3] == 128) and 0.0 < scale <= 1e6
+              and (cap == 0.0 or 1e-3 <= cap <= MAX_CAP))
         radius = -1
         if ok and bias is not None:
             n = bias.shape
@@ -194,7 +195,7 @@ def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
         return out, lse
     lib = _lib.lib()
     docs_q = mask.docs_q
-    nbytes = lib.stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, r.radius, docs_q is not None, form)
+    nbytes = lib.stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, docs_q is not None, form)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None   # this call's own: calls may overlap on other streams and graphs
     qs, ks, vs = r.strides
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(lse), _at(bias), _at(slopes), _at(mask.prefix),

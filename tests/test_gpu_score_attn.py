@@ -120,7 +120,7 @@ def test_lengths_and_head_groups(Sq, Sk, Hq, Hkv, D, dtype):
 def test_table_radius(radius):
     q, k, v, dout = _qkv(1, 2, 1, 170, 230, 64, torch.float16, seed=4)
     bias = torch.randn(2, 2 * radius + 1, generator=_gen(radius)).to(torch.float16)
-    _run(q, k, v, dout, {}, bias=bias, forms=("wide", "rows") if radius < 1024 else ("wide",))
+    _run(q, k, v, dout, {}, bias=bias)
     q, k, v, dout = _qkv(1, 2, 1, 70, 70, 128, torch.bfloat16, seed=4)
     _run(q, k, v, dout, dict(causal=True), bias=bias.to(torch.bfloat16), forms=("wide",))
 
@@ -178,6 +178,50 @@ def test_what_no_query_may_use_is_not_read_as_a_value(form, D):
         _check(g, want[n], n)
 
 
+@pytest.mark.parametrize("form", ["wide", "rows"])
+def test_the_free_part_of_a_cache_behind_causality(form):
+    """No key length given: what causality closes to every query is not read as a value either."""
+    q, k, v, dout = _qkv(2, 2, 1, 40, 150, 64, torch.bfloat16, seed=18)
+    rule = dict(causal=True, q_start=60, prefix=torch.tensor([0, 110], dtype=torch.int32))
+    want = os_.score_attn(q, k, v, dout=dout, **rule)
+    for t in (k, v):
+        t[0, :, 100:] = math.nan
+        t[1, :, 110:] = math.inf
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out = score_attn(*leaves, _mask(rule), launch_form=form)
+    _check(out, want["out"], "out")
+    for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout.cuda())):
+        _check(g, want[n], n)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,S,D", [(4, 4, 2, 300, 64), (8, 2, 1, 520, 128), (1, 16, 8, 260, 64), (2, 8, 8, 200, 64)])
+def test_causal_work_placed_over_the_xcds(B, Hq, Hkv, S, D):
+    """Key heads that divide over the eight XCDs: every tile of every head exactly once."""
+    q, k, v, dout = _qkv(B, Hq, Hkv, S, S, D, torch.float16, seed=19)
+    _run(q, k, v, dout, dict(causal=True))
+    _run(q, k, v, dout, dict(kv_len=torch.randint(0, S + 1, (B,), generator=_gen(S), dtype=torch.int32)))
+
+
+def test_gradient_of_an_expanded_scalar_and_of_broadcast_keys():
+    """out.sum() hands an expanded gradient back; one key head expanded over four collects the sum of their gradients."""
+    q, k, v, _ = _qkv(2, 4, 1, 50, 70, 64, torch.float16, seed=20)
+    want = os_.score_attn(q, k, v, dout=torch.ones_like(q))
+    lq, lk, lv = (t.cuda().requires_grad_() for t in (q, k, v))
+    score_attn(lq, lk, lv).sum().backward()
+    for t, n in ((lq, "dq"), (lk, "dk"), (lv, "dv")):
+        _check(t.grad, want[n], n)
+    lk2, lv2 = (t.cuda().requires_grad_() for t in (k, v))
+    out = score_attn(q.cuda(), lk2.expand(2, 4, 70, 64), lv2.expand(2, 4, 70, 64))
+    _check(out, want["out"], "out")
+    out.sum().backward()
+    # (four rounded gradients summed by autograd in fp16: three more roundings of at most half a step of the largest partial sum)
+    for got, n in ((lk2.grad, "dk"), (lv2.grad, "dv")):
+        value, bound = want[n]
+        parts = os_.score_attn(q, k.expand(2, 4, 70, 64), v.expand(2, 4, 70, 64), dout=torch.ones_like(q))[n]
+        room = parts[1].sum(1, keepdim=True) + 3 * 2.0 ** -11 * parts[0].abs().sum(1, keepdim=True)
+        _check(got, (value, room), n)
+
+
 @pytest.mark.parametrize("dscale", [2.0 ** -12, 1.0, 4096.0])
 def test_fp16_gradients_of_small_and_large_losses(dscale):
     """A loss scaled by a power of two scales every gradient by it, inside the range of the format."""
@@ -233,7 +277,7 @@ def test_single_tokens(B, Hq, Hkv, D, Sk, what):
         kw["bias"] = torch.randn(Hq, 2 * 64 + 1, generator=_gen(1)).to(dtype)
     if what == "slopes":
         kw["slopes"] = torch.rand(Hq, generator=_gen(1)) * 0.05
-    _run(q, k, v, None, dict(kv_len=kv_len, q_start="end"), train=False, forms=(None, "wide", "rows") if what != "table" or Hq // Hkv < 16 else (None, "wide"), **kw)
+    _run(q, k, v, None, dict(kv_len=kv_len, q_start="end"), train=False, forms=(None, "wide", "rows"), **kw)
 
 
 def test_a_sequence_token_by_token_equals_the_whole():

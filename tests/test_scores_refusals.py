@@ -57,15 +57,16 @@ def test_forward_argument_checks(lib):
     for kw in (dict(B=0), dict(Hq=3), dict(Sq=0), dict(Sk=-1), dict(B=1 << 20, Hq=1 << 10, Sq=1 << 20), dict(start=1 << 30), dict(table=P)):
         assert call(**kw) == -2, kw
     for kw in (dict(D=96), dict(dtype=2), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(cap=-1.0), dict(cap=float("inf")),
-               dict(table=P, radius=1025), dict(table=P, radius=4, slopes=P), dict(form=2), dict(table=P, radius=1024, Hq=64, form=1)):
+               dict(cap=1025.0), dict(cap=1e-4), dict(scale=1e7),
+               dict(table=P, radius=1025), dict(table=P, radius=4, slopes=P), dict(form=2)):
         assert call(**kw) == -3, kw
     assert call(dq=P) == -1 and call(end=1) == -1
     assert call(dq=P, dk=P) == -1                                  # documents need a workspace
     assert call(dq=P, dk=P, ws=P, bytes=8) == -2
-    assert h.stof_score_attn_workspace_bytes(2, 4, 2, 8, 8, 64, -1, 0, -1) == 0
-    assert h.stof_score_attn_workspace_bytes(2, 4, 2, 100, 200, 64, -1, 1, 0) == 2 * (2 + 4) * 16
-    assert h.stof_score_attn_workspace_bytes(1, 8, 2, 1, 100000, 64, -1, 0, -1) > 0     # split along the keys
-    assert h.stof_score_attn_workspace_bytes(2, 4, 3, 8, 8, 64, -1, 0, -1) == 0
+    assert h.stof_score_attn_workspace_bytes(2, 4, 2, 8, 8, 64, 0, -1) == 0
+    assert h.stof_score_attn_workspace_bytes(2, 4, 2, 100, 200, 64, 1, 0) == 2 * (2 + 4) * 16
+    assert h.stof_score_attn_workspace_bytes(1, 8, 2, 1, 100000, 64, 0, -1) > 0     # split along the keys
+    assert h.stof_score_attn_workspace_bytes(2, 4, 3, 8, 8, 64, 0, -1) == 0
 
 
 def test_backward_argument_checks(lib):
