@@ -438,7 +438,7 @@ int check_sizes(int64_t M, int64_t N, int64_t K, int dtype) {
 int check_common(const void* wq, const float* sw, const void* bias, const void* out, int64_t K, int64_t N, int64_t ldw, int64_t ldo, int act) {
   if (!wq || !sw || !out) return STOF_ERR_NULL_POINTER;
   if (!stof_aligned16(wq) || !stof_aligned16(sw) || !stof_aligned16(out) || (bias && !stof_aligned16(bias))) return STOF_ERR_MISALIGNED;
-  if (ldw < K || ldo < N || ldw > (1 << 23) || ldo > (1 << 22)) return STOF_ERR_BAD_SHAPE;    // 128 rows of a tile stay below 2^31 bytes
+  if (ldw < K || ldo < N || ldw > (1 << 23) || ldo > (1 << 22)) return STOF_ERR_BAD_SHAPE;    // 256 rows of a tile stay below 2^31 bytes
   if (ldw % 16 != 0 || ldo % 8 != 0) return STOF_ERR_MISALIGNED;
   if (act < STOF_ACT_NONE || act > STOF_ACT_RELU) return STOF_ERR_UNSUPPORTED;
   return STOF_OK;

@@ -820,7 +820,7 @@ __global__ __launch_bounds__(256) void score_attn_bwd_join_kernel(const float* p
 // tile, until 512 workgroups (two per compute unit) have work of at least four tiles each; their fp32 sums are
 // joined by one more kernel.  B2 H16/4 S2048 D128 causal, 128 workgroups: 246 us unsplit, 103 + 12 us with four
 // splits; B8 H12 S512 D64 with a table, 384 workgroups: 51 + 4 us unsplit, 44 + 18 us with two.
-int key_splits(int B, int Hkv, int Sq, int Sk, int group, int D) {
+int key_splits(int B, int Hkv, int Sq, int Sk, int group) {
   const int64_t wgs = (int64_t)B * Hkv * ((Sk + 127) / 128);
   const int64_t want = 512;
   const int most = ((Sq + 63) / 64 * group + 3) / 4;
@@ -840,7 +840,7 @@ Layout layout(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int doc
   l.domax = l.stats + up((int64_t)B * Hq * nq * 64 * 8);
   l.vmax = l.domax + up((int64_t)B * Hq * nq * 4);
   l.part = l.vmax + up((int64_t)B * Hkv * nk * 4);
-  const int splits = key_splits(B, Hkv, Sq, Sk, Hq / Hkv, D);
+  const int splits = key_splits(B, Hkv, Sq, Sk, Hq / Hkv);
   l.kv = l.part + (radius >= 0 ? up((int64_t)B * Hq * kt * splits * (2 * radius + 1) * 4) : 0);
   l.total = l.kv + (splits > 1 ? 2 * splits * up((int64_t)B * Hkv * Sk * D * 4) : 0);
   return l;
@@ -907,8 +907,8 @@ extern "C" int stof_score_attn_bwd(const void* dout, const void* q, const void* 
   p.stats = (floatx2_t*)(ws + l.stats); p.domax = (float*)(ws + l.domax); p.vmax = (float*)(ws + l.vmax); p.tab_part = (float*)(ws + l.part);
   p.scale = scale;
   p.q_tiles = (Sq + 127) / 128; p.k_tiles = (Sk + 127) / 128;
-  p.q_chunk = (B * Hq * p.q_tiles + 7) / 8; 
-  p.splits = key_splits(B, Hkv, Sq, Sk, Hq / Hkv, D);
+  p.q_chunk = (B * Hq * p.q_tiles + 7) / 8;
+  p.splits = key_splits(B, Hkv, Sq, Sk, Hq / Hkv);
   p.kv_part = (float*)(ws + l.kv);
   p.k_chunk = (B * Hkv * p.k_tiles * p.splits + 7) / 8;
   hipStream_t st = (hipStream_t)stream;

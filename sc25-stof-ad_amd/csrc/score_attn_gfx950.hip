@@ -126,7 +126,7 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
 }
 
 // CAP is a template argument: with the cap behind a run-time branch the compiler computes it speculatively for every
-// tile (32 transcendental operations of 16 cycles per 64 keys and wave beside the 32 of the softmax).
+// tile (64 transcendental operations a lane and tile beside the 32 of the softmax).
 template <int D, bool BF, bool CAP>
 __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScoreParams p) {
   typedef TileLoad<D, kBlock, 4> TL;
@@ -500,10 +500,10 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   float l = 0.f;
 #pragma unroll
   for (int w = 0; w < kRowWaves; ++w) {
-    const float mw = stats[w][0][lane];
-    l += mw == -INFINITY ? 0.f : stats[w][1][lane] * __builtin_amdgcn_exp2f(mw - m);
+    // (a wave that saw no key has the sum 0; one that saw only NaN has the maximum -inf too, and the sum NaN, which must stay)
+    const float lw = stats[w][1][lane];
+    l += lw == 0.f ? 0.f : lw * __builtin_amdgcn_exp2f(stats[w][0][lane] - m);
   }
-  // (a NaN maximum does not arise: fmaxf drops NaN; a NaN score makes the sum NaN)
   const float f = sm.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm.m - m);
   constexpr int kRegs = D / 2;                          // registers of O: index 16 dt + x
   constexpr int kHalf = kRegs / 2;
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams 
 #pragma unroll
     for (int x = 0; x < kC; ++x) {
       const float v = base[s * kSlot + j * D + kC * lane + x];
-      o[x] += f == 0.f ? 0.f : f * v;                   // (a split that saw no key wrote zeros; its maximum is -inf)
+      o[x] += f == 0.f ? 0.f : f * v;                   // (a split that saw no key, or only NaN: then l is NaN)
     }
   }
 #pragma unroll

@@ -297,7 +297,7 @@ def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None,
     fp16 or, all alike, bfloat16, head size 64 or 128, any lengths, unit stride in D and other strides
     multiples of 8.  ``mask``: a ``ScoreMask`` (None: every key).  ``scale``: default ``1/sqrt(D)``.
     ``bias``: learned distance table ``[Hq, 2R+1]`` of q's dtype, R up to 1024; ``slopes``: fp32 ``[Hq]``, constants.
-    Returns ``[B,Hq,Sq,D]`` (``out_layout="bhsd"``) or ``[B,Sq,Hq*D]`` (``"bshd"``), with ``return_lse`` also the
+    ``out`` must not overlap the inputs.  Returns ``[B,Hq,Sq,D]`` (``out_layout="bhsd"``) or ``[B,Sq,Hq*D]`` (``"bshd"``), with ``return_lse`` also the
     logarithm of the softmax's denominator, fp32 ``[B,Hq,Sq]``.  Differentiable in q, k, v and bias (through the
     output, not through lse).  ``launch_form``: None, "wide" (128-query tiles) or "rows" (32-row tiles with the
     keys split; single tokens and small grids) - the rule by sizes is in the library."""

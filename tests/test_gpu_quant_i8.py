@@ -179,6 +179,21 @@ def test_batch_dims_strides_and_guard_rows():
     _close(linear_i8(odd, w.cuda(), ws.cuda(), b.cuda()), _want(*_quant64(odd.cpu()), w, ws, b, "none", torch.float16))
 
 
+def test_two_streams_at_once():
+    w, ws, b = (t.cuda() for t in _weights(520, 272, torch.float16, 18))
+    xs = [torch.randn(m, 272, generator=_gen(m)).half().cuda() for m in (300, 333)]
+    want = [linear_i8(x, w, ws, b) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(linear_i8(xs[n], w, ws, b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[n]) for n in range(2) for g in got[n])
+
+
 def test_captured_graphs_replayed_together():
     w, ws, b = (t.cuda() for t in _weights(512, 256, torch.float16, 8))
     for M in (1, 100):

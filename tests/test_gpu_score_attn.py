@@ -194,6 +194,59 @@ def test_the_free_part_of_a_cache_behind_causality(form):
         _check(g, want[n], n)
 
 
+@pytest.mark.parametrize("form", ["wide", "rows"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_nan_in_an_allowed_place_reaches_its_rows(form, D):
+    """A query of NaN, and a NaN key that is the only one of its tile and split: NaN out and NaN lse, never a number."""
+    q, k, v, _ = (t.cuda() for t in _qkv(2, 4, 2, 1, 8192, D, torch.float16, seed=21))
+    q[0, 1] = math.nan
+    for n in (8192, 257, 5):
+        out, lse = score_attn(q, k, v, ScoreMask(kv_len=torch.full((2,), n, dtype=torch.int32, device="cuda")), launch_form=form, return_lse=True)
+        bad = torch.zeros(2, 4, 1, dtype=torch.bool, device="cuda")
+        bad[0, 1] = True
+        assert torch.equal(out.isnan().all(-1), bad) and torch.equal(out.isnan().any(-1), bad) and torch.equal(lse.isnan(), bad)
+    k[1, 0, 256] = math.nan
+    out, lse = score_attn(q, k, v, ScoreMask(kv_len=torch.full((2,), 257, dtype=torch.int32, device="cuda")), launch_form=form, return_lse=True)
+    bad[1, :2] = True
+    assert torch.equal(out.isnan().all(-1), bad) and torch.equal(out.isnan().any(-1), bad) and torch.equal(lse.isnan(), bad)
+
+
+def test_one_tensor_in_all_three_places():
+    x, _, _, dout = _qkv(2, 3, 3, 90, 90, 64, torch.float16, seed=22)
+    want = os_.score_attn(x, x, x, dout=dout, causal=True)
+    leaf = x.cuda().requires_grad_()
+    out = score_attn(leaf, leaf, leaf, ScoreMask(causal=True))
+    _check(out, want["out"], "out")
+    out.backward(dout.cuda())
+    # (three rounded gradients summed by autograd in fp16: two more roundings of at most half a step of the partial sums)
+    parts = [want[n] for n in ("dq", "dk", "dv")]
+    room = sum(p[1] for p in parts) + 2 * 2.0 ** -11 * sum(p[0].abs() for p in parts)
+    _check(leaf.grad, (sum(p[0] for p in parts), room), "dx")
+
+
+def test_training_steps_on_two_streams_at_once():
+    """Forward and backward passes that overlap on two streams: workspaces are each call's own."""
+    sets = [[t.cuda() for t in _qkv(2, 8, 2, 300, 300, 64, torch.float16, seed=s)] for s in (23, 24)]
+    bias = torch.randn(8, 129, generator=_gen(5)).half().cuda()
+    docs = (torch.arange(300, dtype=torch.int32) // 70).expand(2, 300).contiguous().cuda()
+
+    def step(t):
+        out, lse = score_attn(*t[:3], ScoreMask(causal=True, docs=docs), bias=bias, return_lse=True)
+        return (out,) + score_attn_backward(t[3], *t[:3], out, lse, ScoreMask(causal=True, docs=docs), bias=bias)
+    want = [step(t) for t in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(step(sets[n]))
+    torch.cuda.synchronize()
+    for n in range(2):
+        for g in got[n]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[n]))
+
+
 @pytest.mark.parametrize("B,Hq,Hkv,S,D", [(4, 4, 2, 300, 64), (8, 2, 1, 520, 128), (1, 16, 8, 260, 64), (2, 8, 8, 200, 64)])
 def test_causal_work_placed_over_the_xcds(B, Hq, Hkv, S, D):
     """Key heads that divide over the eight XCDs: every tile of every head exactly once."""
