@@ -428,7 +428,7 @@ int stof_gemm_bias_res_ln_cluster_dt(const void* A, const void* Wt, const void* 
  * A row without allowed keys gives zeros and lse = -inf.  prefix, kv_len (clamped to [0, Sk]), docs_*:
  * int32, each may be NULL; they are read by the launch, not before.  Keys at or past kv_len, keys that causality
  * closes to every query of the sample and keys of a negative document are not used as values, whatever they hold
- * (NaN included).  scale in (0, 1e6], cap 0 or in [1e-3, 1024].
+ * (NaN included).  scale in [1e-6, 1e6], cap 0 or in [1e-3, 1024].
  * Strides: (batch, head, row) in elements, multiples of 8, rows at most 2^23; pointers 16-byte aligned.
  * lse [B, Hq, Sq] fp32 may be NULL.  form: -1 the library's choice, 0 128-query tiles, 1 32-row tiles with
  * the keys split over waves and workgroups.  The workspace (bytes below, 0 = none) needs no initial

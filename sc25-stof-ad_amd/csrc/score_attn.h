@@ -48,11 +48,11 @@ struct ScoreParams {
   const int* docs_q; const int* docs_k;    // [B, Sq], [B, Sk], or NULL
   const DocRange* dr_q; const DocRange* dr_k;   // [B, ceil(Sq / 64)], [B, ceil(Sk / 64)]
   int B, Hq, Hkv, Sq, Sk;
-  int radius, bias_kind, causal;
+  int radius, causal;
   int q_start, q_end;                      // p_0 = q_start, or kv_len - Sq with q_end
   int tiles, chunk, cus_per_xcd;           // workgroups per (batch, head); workgroups per XCD; compute units of an XCD
   float c, k1, capl;                       // scale log2e; 2 scale log2e / cap (0: no cap); cap log2e
-  float cc;                                // what turns a rule's result into log2 units: c when it is the raw product, else 1
+  float cc, slope_mul;                     // what turns a rule's result into log2 units: c when it is in units of the raw product, else 1; slopes to the rule's units
   // form for few rows
   int splits, group, table_in_lds; float* part;
 };
@@ -232,18 +232,21 @@ __device__ __forceinline__ void cap_scores(const ScoreParams& p, floatx16& s) {
     s[r] = __builtin_fmaf(u, -2.f * p.capl, p.capl);
   }
 }
-template <bool CAP>
+// The kind of bias is a template argument: behind run-time branches every kind's result is copied to common registers (D
+// = 64 without a bias: 32 moves for 190 other vector instructions a tile).  Slopes stay in units of the raw product
+// (L.slope has p.slope_mul in it), so that a score costs an addition and a multiply-add.
+template <bool CAP, int BIAS>
 __device__ __forceinline__ void bias_scores(const ScoreParams& p, const LaneRow& L, int j0 /* jb + 4 g */, floatx16& s) {
-  const float mul = CAP ? 1.f : p.c;
-  if (p.bias_kind == kBiasTable) {
+  if constexpr (BIAS == kBiasTable) {
+    const float mul = CAP ? 1.f : p.c;
     const int x = min(max(j0 - L.pos, -p.radius - kTabPad), p.radius);
     const float* t = L.tab + (x + p.radius + kTabPad);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, t[key_off(r)]);
-  } else if (p.bias_kind == kBiasSlopes) {
+  } else if constexpr (BIAS == kBiasSlopes) {
     const float x = (float)(j0 - L.pos);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, -L.slope * __builtin_fabsf(x + (float)key_off(r)));
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(__builtin_fabsf(x + (float)key_off(r)), -L.slope, s[r]);
   }
 }
 __device__ __forceinline__ void limit_scores(const LaneRow& L, int j0, floatx16& s) {

@@ -185,7 +185,7 @@ __device__ __forceinline__ void store_rows(const floatx16 (&o)[D / 32], float mu
 // delta' = sum_j P_ij dP_ij is formed along the way in fp32, and with M = P (1 - tanh^2) K as one product more
 //     dQ = scale (dT(delta) K - (delta' - delta) M)
 // is exact in delta while the second term stays small.  delta' replaces delta for the kernel of the keys.
-template <int D, bool BF, bool CAP>
+template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;
   typedef TileLoad<D, kBlock, 4> TL;
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   L.pos = first + i;
   L.limit = row_limit(p.causal, klen, prefix, L.pos);
   L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, i < p.Sq, -1) : 0;
-  L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
+  L.slope = BIAS == kBiasSlopes ? p.slopes[h] * p.slope_mul : 0.f;
   L.tab = tab;
   floatx2_t st = {INFINITY, 0.f};
   if (i < p.Sq) st = bp.stats[(int64_t)bh * (64 * nqb) + i];
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
     auto rule = [&](int mt) {
       const int j0 = cur.t * kBlock + 32 * mt + 4 * g;
       if constexpr (CAP) cap_scores_grad(p, s[mt], w[mt]);
-      if (p.bias_kind != kBiasNone) bias_scores<CAP>(p, L, j0, s[mt]);
+      bias_scores<CAP, BIAS>(p, L, j0, s[mt]);
       if (!cur.full) {
         limit_scores(L, j0, s[mt]);
         if (docs) doc_scores(L, &doc_ids[wave][32 * mt + 4 * g], s[mt]);
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   };
   Step cur = next_step();
   if (cur.t >= 0) issue(cur.t, (lds_byte*)k0, (lds_byte*)v0);
-  if (p.bias_kind == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);   // (the walk's first barrier covers it)
+  if constexpr (BIAS == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);   // (the walk's first barrier covers it)
   while (cur.t >= 0) {
     Step nxt = next_step();
     step(cur, nxt, (lds_byte*)k0, (lds_byte*)v0, (lds_byte*)k1, (lds_byte*)v1);
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(1024) void score_attn_bwd_table_kernel(const BwdPar
 // the wave's own array; diagonals that clip, and pieces that lie beyond the radius as a whole, are
 // added in two registers per lane.  After each head the waves' arrays are joined and written to the
 // workspace, which a last kernel adds up over batch and key tiles.
-template <int D, bool BF, bool CAP, bool TAB>
+template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;
   typedef TileLoad<D, kBlock, 4> TL;
@@ -465,6 +465,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
   __shared__ int doc_ids[4][kBlock];
   __shared__ __attribute__((aligned(16))) float st_lse[4][kBlock];
   __shared__ __attribute__((aligned(16))) float st_del[4][kBlock];
+  constexpr bool TAB = BIAS == kBiasTable;
   __shared__ float skew[TAB ? 4 : 1][TAB ? 32 + 32 * 33 + 32 : 1];
   extern __shared__ float tab[];                // kBiasTable: the head's table, then 2 R + 1 sums per wave
 
@@ -629,7 +630,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
       load_table<BF>(p, hk * p.group + cur.head, tab, threadIdx.x, 256);
       table_head = cur.head;
     }
-    if (p.bias_kind == kBiasSlopes) slope = p.slopes[hk * p.group + cur.head] * kLog2e;
+    if constexpr (BIAS == kBiasSlopes) slope = p.slopes[hk * p.group + cur.head] * p.slope_mul;
     __syncthreads();
     if (nxt.t >= 0) issue(nxt, qn, dn);
     if (!cur.mine) return;
@@ -667,18 +668,18 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
       x[mt][r >> 3][r & 7] = to_elem<BF>(BF ? d : d * up);
     };
     auto rule = [&](int mt) {
-      const float mul = CAP ? 1.f : p.c;
       const int pos0 = first + cur.t * kBlock + 32 * mt + 4 * g;    // position of the lane's score 0; score r: + key_off(r)
       if constexpr (CAP) cap_scores_grad(p, s[mt], w[mt]);
       if constexpr (TAB) {
         const int at = min(max(j - pos0, -p.radius), p.radius + kTabPad);   // distance j - p falls with the row
         const float* t = tab + (at + p.radius + kTabPad);
+        const float mul = CAP ? 1.f : p.c;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], mul, t[-key_off(r)]);
-      } else if (p.bias_kind == kBiasSlopes) {
+      } else if constexpr (BIAS == kBiasSlopes) {
         const float at = (float)(j - pos0);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], mul, -slope * __builtin_fabsf(at - (float)key_off(r)));
+        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(__builtin_fabsf(at - (float)key_off(r)), -slope, s[mt][r]);
       }
       if (!cur.full) {
         const int rel = from - pos0;
@@ -846,26 +847,30 @@ Layout layout(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int doc
   return l;
 }
 
-template <int D, bool BF, bool CAP>
+template <int D, bool BF, bool CAP, int BIAS>
 void launch_main(BwdParams& p, hipStream_t st) {
-  const ScoreParams& s = p.s;
-  const int n_tab = s.bias_kind == kBiasTable ? 2 * s.radius + 1 + 2 * kTabPad : 0;
+  const int n_dist = BIAS == kBiasTable ? 2 * p.s.radius + 1 : 0, n_tab = BIAS == kBiasTable ? n_dist + 2 * kTabPad : 0;
   const unsigned gq = 8u * (unsigned)p.q_chunk, gk = 8u * (unsigned)p.k_chunk;
-  score_attn_bwd_q_kernel<D, BF, CAP><<<dim3(gq), dim3(256), (size_t)n_tab * 4, st>>>(p);
-  if (n_tab) score_attn_bwd_k_kernel<D, BF, CAP, true><<<dim3(gk), dim3(256), (size_t)(n_tab + 4 * (2 * s.radius + 1)) * 4, st>>>(p);
-  else score_attn_bwd_k_kernel<D, BF, CAP, false><<<dim3(gk), dim3(256), 0, st>>>(p);
+  score_attn_bwd_q_kernel<D, BF, CAP, BIAS><<<dim3(gq), dim3(256), (size_t)n_tab * 4, st>>>(p);
+  score_attn_bwd_k_kernel<D, BF, CAP, BIAS><<<dim3(gk), dim3(256), (size_t)(n_tab + 4 * n_dist) * 4, st>>>(p);
+}
+template <int D, bool BF, bool CAP>
+void launch_bias(BwdParams& p, hipStream_t st) {
+  if (p.s.table) launch_main<D, BF, CAP, kBiasTable>(p, st);
+  else if (p.s.slopes) launch_main<D, BF, CAP, kBiasSlopes>(p, st);
+  else launch_main<D, BF, CAP, kBiasNone>(p, st);
 }
 template <int D, bool BF>
 void launch_bwd(BwdParams& p, hipStream_t st) {
   const ScoreParams& s = p.s;
   const int nq = (s.Sq + 63) / 64, nk = (s.Sk + 63) / 64;
   score_attn_bwd_prep_kernel<D, BF><<<dim3((unsigned)(s.B * s.Hq * nq + (BF ? 0 : s.B * s.Hkv * nk))), dim3(256), 0, st>>>(p);
-  s.k1 != 0.f ? launch_main<D, BF, true>(p, st) : launch_main<D, BF, false>(p, st);
+  s.k1 != 0.f ? launch_bias<D, BF, true>(p, st) : launch_bias<D, BF, false>(p, st);
   if (p.splits > 1) {
     const int64_t n = (int64_t)s.B * s.Hkv * s.Sk * D;
     score_attn_bwd_join_kernel<BF><<<dim3((unsigned)((2 * n / 8 + 255) / 256)), dim3(256), 0, st>>>(p.kv_part, p.dk, p.dv, n, p.splits);
   }
-  if (s.bias_kind == kBiasTable)
+  if (s.table)
     score_attn_bwd_table_kernel<BF><<<dim3((unsigned)((2 * s.radius + 64) / 64), (unsigned)s.Hq), dim3(1024), 0, st>>>(p);
 }
 

@@ -127,7 +127,7 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
 
 // CAP is a template argument: with the cap behind a run-time branch the compiler computes it speculatively for every
 // tile (64 transcendental operations a lane and tile beside the 32 of the softmax).
-template <int D, bool BF, bool CAP>
+template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScoreParams p) {
   typedef TileLoad<D, kBlock, 4> TL;
   __shared__ __attribute__((aligned(1024))) unsigned char k0[TL::kBytes];
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   L.pos = first + i;
   L.limit = row_limit(p.causal, klen, prefix, L.pos);
   L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, i < p.Sq, -1) : 0;
-  L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
+  L.slope = BIAS == kBiasSlopes ? p.slopes[h] * p.slope_mul : 0.f;
   L.tab = tab;
 
   // Q^T as the B operand: lane (query j32, group g) holds 8 consecutive d per step; rows past the end re-read the last
@@ -272,7 +272,8 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
     }
     const int j0 = cur.t * kBlock + 4 * g;
     if constexpr (CAP) { cap_scores(p, s[0]); cap_scores(p, s[1]); }
-    if (p.bias_kind != kBiasNone) { bias_scores<CAP>(p, L, j0, s[0]); bias_scores<CAP>(p, L, j0 + 32, s[1]); }
+    bias_scores<CAP, BIAS>(p, L, j0, s[0]);
+    bias_scores<CAP, BIAS>(p, L, j0 + 32, s[1]);
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
       limit_scores(L, j0 + 32, s[1]);
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   Step cur = next_step();
   if (cur.t >= 0) issue(cur.t, (lds_byte*)k0, (lds_byte*)v0);
   // (behind the first tile's loads, whose latency it shares; the walk's first barrier covers it)
-  if (p.bias_kind == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);
+  if constexpr (BIAS == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);
   while (cur.t >= 0) {
     Step nxt = next_step();
     step(cur, nxt, (lds_byte*)k0, (lds_byte*)v0, (lds_byte*)k1, (lds_byte*)v1);
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
 constexpr int kRowKeys = 32;
 constexpr int kRowWaves = 8;
 
-template <int D, bool BF, bool CAP>
+template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(const ScoreParams p) {
   typedef TileLoad<D, kRowKeys, 1> TL;
   __shared__ __attribute__((aligned(1024))) unsigned char k_lds[kRowWaves * TL::kBytes];
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   L.pos = first + i;
   L.limit = row_limit(p.causal, klen, prefix, L.pos);
   L.doc = docs ? doc_at(p.docs_q, (int64_t)b * p.Sq + i, true, -1) : 0;
-  L.slope = p.bias_kind == kBiasSlopes ? p.slopes[h] * kLog2e : 0.f;
+  L.slope = BIAS == kBiasSlopes ? p.slopes[h] * p.slope_mul : 0.f;
   L.tab = tab + hg * n_tab;
   L.gtab = p.table + (int64_t)h * (2 * p.radius + 1);
   half8_t qf[D / 16];
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
   constexpr int kAllButOne = (TL::kN & 15) | ((TL::kN >> 4) << 14) | 0x0F70;   // vmcnt: the loads of one tile may be out
   Step cur = next_step();
   if (cur.t >= 0) { issue_k(cur.t); issue_v(cur.t); }
-  if (p.bias_kind == kBiasTable && p.table_in_lds) {      // (behind the first loads, whose latency it shares)
+  if (BIAS == kBiasTable && p.table_in_lds) {      // (behind the first loads, whose latency it shares)
     for (int x = 0; x < G; ++x) load_table<BF>(p, hk * G + x, tab + x * n_tab, threadIdx.x, 64 * kRowWaves);
     __syncthreads();
   }
@@ -459,15 +460,15 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
     if (nxt.t >= 0) issue_k(nxt.t);
     const int j0 = cur.t * kRowKeys + 4 * g;
     if constexpr (CAP) cap_scores(p, s[0]);
-    if (p.bias_kind == kBiasTable && !p.table_in_lds) {
+    if (BIAS == kBiasTable && !p.table_in_lds) {
       // more heads share the cache than tables fit: entries straight from memory
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int x = min(max(j0 + key_off(r) - L.pos, -p.radius), p.radius) + p.radius;
         s[0][r] = __builtin_fmaf(s[0][r], CAP ? 1.f : p.c, table_entry<BF>(L.gtab[x]));
       }
-    } else if (p.bias_kind != kBiasNone) {
-      bias_scores<CAP>(p, L, j0, s[0]);
+    } else {
+      bias_scores<CAP, BIAS>(p, L, j0, s[0]);
     }
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
@@ -656,7 +657,7 @@ int score_attn_check(const void* const* req, int n_req, const int64_t* const* st
   if ((int64_t)B * Hq * ((Sq + 31) / 32) > 0x3fffffff || (int64_t)B * Hq * (int64_t)((Sk + 31) / 32) > 0x3fffffff || Sq > (1 << 29) || Sk > (1 << 29)) return STOF_ERR_BAD_SHAPE;
   if (D != 64 && D != 128) return STOF_ERR_UNSUPPORTED;
   if (dtype != STOF_DTYPE_F16 && dtype != STOF_DTYPE_BF16) return STOF_ERR_UNSUPPORTED;
-  if (!(scale > 0.f) || scale > 1e6f || !(cap >= 0.f) || cap > STOF_SCORE_MAX_CAP || (cap > 0.f && cap < 1e-3f)) return STOF_ERR_UNSUPPORTED;
+  if (!(scale >= 1e-6f) || scale > 1e6f || !(cap >= 0.f) || cap > STOF_SCORE_MAX_CAP || (cap > 0.f && cap < 1e-3f)) return STOF_ERR_UNSUPPORTED;
   if (radius > STOF_SCORE_MAX_RADIUS) return STOF_ERR_UNSUPPORTED;
   for (int i = 0; i < n_strides; ++i) {
     if (!strides[i]) return STOF_ERR_NULL_POINTER;
@@ -677,14 +678,14 @@ void score_attn_params(ScoreParams& p, const void* q, const void* k, const void*
   p.docs_q = (const int*)docs_q; p.docs_k = (const int*)docs_k;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.group = Hq / Hkv;
   p.radius = radius < 0 ? 0 : radius;
-  p.bias_kind = table ? kBiasTable : slopes ? kBiasSlopes : kBiasNone;
   p.causal = causal != 0; p.q_start = q_start; p.q_end = q_end != 0;
   p.c = scale * kLog2e;
   p.k1 = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
   p.capl = cap * kLog2e;
   int cus = stof_device_compute_units();
   p.cus_per_xcd = cus >= 8 ? cus / 8 : 32;
-  p.cc = (cap > 0.f || p.bias_kind != kBiasNone) ? 1.f : p.c;
+  p.cc = (cap > 0.f || table) ? 1.f : p.c;
+  p.slope_mul = cap > 0.f ? kLog2e : 1.f / scale;
 }
 
 void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st) {
@@ -695,20 +696,26 @@ void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st) {
   doc_ranges_kernel<<<dim3((unsigned)(p.B * (nq + nk))), dim3(64), 0, st>>>(p.docs_q, p.docs_k, dq, dk, p.B, p.Sq, p.Sk);
 }
 
-template <int D, bool BF, bool CAP>
+template <int D, bool BF, bool CAP, int BIAS>
 static void launch_form(ScoreParams& p, const Form& f, hipStream_t st) {
-  const int n_tab = p.bias_kind == kBiasTable ? 2 * p.radius + 1 + 2 * kTabPad : 0;
+  const int n_tab = BIAS == kBiasTable ? 2 * p.radius + 1 + 2 * kTabPad : 0;
   if (f.rows) {
     const unsigned grid = (unsigned)(p.B * p.Hkv) * (unsigned)p.tiles * (unsigned)p.splits;
-    score_attn_rows_kernel<D, BF, CAP><<<dim3(grid), dim3(64 * kRowWaves), (size_t)(p.table_in_lds ? p.group * n_tab : 0) * 4, st>>>(p);
+    score_attn_rows_kernel<D, BF, CAP, BIAS><<<dim3(grid), dim3(64 * kRowWaves), (size_t)(p.table_in_lds ? p.group * n_tab : 0) * 4, st>>>(p);
   } else {
     p.chunk = (p.B * p.Hq * p.tiles + 7) / 8;
-    score_attn_wide_kernel<D, BF, CAP><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
+    score_attn_wide_kernel<D, BF, CAP, BIAS><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
   }
+}
+template <int D, bool BF, bool CAP>
+static void launch_bias(ScoreParams& p, const Form& f, hipStream_t st) {
+  if (p.table) launch_form<D, BF, CAP, kBiasTable>(p, f, st);
+  else if (p.slopes) launch_form<D, BF, CAP, kBiasSlopes>(p, f, st);
+  else launch_form<D, BF, CAP, kBiasNone>(p, f, st);
 }
 template <int D, bool BF>
 static void launch_fwd(ScoreParams& p, const Form& f, hipStream_t st) {
-  p.k1 != 0.f ? launch_form<D, BF, true>(p, f, st) : launch_form<D, BF, false>(p, f, st);
+  p.k1 != 0.f ? launch_bias<D, BF, true>(p, f, st) : launch_bias<D, BF, false>(p, f, st);
   if (p.splits > 1) {
     const int64_t n = (int64_t)p.B * p.Hkv * p.Sq * p.group;
     score_attn_join_kernel<D, BF><<<dim3((unsigned)n), dim3(256), 0, st>>>(p);

@@ -106,8 +106,8 @@ def _refuse(q, k, v, mask, scale, cap, bias, slopes):
         raise StofError(f"the number of query heads ({Hq}) must be a multiple of the number of key heads ({Hkv})")
     if D not in (64, 128):
         raise StofError(f"head size must be 64 or 128, got {D}")
-    if not 0.0 < scale <= 1e6:
-        raise StofError(f"scale must be positive and at most 1e6, got {scale}")
+    if not 1e-6 <= scale <= 1e6:
+        raise StofError(f"scale must be between 1e-6 and 1e6, got {scale}")
     if cap != 0.0 and not 1e-3 <= cap <= MAX_CAP:
         raise StofError(f"cap must be between 1e-3 and {MAX_CAP}, got {cap}")
     if bias is not None and slopes is not None:
@@ -138,7 +138,7 @@ class _Rule:
         qt, kt, vt = q.stride(), k.stride(), v.stride()
         ok = (q.is_cuda and dtype in _DTYPES and len(qs) == 4 and len(ks) == 4 and vs == ks and qt[3] == 1 and kt[3] == 1 and vt[3] == 1
               and k.dtype == dtype and v.dtype == dtype and k.device == dev and v.device == dev and ks[0] == qs[0] and ks[3] == qs[3]
-              and ks[1] > 0 and qs[1] % ks[1] == 0 and (qs[3] == 64 or qs[3] == 128) and 0.0 < scale <= 1e6
+              and ks[1] > 0 and qs[1] % ks[1] == 0 and (qs[3] == 64 or qs[3] == 128) and 1e-6 <= scale <= 1e6
               and (cap == 0.0 or 1e-3 <= cap <= MAX_CAP))
         radius = -1
         if ok and bias is not None:
