@@ -4,11 +4,15 @@
 // Query i of a sample stands at position p_i = first + i, query head h reads key head
 // h / (Hq / Hkv).  With c = scale * log2(e) the kernels work on scores in units of log2:
 //     t_ij = c q_i.k_j                                        without a cap
-//     t_ij = cap' (1 - 2 / (1 + exp2(2 c q_i.k_j / cap')))     cap' = cap * log2(e): cap tanh(scale q.k / cap)
+//     t_ij = cap' + 2 cap' u_ij, u_ij = -1 / (1 + exp2(2 c q_i.k_j / cap'))    cap' = cap * log2(e): cap tanh(scale q.k / cap)
 //     t_ij += table[h][clip(j - p_i, -R, R) + R] * log2(e)     or   t_ij -= slope_h * log2(e) * |p_i - j|
 // over the allowed keys j < limit_i (and of the query's document), where limit_i = kv_len, or
 // min(kv_len, max(p_i + 1, prefix)) for a causal rule: every mask but the documents is one
 // per-row limit.  A row without allowed keys yields zeros, lse = -inf and no gradients.
+//
+// A capped score is kept as u: its constant cap' changes no probability and its factor 2 cap' goes into the
+// multiply-add before the exponential, where the factor c of an uncapped score goes.  So `raw` below is q.k or u, p.c
+// what turns it into log2 units, and cap' is only added to lse.
 #pragma once
 #include "stof_common.h"
 
@@ -51,8 +55,8 @@ struct ScoreParams {
   int radius, causal;
   int q_start, q_end;                      // p_0 = q_start, or kv_len - Sq with q_end
   int tiles, chunk, cus_per_xcd;           // workgroups per (batch, head); workgroups per XCD; compute units of an XCD
-  float c, k1, capl;                       // scale log2e; 2 scale log2e / cap (0: no cap); cap log2e
-  float cc, slope_mul;                     // what turns a rule's result into log2 units: c when it is in units of the raw product, else 1; slopes to the rule's units
+  float c, k1, lse_add;                    // raw scores to log2 units: scale log2e, or 2 cap log2e; 2 scale log2e / cap (0: no cap); cap log2e or 0
+  float cc, slope_mul;                     // what turns a rule's result into log2 units: c when it is in raw units, else 1 (tables); slopes to raw units
   // form for few rows
   int splits, group, table_in_lds; float* part;
 };
@@ -221,28 +225,27 @@ __device__ __forceinline__ void load_table(const ScoreParams& p, int head, float
 // What one lane knows of its query.
 struct LaneRow { int pos, limit, doc; float slope; const float* tab; const half_t* gtab; };
 
-// The rule on 16 scores of the lane's query: s[r] belongs to key jb + 4 g + 8 (r / 4) + r % 4.  Raw products
-// in, what p.cc turns into log2 units out.
+// The rule on 16 scores of the lane's query: s[r] belongs to key jb + 4 g + 8 (r / 4) + r % 4.  Raw
+// scores in, what p.cc turns into log2 units out.
 __device__ __forceinline__ int key_off(int r) { return 8 * (r >> 2) + (r & 3); }
 
+__device__ __forceinline__ float capped(const ScoreParams& p, float raw) {
+  return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(raw * p.k1));
+}
 __device__ __forceinline__ void cap_scores(const ScoreParams& p, floatx16& s) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const float u = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * p.k1));
-    s[r] = __builtin_fmaf(u, -2.f * p.capl, p.capl);
-  }
+  for (int r = 0; r < 16; ++r) s[r] = capped(p, s[r]);
 }
 // The kind of bias is a template argument: behind run-time branches every kind's result is copied to common registers (D
-// = 64 without a bias: 32 moves for 190 other vector instructions a tile).  Slopes stay in units of the raw product
+// = 64 without a bias: 32 moves for 190 other vector instructions a tile).  Slopes stay in raw units
 // (L.slope has p.slope_mul in it), so that a score costs an addition and a multiply-add.
-template <bool CAP, int BIAS>
+template <int BIAS>
 __device__ __forceinline__ void bias_scores(const ScoreParams& p, const LaneRow& L, int j0 /* jb + 4 g */, floatx16& s) {
   if constexpr (BIAS == kBiasTable) {
-    const float mul = CAP ? 1.f : p.c;
     const int x = min(max(j0 - L.pos, -p.radius - kTabPad), p.radius);
     const float* t = L.tab + (x + p.radius + kTabPad);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mul, t[key_off(r)]);
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.c, t[key_off(r)]);
   } else if constexpr (BIAS == kBiasSlopes) {
     const float x = (float)(j0 - L.pos);
 #pragma unroll

@@ -27,7 +27,7 @@ struct BwdParams {
   const half_t* dout; const half_t* o; const float* lse;
   int64_t dos[3], oos[3];
   half_t* dq; half_t* dk; half_t* dv;        // contiguous [B, Hq, Sq, D], [B, Hkv, Sk, D]
-  floatx2_t* stats;                          // [B, Hq, 64 ceil(Sq / 64)]: (lse in log2 units, delta); +inf = a row without keys or past the end
+  floatx2_t* stats;                          // [B, Hq, 64 ceil(Sq / 64)]: (lse in log2 units less lse_add, delta); +inf = a row without keys or past the end
   float* vmax; float* domax;                 // fp16: largest |V| per (b, hk, key block), largest |dO| per (b, h, query block)
   float* tab_part; half_t* dtable;           // per workgroup of the query kernel: sums of the 2 R + 1 distances
   float scale;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void score_attn_bwd_prep_kernel(const BwdParam
 #pragma unroll
       for (int o = 1; o < kC; o <<= 1) d += __shfl_xor(d, o, 64);
       mx = fmaxf(mx, m);
-      if (c == 0) p.stats[(int64_t)bh * (64 * nq) + r] = floatx2_t{l == -INFINITY ? INFINITY : l * kLog2e, d};
+      if (c == 0) p.stats[(int64_t)bh * (64 * nq) + r] = floatx2_t{l == -INFINITY ? INFINITY : __builtin_fmaf(l, kLog2e, -s.lse_add), d};
     }
   } else {
     const int idx = blockIdx.x - s.B * s.Hq * nq, bh = idx / nk, t = idx - bh * nk;
@@ -120,9 +120,8 @@ __device__ __forceinline__ float wave_max_of(const float* a, int n) {
 __device__ __forceinline__ void cap_scores_grad(const ScoreParams& p, floatx16& s, floatx16& w) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const float u = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * p.k1));
-    w[r] = 4.f * __builtin_fmaf(-u, u, u);
-    s[r] = __builtin_fmaf(u, -2.f * p.capl, p.capl);
+    s[r] = capped(p, s[r]);
+    w[r] = -4.f * __builtin_fmaf(s[r], s[r], s[r]);
   }
 }
 
@@ -352,7 +351,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
     auto rule = [&](int mt) {
       const int j0 = cur.t * kBlock + 32 * mt + 4 * g;
       if constexpr (CAP) cap_scores_grad(p, s[mt], w[mt]);
-      bias_scores<CAP, BIAS>(p, L, j0, s[mt]);
+      bias_scores<BIAS>(p, L, j0, s[mt]);
       if (!cur.full) {
         limit_scores(L, j0, s[mt]);
         if (docs) doc_scores(L, &doc_ids[wave][32 * mt + 4 * g], s[mt]);
@@ -673,9 +672,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
       if constexpr (TAB) {
         const int at = min(max(j - pos0, -p.radius), p.radius + kTabPad);   // distance j - p falls with the row
         const float* t = tab + (at + p.radius + kTabPad);
-        const float mul = CAP ? 1.f : p.c;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], mul, t[-key_off(r)]);
+        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], p.c, t[-key_off(r)]);
       } else if constexpr (BIAS == kBiasSlopes) {
         const float at = (float)(j - pos0);
 #pragma unroll

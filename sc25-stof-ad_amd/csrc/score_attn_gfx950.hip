@@ -272,8 +272,8 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
     }
     const int j0 = cur.t * kBlock + 4 * g;
     if constexpr (CAP) { cap_scores(p, s[0]); cap_scores(p, s[1]); }
-    bias_scores<CAP, BIAS>(p, L, j0, s[0]);
-    bias_scores<CAP, BIAS>(p, L, j0 + 32, s[1]);
+    bias_scores<BIAS>(p, L, j0, s[0]);
+    bias_scores<BIAS>(p, L, j0 + 32, s[1]);
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
       limit_scores(L, j0 + 32, s[1]);
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
   if (rows <= 0) return;
   const float l = pair_sum(sm.l);
   const float inv = l == 0.f ? 0.f : 1.f / l;              // no allowed key at all: zeros
-  if (p.lse && g == 0 && i < p.Sq) p.lse[(int64_t)bh * p.Sq + i] = l == 0.f ? -INFINITY : (sm.m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (p.lse && g == 0 && i < p.Sq) p.lse[(int64_t)bh * p.Sq + i] = l == 0.f ? -INFINITY : (sm.m + __builtin_amdgcn_logf(l) + p.lse_add) * kLn2;
   lds_byte* stage = (lds_byte*)(wave == 0 ? k0 : wave == 1 ? k1 : wave == 2 ? v0 : v1);
   stage_rows<D, BF>(sm.o, inv, stage, j32, g);
   half_t* ob = p.out + b * p.os[0] + h * p.os[1] + (int64_t)row0 * p.os[2];
@@ -465,10 +465,10 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int x = min(max(j0 + key_off(r) - L.pos, -p.radius), p.radius) + p.radius;
-        s[0][r] = __builtin_fmaf(s[0][r], CAP ? 1.f : p.c, table_entry<BF>(L.gtab[x]));
+        s[0][r] = __builtin_fmaf(s[0][r], p.c, table_entry<BF>(L.gtab[x]));
       }
     } else {
-      bias_scores<CAP, BIAS>(p, L, j0, s[0]);
+      bias_scores<BIAS>(p, L, j0, s[0]);
     }
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
     for (int e = 0; e < 4; ++e) o4[e] = to_elem<BF>(part[x + e] * inv);
     *reinterpret_cast<half4_t*>(orow + col) = o4;
   }
-  if (p.lse && wave == 0 && g == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (p.lse && wave == 0 && g == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l) + p.lse_add) * kLn2;
 }
 
 // Joins the splits of the row form: one workgroup per row, every fourth split to a wave, D / 64 columns per lane; the
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams 
     const int c = kC * lane + x;
     orow[c] = to_elem<BF>(((sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c])) * inv);
   }
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l) + p.lse_add) * kLn2;
 }
 
 }  // namespace
@@ -679,13 +679,13 @@ void score_attn_params(ScoreParams& p, const void* q, const void* k, const void*
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.group = Hq / Hkv;
   p.radius = radius < 0 ? 0 : radius;
   p.causal = causal != 0; p.q_start = q_start; p.q_end = q_end != 0;
-  p.c = scale * kLog2e;
+  p.c = cap > 0.f ? 2.f * cap * kLog2e : scale * kLog2e;
   p.k1 = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
-  p.capl = cap * kLog2e;
+  p.lse_add = cap * kLog2e;
   int cus = stof_device_compute_units();
   p.cus_per_xcd = cus >= 8 ? cus / 8 : 32;
-  p.cc = (cap > 0.f || table) ? 1.f : p.c;
-  p.slope_mul = cap > 0.f ? kLog2e : 1.f / scale;
+  p.cc = table ? 1.f : p.c;
+  p.slope_mul = kLog2e / p.c;
 }
 
 void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st) {
