@@ -431,7 +431,7 @@ int stof_gemm_bias_res_ln_cluster_dt(const void* A, const void* Wt, const void* 
  * (NaN included).  scale in [1e-6, 1e6], cap 0 or in [1e-3, 1024].
  * Strides: (batch, head, row) in elements, multiples of 8, rows at most 2^23; pointers 16-byte aligned.
  * lse [B, Hq, Sq] fp32 may be NULL.  form: -1 the library's choice, 0 128-query tiles, 1 32-row tiles with
- * the keys split over waves and workgroups.  The workspace (bytes below, 0 = none) needs no initial
+ * the keys split over waves and workgroups, 2 128-query tiles with the keys in two parts.  The workspace (bytes below, 0 = none) needs no initial
  * contents and belongs to this call until its work is done.
  */
 #define STOF_SCORE_MAX_RADIUS 1024

@@ -9,7 +9,8 @@
 //  * wide form: four waves x 32 queries of one head share K and V tiles of 64 keys, direct-to-LDS
 //    loads double buffered, one barrier per tile.  Which tiles a workgroup visits and which of them
 //    need the element test is decided for 64 tiles at a time, one tile per lane: limits and document
-//    ranges become three 64-bit sets that the walk takes bit by bit.
+//    ranges become three 64-bit sets that the walk takes bit by bit.  On small grids two such sets of four waves
+//    walk every other tile each (parts) and join their rows through LDS.
 //  * row form, for few rows and long keys (single tokens) and for small grids: one workgroup owns 32
 //    rows, row r = (query r / G, head r % G of the G heads that share a key head), so a token's heads
 //    read the cache once; its eight waves take every eighth tile of 32 keys through a buffer of their own
@@ -127,21 +128,21 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
 
 // CAP is a template argument: with the cap behind a run-time branch the compiler computes it speculatively for every
 // tile (64 transcendental operations a lane and tile beside the 32 of the softmax).
-template <int D, bool BF, bool CAP, int BIAS>
-__global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScoreParams p) {
+template <int D, bool BF, bool CAP, int BIAS, int KG>
+__global__ __launch_bounds__(256 * KG, 2) void score_attn_wide_kernel(const ScoreParams p) {
   typedef TileLoad<D, kBlock, 4> TL;
-  __shared__ __attribute__((aligned(1024))) unsigned char k0[TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) unsigned char k1[TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) unsigned char v0[TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) unsigned char v1[TL::kBytes];
-  __shared__ int doc_ids[4][kBlock];            // per wave: the documents of the current tile's keys
+  __shared__ __attribute__((aligned(1024))) unsigned char k0[KG * TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char k1[KG * TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char v0[KG * TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) unsigned char v1[KG * TL::kBytes];
+  __shared__ int doc_ids[4 * KG][kBlock];       // per wave: the documents of the current tile's keys
   extern __shared__ float tab[];                // distance table (kBiasTable)
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all_waves & 3, part = all_waves >> 2;   // (part < KG)
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
 
   Placed at;
-  if (!place(blockIdx.x, p.B * p.Hq, p.group, p.tiles, p.chunk, p.cus_per_xcd, D == 64 ? 3 : 2, p.causal, at)) return;
+  if (!place(blockIdx.x, p.B * p.Hq, p.group, p.tiles, p.chunk, p.cus_per_xcd, KG == 2 ? 1 : D == 64 ? 3 : 2, p.causal, at)) return;
   const int bh = at.head, tile = p.tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
 
@@ -209,17 +210,27 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
     }
     set_load = __ballot(load); set_mine = __ballot(own); set_full = __ballot(full);
   };
-  struct Step { int t; int mine; int full; };
+  struct Step { int more; int t; int mine; int full; };       // more: some part has a tile
   int win = 0;
   if (n_win > 0) window(0);
-  auto next_step = [&]() -> Step {
+  auto next_tile = [&]() -> Step {
     while (set_load == 0) {
-      if (++win >= n_win) return Step{-1, 0, 0};
+      if (++win >= n_win) return Step{0, -1, 0, 0};
       window(win);
     }
     const int bit = __builtin_ctzll(set_load);
     set_load &= set_load - 1;
-    return Step{64 * win + bit, (int)((set_mine >> bit) & 1), (int)((set_full >> bit) & 1)};
+    return Step{1, 64 * win + bit, (int)((set_mine >> bit) & 1), (int)((set_full >> bit) & 1)};
+  };
+  auto next_step = [&]() -> Step {
+    Step s = next_tile();
+    if constexpr (KG == 2) {
+      if (s.more) {
+        const Step second = next_tile();
+        if (part) { s = second; s.more = 1; }
+      }
+    }
+    return s;
   };
 
   Softmax<D, 2, BF> sm;
@@ -278,10 +289,10 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
       limit_scores(L, j0, s[0]);
       limit_scores(L, j0 + 32, s[1]);
       if (docs) {
-        doc_ids[wave][lane] = cur_id;
+        doc_ids[all_waves][lane] = cur_id;
         __builtin_amdgcn_wave_barrier();
-        doc_scores(L, &doc_ids[wave][4 * g], s[0]);
-        doc_scores(L, &doc_ids[wave][32 + 4 * g], s[1]);
+        doc_scores(L, &doc_ids[all_waves][4 * g], s[0]);
+        doc_scores(L, &doc_ids[all_waves][32 + 4 * g], s[1]);
       }
     }
     half8_t pf[2][2];
@@ -295,26 +306,56 @@ __global__ __launch_bounds__(256, 2) void score_attn_wide_kernel(const ScorePara
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  lds_byte* const ka = (lds_byte*)k0 + part * TL::kBytes;
+  lds_byte* const kb = (lds_byte*)k1 + part * TL::kBytes;
+  lds_byte* const va = (lds_byte*)v0 + part * TL::kBytes;
+  lds_byte* const vb = (lds_byte*)v1 + part * TL::kBytes;
   Step cur = next_step();
-  if (cur.t >= 0) issue(cur.t, (lds_byte*)k0, (lds_byte*)v0);
+  if (cur.t >= 0) issue(cur.t, ka, va);
   // (behind the first tile's loads, whose latency it shares; the walk's first barrier covers it)
-  if constexpr (BIAS == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256);
-  while (cur.t >= 0) {
+  if constexpr (BIAS == kBiasTable) load_table<BF>(p, h, tab, threadIdx.x, 256 * KG);
+  while (cur.more) {
     Step nxt = next_step();
-    step(cur, nxt, (lds_byte*)k0, (lds_byte*)v0, (lds_byte*)k1, (lds_byte*)v1);
+    step(cur, nxt, ka, va, kb, vb);
     cur = nxt;
-    if (nxt.t >= 0) {
+    if (nxt.more) {
       cur = next_step();
-      step(nxt, cur, (lds_byte*)k1, (lds_byte*)v1, (lds_byte*)k0, (lds_byte*)v0);
+      step(nxt, cur, kb, vb, ka, va);
     }
   }
 
   __syncthreads();             // every wave has left the walk: the tile buffers become output stages
+  lds_byte* stage = (lds_byte*)(wave == 0 ? k0 : wave == 1 ? k1 : wave == 2 ? v0 : v1);
+  if constexpr (KG == 2) {
+    // the second part's rows to the first: O through the second part's tile buffers, maxima and sums where the documents were
+    float* od = reinterpret_cast<float*>((unsigned char*)(wave == 0 ? k0 : wave == 1 ? k1 : wave == 2 ? v0 : v1) + TL::kBytes);
+    if (part) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) od[(16 * dt + r) * 64 + lane] = sm.o[dt][r];
+      doc_ids[wave][lane] = __builtin_bit_cast(int, sm.m);
+      doc_ids[4 + wave][lane] = __builtin_bit_cast(int, sm.l);
+    }
+    __syncthreads();
+    if (part) return;
+    const float m1 = __builtin_bit_cast(float, doc_ids[wave][lane]), l1 = __builtin_bit_cast(float, doc_ids[4 + wave][lane]);
+    const float m = fmaxf(sm.m, m1);
+    // a part that saw no key has the maximum -inf; one that saw only NaN too, and a sum of NaN, which must stay (a lane's sum
+    // is that of its own keys: 0 where those are masked, whatever the row's maximum)
+    const float e0 = __builtin_amdgcn_exp2f(sm.m - m), e1 = __builtin_amdgcn_exp2f(m1 - m);
+    const float f0 = sm.m == -INFINITY ? 0.f : e0, f1 = m1 == -INFINITY ? 0.f : e1;
+    sm.l = (sm.l == 0.f ? 0.f : sm.l * e0) + (l1 == 0.f ? 0.f : l1 * e1);
+    sm.m = m;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sm.o[dt][r] = sm.o[dt][r] * f0 + od[(16 * dt + r) * 64 + lane] * f1;
+  }
   if (rows <= 0) return;
   const float l = pair_sum(sm.l);
   const float inv = l == 0.f ? 0.f : 1.f / l;              // no allowed key at all: zeros
   if (p.lse && g == 0 && i < p.Sq) p.lse[(int64_t)bh * p.Sq + i] = l == 0.f ? -INFINITY : (sm.m + __builtin_amdgcn_logf(l) + p.lse_add) * kLn2;
-  lds_byte* stage = (lds_byte*)(wave == 0 ? k0 : wave == 1 ? k1 : wave == 2 ? v0 : v1);
   stage_rows<D, BF>(sm.o, inv, stage, j32, g);
   half_t* ob = p.out + b * p.os[0] + h * p.os[1] + (int64_t)row0 * p.os[2];
   const __amdgpu_buffer_rsrc_t o_rsrc = stof_wave_rsrc(ob);
@@ -609,36 +650,40 @@ __global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams 
 
 // ---- host side
 
-// Form and number of key splits.  The row form takes calls whose rows fit one 32-row tile per key head (single tokens: a
-// token's heads read the cache once), and grids that leave most of the device to a few workgroups of the wide form,
-// each of which then walks all keys alone (us, wide | rows): B1 H8 S1024 D64 (64 workgroups) 16.8 | 8.6, B2 H12
-// S512 (96) 10.5 | 12.3, B1 H8 S2048 (128) 31.1 | 23.0, B2 H8 S1024 D128 (128) 23.3 | 25.6, B3 H8 S1000 (192) 18.0 |
-// 23.3, B8 H32 4 queries over 1024 keys 16.7 | 14.0.  With less than a workgroup per compute unit the keys are
-// split further until four per unit have work (of two tiles for each wave at least), which also evens out
-// caches of different length: B16 H32/8 up to 16384 keys D128, two splits 146 us, eight 128.
+// Form, parts and number of key splits (us at 16 bits, D64 unless said otherwise).
+//  * The row form takes calls whose rows fit one 32-row tile per key head (single tokens: a token's heads read the cache
+//    once) and grids whose row tiles are all on the device at once, where a workgroup of the wide form would walk
+//    all keys alone.  Wide form in two parts | row form: B1 H12 S512 9.9 | 8.7, B1 H8 S1024 14.9 | 9.3, D128 19.8 | 16.0;
+//    with more row tiles than units B1 H20 queries 512 keys 1024 15.0 | 16.0, B2 H12 S512 10.3 | 11.3, D128 13.3 | 19.4.
+//  * The wide form walks the keys in two parts while every workgroup can have a compute unit to itself: 256
+//    workgroups, B2 H8 S2048, one part | two: 31.8 | 28.3, causal 29.9 | 25.2, D128 causal 42.1 | 35.0; 384, B8 H12 S512
+//    13.9 | 17.9, B3 H8 S2048 44.7 | 50.2.
+//  * Splitting costs a launch (3 us) and the partial results.  Past 2048 keys the row form's splits give every unit a workgroup:
+//    64 workgroups over 4096 keys 20.6 unsplit, 13.8 with four splits, 18.8 with six, over 16384 keys 64.8 | 25.2 | 35.3;
+//    but 2048 keys 12.1 | 13.6 | 16.3.  Single tokens of many heads are bound by memory and gain from splits only what
+//    evens out caches of different length: 128 workgroups, equal | uneven lengths, D128 over 16384 keys 203 | 179 unsplit, 186 | 129
+//    with four splits, 190 | 130 with eight, over 4096 keys 41 | 32 unsplit, 47 | 34 with four.
 namespace {
 
-struct Form { bool rows; int tiles, splits; };
+struct Form { bool rows; int parts, tiles, splits; };
 
 // whether the tables of the heads that share a key head fit into LDS (beside 133 KB of tiles)
 inline bool tables_fit(int group, int radius) { return group * (2 * radius + 1 + 2 * kTabPad) * 4 <= 26 * 1024; }
 
 inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int form) {
   const int group = Hq / Hkv, cus = 256;
-  const int64_t wide = (int64_t)B * Hq * ((Sq + 127) / 128);
-  const int64_t rows = (int64_t)Sq * group;
-  bool use_rows = form == 1 || (form < 0 && (rows <= 32 || wide < 96 || (wide <= 128 && Sk >= 2048)));
-  if (!use_rows) return Form{false, (Sq + 127) / 128, 1};
-  const int tiles = (int)((rows + 31) / 32);
-  const int64_t wgs = (int64_t)B * Hkv * tiles;
-  const int64_t want = 4 * cus;
-  const int key_tiles = (Sk + kRowKeys - 1) / kRowKeys;
-  int64_t splits = wgs >= cus ? 1 : (want + wgs - 1) / wgs;
-  const int most = (key_tiles + 2 * kRowWaves - 1) / (2 * kRowWaves);      // two tiles per wave
+  const int64_t rows = (int64_t)Sq * group, tiles = (rows + 31) / 32, wgs = (int64_t)B * Hkv * tiles;
+  const bool use_rows = form == 1 || (form < 0 && (tiles == 1 || wgs <= cus));
+  if (!use_rows) {
+    const int wide_tiles = (Sq + 127) / 128;
+    return Form{false, form == 2 || (form < 0 && (int64_t)B * Hq * wide_tiles <= cus) ? 2 : 1, wide_tiles, 1};
+  }
+  int64_t splits = Sk > 2048 && wgs < cus ? cus / wgs : 1;
+  if (tiles == 1 && wgs > 64 && wgs < cus) splits = Sk >= 8192 ? 4 : 1;
+  const int64_t most = ((Sk + kRowKeys - 1) / kRowKeys + 2 * kRowWaves - 1) / (2 * kRowWaves);   // two tiles per wave
   if (splits > most) splits = most;
   if (splits > 64) splits = 64;                                            // one lane each in the join
-  if (splits < 1) splits = 1;
-  return Form{true, tiles, (int)splits};
+  return Form{true, 1, (int)tiles, (int)splits};
 }
 
 inline int64_t ranges_bytes(int B, int Sq, int Sk) {
@@ -704,7 +749,9 @@ static void launch_form(ScoreParams& p, const Form& f, hipStream_t st) {
     score_attn_rows_kernel<D, BF, CAP, BIAS><<<dim3(grid), dim3(64 * kRowWaves), (size_t)(p.table_in_lds ? p.group * n_tab : 0) * 4, st>>>(p);
   } else {
     p.chunk = (p.B * p.Hq * p.tiles + 7) / 8;
-    score_attn_wide_kernel<D, BF, CAP, BIAS><<<dim3(8u * (unsigned)p.chunk), dim3(256), (size_t)n_tab * 4, st>>>(p);
+    const dim3 grid(8u * (unsigned)p.chunk);
+    if (f.parts == 2) score_attn_wide_kernel<D, BF, CAP, BIAS, 2><<<grid, dim3(512), (size_t)n_tab * 4, st>>>(p);
+    else score_attn_wide_kernel<D, BF, CAP, BIAS, 1><<<grid, dim3(256), (size_t)n_tab * 4, st>>>(p);
   }
 }
 template <int D, bool BF, bool CAP>
@@ -746,7 +793,7 @@ extern "C" int stof_score_attn_fwd(const void* q, const void* k, const void* v, 
   if ((docs_q == nullptr) != (docs_k == nullptr)) return STOF_ERR_NULL_POINTER;
   if (q_end && !kv_len) return STOF_ERR_NULL_POINTER;
   if (q_start > (1 << 29) || q_start < -(1 << 29)) return STOF_ERR_BAD_SHAPE;
-  if (form < -1 || form > 1) return STOF_ERR_UNSUPPORTED;
+  if (form < -1 || form > 2) return STOF_ERR_UNSUPPORTED;
   const Form f = pick_form(B, Hq, Hkv, Sq, Sk, form);
   const int64_t need = stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, docs_q != nullptr, form);
   if (need > 0) {

@@ -30,7 +30,7 @@ __all__ = ["ScoreMask", "score_attn", "score_attn_backward", "MAX_RADIUS", "MAX_
 
 MAX_RADIUS = 1024
 MAX_CAP = 1024.0        # the cap is formed to 2^-22 of its size: a larger one would take more from the scores than 16-bit outputs show
-_FORMS = {None: -1, "auto": -1, "wide": 0, "rows": 1}
+_FORMS = {None: -1, "auto": -1, "wide": 0, "rows": 1, "wide2": 2}
 
 
 class ScoreMask:
@@ -165,7 +165,7 @@ class _Rule:
 
 def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
     if launch_form not in _FORMS:
-        raise StofError(f"launch form must be one of None, 'auto', 'wide', 'rows', got {launch_form!r}")
+        raise StofError(f"launch form must be one of None, 'auto', 'wide', 'wide2', 'rows', got {launch_form!r}")
     form = _FORMS[launch_form]
     B, Hq, Hkv, Sq, Sk, D = sizes = r.sizes
     dev, mask = r.dev, r.mask
@@ -299,8 +299,9 @@ def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None,
     ``bias``: learned distance table ``[Hq, 2R+1]`` of q's dtype, R up to 1024; ``slopes``: fp32 ``[Hq]``, constants.
     ``out`` must not overlap the inputs.  Returns ``[B,Hq,Sq,D]`` (``out_layout="bhsd"``) or ``[B,Sq,Hq*D]`` (``"bshd"``), with ``return_lse`` also the
     logarithm of the softmax's denominator, fp32 ``[B,Hq,Sq]``.  Differentiable in q, k, v and bias (through the
-    output, not through lse).  ``launch_form``: None, "wide" (128-query tiles) or "rows" (32-row tiles with the
-    keys split; single tokens and small grids) - the rule by sizes is in the library."""
+    output, not through lse).  ``launch_form``: None, "wide" (128-query tiles), "wide2" (those with the keys
+    in two parts; small grids) or "rows" (32-row tiles with the keys split; single tokens and smaller grids) - the rule by
+    sizes is in the library."""
     r = _Rule(q, k, v, _NO_MASK if mask is None else mask, scale, cap, bias, slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         if out is not None:

@@ -42,7 +42,7 @@ def _mask(rule):
     return ScoreMask(**{k: c(v) for k, v in rule.items()})
 
 
-def _run(q, k, v, dout, rule, forms=("wide", "rows"), train=True, **kw):
+def _run(q, k, v, dout, rule, forms=("wide", "wide2", "rows"), train=True, **kw):
     """Every form of the forward pass, and the gradients through autograd, against the oracle."""
     want = os_.score_attn(q, k, v, dout=dout if train else None, **{**kw, **rule})
     cu = {n: (t.cuda() if torch.is_tensor(t) else t) for n, t in kw.items()}
@@ -137,7 +137,7 @@ def test_table_entries_at_the_ends_of_the_format(dtype):
     bias[1, :] = -math.inf           # head 1: nothing
     bias[2, :] = lo                  # head 2: everything, very low
     m = ScoreMask()
-    for f in ("wide", "rows"):
+    for f in ("wide", "wide2", "rows"):
         out, lse = score_attn(q.cuda(), k.cuda(), v.cuda(), m, bias=bias.cuda(), return_lse=True, launch_form=f)
         assert torch.equal(out[0, 0].cpu(), v[0, 0]) and torch.equal(out[0, 1].cpu(), torch.zeros(80, 64, dtype=DT[dtype]))
         assert bool(torch.isinf(lse[0, 1]).all())
@@ -154,7 +154,7 @@ def test_table_entries_at_the_ends_of_the_format(dtype):
     assert not bool(grads[0][0, 1].any()) and not bool(grads[3][1].any())
 
 
-@pytest.mark.parametrize("form", ["wide", "rows"])
+@pytest.mark.parametrize("form", ["wide", "wide2", "rows"])
 @pytest.mark.parametrize("D", [64, 128])
 def test_what_no_query_may_use_is_not_read_as_a_value(form, D):
     """NaN and infinities past kv_len, at positions without a document and in padded query rows."""
@@ -178,7 +178,7 @@ def test_what_no_query_may_use_is_not_read_as_a_value(form, D):
         _check(g, want[n], n)
 
 
-@pytest.mark.parametrize("form", ["wide", "rows"])
+@pytest.mark.parametrize("form", ["wide", "wide2", "rows"])
 def test_the_free_part_of_a_cache_behind_causality(form):
     """No key length given: what causality closes to every query is not read as a value either."""
     q, k, v, dout = _qkv(2, 2, 1, 40, 150, 64, torch.bfloat16, seed=18)
@@ -194,7 +194,7 @@ def test_the_free_part_of_a_cache_behind_causality(form):
         _check(g, want[n], n)
 
 
-@pytest.mark.parametrize("form", ["wide", "rows"])
+@pytest.mark.parametrize("form", ["wide", "wide2", "rows"])
 @pytest.mark.parametrize("D", [64, 128])
 def test_nan_in_an_allowed_place_reaches_its_rows(form, D):
     """A query of NaN, and a NaN key that is the only one of its tile and split: NaN out and NaN lse, never a number."""
@@ -303,7 +303,7 @@ def test_strided_views_layouts_and_rows_behind_the_last():
         for t, n in enumerate(("dq", "dk", "dv")):
             _check(g[..., t * H * D:(t + 1) * H * D].view(B, S, H, D).permute(0, 2, 1, 3), want[n], f"{layout} {n}")
     big = torch.full((B, H, S + 40, D), 7.0, dtype=torch.float16, device="cuda")
-    for f in ("wide", "rows"):
+    for f in ("wide", "wide2", "rows"):
         score_attn(vq.detach(), vk.detach(), vv.detach(), ScoreMask(causal=True), out=big[:, :, 20:20 + S], launch_form=f)
         _check(big[:, :, 20:20 + S], want["out"], f"out= ({f})")
         assert bool((big[:, :, :20] == 7).all()) and bool((big[:, :, 20 + S:] == 7).all())
@@ -312,7 +312,7 @@ def test_strided_views_layouts_and_rows_behind_the_last():
     vals = torch.full((B, 512, H, D), math.nan, dtype=torch.float16, device="cuda").permute(0, 2, 1, 3)
     vals[:, :, :S] = v.cuda()
     m = ScoreMask(causal=True, kv_len=torch.full((B,), S, dtype=torch.int32, device="cuda"), q_start="end")
-    for f in ("wide", "rows"):
+    for f in ("wide", "wide2", "rows"):
         _check(score_attn(q.cuda(), cache, vals, m, launch_form=f), want["out"], f"cache ({f})")
 
 
@@ -330,7 +330,7 @@ def test_single_tokens(B, Hq, Hkv, D, Sk, what):
         kw["bias"] = torch.randn(Hq, 2 * 64 + 1, generator=_gen(1)).to(dtype)
     if what == "slopes":
         kw["slopes"] = torch.rand(Hq, generator=_gen(1)) * 0.05
-    _run(q, k, v, None, dict(kv_len=kv_len, q_start="end"), train=False, forms=(None, "wide", "rows"), **kw)
+    _run(q, k, v, None, dict(kv_len=kv_len, q_start="end"), train=False, forms=(None, "wide", "wide2", "rows"), **kw)
 
 
 def test_a_sequence_token_by_token_equals_the_whole():
@@ -378,7 +378,7 @@ def test_long_cache_past_32_bit_offsets():
     p = torch.softmax((view[0, 0].double() @ q[0, 0, 0].double()) / 8, 0)
     want = p @ view[0, 0].double()
     size = float((p[:, None] * view[0, 0].double().abs()).sum(0).max())
-    for f in ("wide", "rows"):
+    for f in ("wide", "wide2", "rows"):
         out = score_attn(q, view, view, launch_form=f)[0, 0, 0].double()
         # roundings of P and out, fp32 scores of at most 6: (64 + 8) 2^-24 * 6 * 8 twice; small P: 2^-25 each against a sum of S terms
         bound = (2.0 ** -11 + 2 * 72 * 48 * 2.0 ** -24) * size + 2.0 ** -11 * want.abs() + 2.0 ** -25

@@ -58,7 +58,7 @@ def test_forward_argument_checks(lib):
         assert call(**kw) == -2, kw
     for kw in (dict(D=96), dict(dtype=2), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(cap=-1.0), dict(cap=float("inf")),
                dict(cap=1025.0), dict(cap=1e-4), dict(scale=1e7),
-               dict(table=P, radius=1025), dict(table=P, radius=4, slopes=P), dict(form=2)):
+               dict(table=P, radius=1025), dict(table=P, radius=4, slopes=P), dict(form=3)):
         assert call(**kw) == -3, kw
     assert call(dq=P) == -1 and call(end=1) == -1
     assert call(dq=P, dk=P) == -1                                  # documents need a workspace
