@@ -296,79 +296,120 @@ __global__ __launch_bounds__(64 * WM * WN * KG, OCC) void gemm_i8_kernel(const I
   }
 }
 
-// ---- token form: up to 16 tokens, 16 features per workgroup, K split over the four waves.
+// ---- token form: up to 16 tokens, 16 features at a time per workgroup, K split over the four waves.
 // v_mfma_i32_16x16x64_i8: A = 16 weight rows (lane & 15) x 64 of K (16 bytes per lane, group lane >> 4), B = the tokens from
 // LDS.  Result: token lane & 15, features 4 (lane >> 4) + r.  A wave's weights arrive in rounds of kTokLoads loads, the
-// next round requested before the products of the current one.
+// next round (of the next 16 features, too) requested before the products of the current one.
+//
+// Bound: the weights for one token, quantising for many, which every workgroup does for itself: from two tokens on
+// each wave takes whole rows (registers hold them between the search for the maximum and the rounding; the waves
+// sharing every row: 16 x 1024 -> 4096 16.9 us, so 8.6), and a workgroup takes every gridDim-th block of 16 features (16 x 1024
+// -> 16384 23.2 -> 12.5).  Against a quantising launch and the tile form, whose gap of 2 us is not in these figures: 1 x
+// 1024 -> 4096 4.2 | 8.3 us, 1 x 4096 -> 4096 8.8 | 13.0, 16 x 1024 -> 4096 8.6 | 8.9, 8 x 4096 -> 4096 12.3 | 13.8, 1 x 4096 -> 16384
+// 20.3 | 17.9; 16 x 4096 -> 4096 17.5 | 14.2, so rows beyond 64 KB of LDS take two launches.
 constexpr int kTokMax = 16;
 constexpr int kTokLoads = 8;
 constexpr int kTokLds = 64 * 1024;
+constexpr int kTokGrid = 512;
+constexpr int kTokKeep = 8;        // chunks of 512 values of a row in registers
 
 template <int ACT, bool BF>
 __global__ __launch_bounds__(256) void linear_i8_token_kernel(const I8Params p) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char xq_lds[];       // [M][Kp], Kp = K rounded up to 64, zeros beyond K
-  __shared__ unsigned tops[4][kTokMax];
+  extern __shared__ __attribute__((aligned(16))) unsigned char xq_lds[];       // [M][Kp + 16], Kp = K rounded up to 64, zeros beyond K
+  __shared__ unsigned tops[4];
   __shared__ float sxs[kTokMax];
-  __shared__ int sums[4][16][17];
+  __shared__ int sums[2][4][16][17];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int steps = (p.K + 63) / 64, Kp = steps * 64;
-  const int8_t* wrow = p.wq + (int64_t)min(n0 + row, p.N - 1) * p.ldw;
-  // K step s of this wave: 64 (4 s + wave)
-  auto weights = [&](int s) -> int4_t {
-    const int k = 64 * (4 * s + wave) + 16 * kg;
-    return *reinterpret_cast<const int4_t*>(wrow + (k < p.K ? k : 0));          // (times zeros of x beyond K)
-  };
+  const int steps = (p.K + 63) / 64, Kp = steps * 64, pitch = Kp + 16, blocks = (p.N + 15) / 16;
   const int mine = (steps - wave + 3) / 4;
+  auto k_of = [&](int s) { return 64 * (4 * s + wave) + 16 * kg; };          // this wave's step s
+  auto weights = [&](int block, int s) -> int4_t {
+    const int k = k_of(s);
+    return *reinterpret_cast<const int4_t*>(p.wq + (int64_t)min(16 * block + row, p.N - 1) * p.ldw + (k < p.K ? k : 0));   // (times zeros of x beyond K)
+  };
+  int block = blockIdx.x;
   int4_t wa[kTokLoads];
 #pragma unroll
-  for (int i = 0; i < kTokLoads; ++i) wa[i] = i < mine ? weights(i) : int4_t{0, 0, 0, 0};
+  for (int i = 0; i < kTokLoads; ++i) wa[i] = i < mine ? weights(block, i) : int4_t{0, 0, 0, 0};
 
-  // the tokens: one or more passes of 256 threads x 8 values over each row
-  for (int m = 0; m < p.M; ++m) {
+  if (p.M == 1) {          // the waves share the row
     unsigned top = 0;
-    for (int k = 8 * threadIdx.x; k < p.K; k += 2048) top = max_pattern(*reinterpret_cast<const half8_t*>(p.x + m * p.ldx + k), top);
+    for (int k = 8 * threadIdx.x; k < p.K; k += 2048) top = max_pattern(*reinterpret_cast<const half8_t*>(p.x + k), top);
     top = wave_max_u(top);
-    if (lane == 0) tops[wave][m] = top;
-  }
-  __syncthreads();
-  for (int m = 0; m < p.M; ++m) {
-    const RowQuant<BF> q(max(max(tops[0][m], tops[1][m]), max(tops[2][m], tops[3][m])));
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    const RowQuant<BF> q(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
     for (int k = 8 * threadIdx.x; k < Kp; k += 2048)
-      *reinterpret_cast<uint64_t*>(xq_lds + m * Kp + k) = k < p.K ? q.pack(*reinterpret_cast<const half8_t*>(p.x + m * p.ldx + k)) : 0;
-    if (threadIdx.x == 0) sxs[m] = q.scale;
-  }
-  __syncthreads();
-
-  const unsigned char* xrow = xq_lds + min(row, p.M - 1) * Kp;
-  int4_t acc = {0, 0, 0, 0};
-  for (int s0 = 0; s0 < mine; s0 += kTokLoads) {
-    int4_t wn[kTokLoads];
+      *reinterpret_cast<uint64_t*>(xq_lds + k) = k < p.K ? q.pack(*reinterpret_cast<const half8_t*>(p.x + k)) : 0;
+    if (threadIdx.x == 0) sxs[0] = q.scale;
+  } else {
+    for (int m = wave; m < p.M; m += 4) {
+      const half_t* src = p.x + m * p.ldx;
+      half8_t v[kTokKeep];
+      unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < kTokLoads; ++i) wn[i] = s0 + kTokLoads + i < mine ? weights(s0 + kTokLoads + i) : int4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < kTokLoads; ++i)
-      if (s0 + i < mine) {
-        const int4_t xb = *reinterpret_cast<const int4_t*>(xrow + 64 * (4 * (s0 + i) + wave) + 16 * kg);
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wa[i], xb, acc, 0, 0, 0);
+      for (int i = 0; i < kTokKeep; ++i) {
+        const int k = 512 * i + 8 * lane;
+        const half8_t z = {};
+        v[i] = k < p.K ? *reinterpret_cast<const half8_t*>(src + k) : z;
       }
 #pragma unroll
-    for (int i = 0; i < kTokLoads; ++i) wa[i] = wn[i];
-  }
+      for (int i = 0; i < kTokKeep; ++i) top = max_pattern(v[i], top);
+      for (int k = 512 * kTokKeep + 8 * lane; k < p.K; k += 512) top = max_pattern(*reinterpret_cast<const half8_t*>(src + k), top);
+      const RowQuant<BF> q(wave_max_u(top));
 #pragma unroll
-  for (int r = 0; r < 4; ++r) sums[wave][row][4 * kg + r] = acc[r];
+      for (int i = 0; i < kTokKeep; ++i) {
+        const int k = 512 * i + 8 * lane;
+        if (k < Kp) *reinterpret_cast<uint64_t*>(xq_lds + m * pitch + k) = q.pack(v[i]);      // (zeros beyond K)
+      }
+      for (int k = 512 * kTokKeep + 8 * lane; k < Kp; k += 512)
+        *reinterpret_cast<uint64_t*>(xq_lds + m * pitch + k) = k < p.K ? q.pack(*reinterpret_cast<const half8_t*>(src + k)) : 0;
+      if (lane == 0) sxs[m] = q.scale;
+    }
+  }
   __syncthreads();
-  // thread (token t, feature f)
-  const int t = threadIdx.x >> 4, f = threadIdx.x & 15, n = n0 + f;
-  if (t < p.M && n < p.N) {
-    const int total = (sums[0][t][f] + sums[1][t][f]) + (sums[2][t][f] + sums[3][t][f]);
-    const float b = p.bias ? from_elem<BF>(p.bias[n]) : 0.f;
-    p.out[(int64_t)t * p.ldo + n] = to_elem<BF>(act_i8<ACT>(__builtin_fmaf((float)total, sxs[t] * p.sw[n], b)));
+
+  const unsigned char* xrow = xq_lds + min(row, p.M - 1) * pitch;
+  // thread (token t, feature f) of the epilogue
+  const int t = threadIdx.x >> 4, f = threadIdx.x & 15;
+  for (int it = 0; block < blocks; ++it) {
+    const int next = block + gridDim.x;
+    int4_t acc = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < mine; s0 += kTokLoads) {
+      const bool last = s0 + kTokLoads >= mine;
+      int4_t wn[kTokLoads];
+#pragma unroll
+      for (int i = 0; i < kTokLoads; ++i) {
+        const int s = last ? i : s0 + kTokLoads + i;
+        wn[i] = s < mine && (!last || next < blocks) ? weights(last ? next : block, s) : int4_t{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int i = 0; i < kTokLoads; ++i)
+        if (s0 + i < mine) {
+          const int4_t xb = *reinterpret_cast<const int4_t*>(xrow + k_of(s0 + i));
+          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wa[i], xb, acc, 0, 0, 0);
+        }
+#pragma unroll
+      for (int i = 0; i < kTokLoads; ++i) wa[i] = wn[i];
+    }
+    // (two sets of sums in turn: a set is written again only behind the barrier of the block between)
+    int (*part)[16][17] = sums[it & 1];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) part[wave][row][4 * kg + r] = acc[r];
+    __syncthreads();
+    const int n = 16 * block + f;
+    if (t < p.M && n < p.N) {
+      const int total = (part[0][t][f] + part[1][t][f]) + (part[2][t][f] + part[3][t][f]);
+      const float b = p.bias ? from_elem<BF>(p.bias[n]) : 0.f;
+      p.out[(int64_t)t * p.ldo + n] = to_elem<BF>(act_i8<ACT>(__builtin_fmaf((float)total, sxs[t] * p.sw[n], b)));
+    }
+    block = next;
   }
 }
 
-bool token_form(int64_t M, int64_t K) { return M <= kTokMax && M * ((K + 63) / 64 * 64) <= kTokLds; }
+int64_t token_pitch(int64_t K) { return (K + 63) / 64 * 64 + 16; }
+bool token_form(int64_t M, int64_t K) { return M <= kTokMax && M * token_pitch(K) <= kTokLds; }
 int64_t padded(int64_t K) { return (K + 15) / 16 * 16; }
 
 // Which tile form, by the number of tiles and the length of K (us, form taken | its neighbour):
@@ -405,8 +446,8 @@ void launch_gemm(I8Params& p, hipStream_t st) {
 }
 template <int ACT, bool BF>
 void launch_token(I8Params& p, hipStream_t st) {
-  const size_t lds = (size_t)p.M * ((p.K + 63) / 64 * 64);
-  linear_i8_token_kernel<ACT, BF><<<dim3((unsigned)((p.N + 15) / 16)), dim3(256), lds, st>>>(p);
+  const size_t lds = (size_t)p.M * (size_t)token_pitch(p.K);
+  linear_i8_token_kernel<ACT, BF><<<dim3((unsigned)min((p.N + 15) / 16, kTokGrid)), dim3(256), lds, st>>>(p);
 }
 template <bool BF>
 void launch_act(I8Params& p, int act, bool token, hipStream_t st) {

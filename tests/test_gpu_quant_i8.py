@@ -146,7 +146,7 @@ def test_sums_at_the_largest_k():
     assert bool(((y - 2147221504e-9).abs() <= 2.0 ** -8 * 2.15).all())
 
 
-@pytest.mark.parametrize("M,K", [(16, 4096), (1, 65536), (16, 4112), (2, 32768), (2, 32784)])
+@pytest.mark.parametrize("M,K", [(16, 4048), (1, 65520), (16, 4096), (2, 32752), (2, 32768), (3, 4640), (15, 2064), (1, 65536)])
 def test_token_form_at_the_limit_of_its_lds(M, K):
     """64 KB of quantised rows in LDS, and the first sizes beyond, which take the other form."""
     x = torch.randn(M, K, generator=_gen(M)).bfloat16()
@@ -177,6 +177,13 @@ def test_batch_dims_strides_and_guard_rows():
     assert linear_i8(x.cuda()[:0, :, :64], w.cuda(), ws.cuda()).shape == (0, 30, 24)
     odd = torch.randn(4, 65, generator=_gen(7)).half().cuda()[:, 1:]      # rows that cannot be read as they lie: a copy
     _close(linear_i8(odd, w.cuda(), ws.cuda(), b.cuda()), _want(*_quant64(odd.cpu()), w, ws, b, "none", torch.float16))
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 96, 8200), (2, 1040, 8208), (5, 64, 20000), (16, 512, 16392)])
+def test_token_form_with_several_feature_blocks_per_workgroup(M, K, N):
+    x = torch.randn(M, K, generator=_gen(M)).half()
+    w, ws, b = _weights(N, K, torch.float16, 4)
+    _close(linear_i8(x.cuda(), w.cuda(), ws.cuda(), b.cuda(), act="gelu"), _want(*_quant64(x), w, ws, b, "gelu", torch.float16))
 
 
 def test_two_streams_at_once():
