@@ -62,7 +62,7 @@ def _weights(N, K, dtype, seed):
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-@pytest.mark.parametrize("M,K", [(1, 16), (5, 48), (64, 512), (3, 1040), (130, 4096)])
+@pytest.mark.parametrize("M,K", [(1, 16), (5, 48), (64, 512), (3, 1040), (130, 4096), (3, 5008), (9, 8192), (2, 8208), (2, 16384), (3, 16400)])
 def test_quantised_rows_exactly(dtype, M, K):
     x = torch.randn(M, K, generator=_gen(K)).to(DT[dtype])
     x[0, 0] = 100.0
