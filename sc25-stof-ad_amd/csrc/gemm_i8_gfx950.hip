@@ -14,9 +14,10 @@
 // Large products use the tile form of the 16-bit GEMM (C^T = W X^T, both operands K-contiguous through LDS
 // rows of 128 bytes): a row of 128 bytes now holds 128 of K, so the loads, LDS reads and MFMAs of a tile
 // are those of the 16-bit kernel and do twice the arithmetic.  Bound at long K by the LDS reads beside the MFMAs
-// (8192^3: 2.25 POP/s, a library's product 2.08), at K ~ 1024 by what a tile pays beside its products: scales and
-// bias are therefore requested ahead of the operands and wait in LDS for the epilogue (8192 x 1024 -> 4096 60 -> 53 us).  A few tokens use the token form: weights
-// go straight to registers, each exactly once, and every workgroup quantises the tokens itself, so a
+// (8192^3: 486 us, 2.26 POP/s, MFMA busy 66 %; a library's product 2.08), at K ~ 1024 by what a tile pays beside its
+// products: scales and bias are therefore requested ahead of the operands and wait in LDS for the epilogue
+// (8192 x 1024 -> 4096 60 -> 53 us, since 44 with single-buffered tiles, 46 with the GELU).  A few tokens use the token form: weights go
+// straight to registers, each exactly once, and every workgroup quantises the tokens itself, so a
 // single-token projection is one launch.
 #include "gemm_tile.h"
 

@@ -29,7 +29,7 @@ struct BwdParams {
   half_t* dq; half_t* dk; half_t* dv;        // contiguous [B, Hq, Sq, D], [B, Hkv, Sk, D]
   floatx2_t* stats;                          // [B, Hq, 64 ceil(Sq / 64)]: (lse in log2 units less lse_add, delta); +inf = a row without keys or past the end
   float* vmax; float* domax;                 // fp16: largest |V| per (b, hk, key block), largest |dO| per (b, h, query block)
-  float* tab_part; half_t* dtable;           // per workgroup of the query kernel: sums of the 2 R + 1 distances
+  float* tab_part; half_t* dtable;           // per (b, h), key tile and split: sums of the 2 R + 1 distances
   float scale;
   int q_tiles, k_tiles, q_chunk, k_chunk;
   int splits; float* kv_part;                // workgroups that share a key tile; their fp32 sums, [2][splits][B Hkv Sk D]
@@ -184,6 +184,9 @@ __device__ __forceinline__ void store_rows(const floatx16 (&o)[D / 32], float mu
 // delta' = sum_j P_ij dP_ij is formed along the way in fp32, and with M = P (1 - tanh^2) K as one product more
 //     dQ = scale (dT(delta) K - (delta' - delta) M)
 // is exact in delta while the second term stays small.  delta' replaces delta for the kernel of the keys.
+//
+// Bound: MFMA and vector issue, 4 products of 2 D FLOP a pair.  bf16, B2 H16 S2048: D64 75 us (914 TFLOP/s, MFMA busy 51 %), D128
+// 140 us (984 TFLOP/s, 51 %; one workgroup of four waves per unit, whose accumulators take 380 registers).
 template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;
@@ -453,6 +456,9 @@ __global__ __launch_bounds__(1024) void score_attn_bwd_table_kernel(const BwdPar
 // the wave's own array; diagonals that clip, and pieces that lie beyond the radius as a whole, are
 // added in two registers per lane.  After each head the waves' arrays are joined and written to the
 // workspace, which a last kernel adds up over batch and key tiles.
+//
+// Bound: LDS reads beside MFMA and vector issue (both operands of the sums' products are transposed on the way; 1.8 to 2.1 reads
+// per MFMA).  bf16, B2 H16 S2048: D64 93 us (740 TFLOP/s, MFMA busy 43 %), with a table 115; D128 166 us (828 TFLOP/s, 41 %), table 206.
 template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;

@@ -126,6 +126,13 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
     }
 }
 
+// ---- wide form.  Bound: vector issue beside the MFMAs.  A wave's 32 x 64 scores cost 4 D / 16 MFMAs of 32 cycles and, without
+// a rule, 107 vector instructions of 4 cycles and 32 exponentials (+ 64 for slopes, 32 and as many LDS reads for a table, 32
+// and 64 transcendental for a cap), and the two kinds of issue overlap by about a third.  bf16, B2 H16 S2048: D64
+// 50 us (680 TFLOP/s, MFMA busy 36 %), with a table 60, capped and causal 45; D128 73 us (940 TFLOP/s, 51 %), table
+// 80, capped and causal 58.  Tiles of 64 keys keep a 32-row wave within 170 registers at D64 (three workgroups per unit; held to
+// four it spilled: B8 H12 S1024 with a table 41 -> 50 us) and 232 at D128 (two).
+//
 // CAP is a template argument: with the cap behind a run-time branch the compiler computes it speculatively for every
 // tile (64 transcendental operations a lane and tile beside the 32 of the softmax).
 template <int D, bool BF, bool CAP, int BIAS, int KG>
@@ -373,7 +380,8 @@ __global__ __launch_bounds__(256 * KG, 2) void score_attn_wide_kernel(const Scor
 // Bound: the reading of K and V, or for short caches the chain of dependent loads.  Each wave keeps one K and one V
 // tile of 32 keys: the next K tile is requested as soon as the scores of the current one are formed, the next V
 // tile after the second product, so one of the two is always on its way while the wave computes, and
-// eight waves with 128 KB of requests (head size 128) per compute unit cover the memory's latency.
+// eight waves with 128 KB of requests (head size 128) per compute unit cover the memory's latency.  One token of
+// B1 H32/8 over 16384 keys, D128: 14.0 us + 4.6 us for the join (67 MB: 4.8 TB/s); B1 H12 over 512 keys 7 us.
 constexpr int kRowKeys = 32;
 constexpr int kRowWaves = 8;
 
