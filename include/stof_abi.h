@@ -8,7 +8,7 @@
  *   - every pointer is a DEVICE pointer unless stated otherwise; the library never
  *     allocates, frees or retains caller memory;
  *   - all activations are IEEE fp16 (two bytes; the attention entry points also take bfloat16);
- *     accumulation and statistics are fp32;
+ *     accumulation and statistics are fp32 (int32 in the 8-bit products);
  *   - `stream` is a hipStream_t passed as void* (NULL = the null stream); launches
  *     are asynchronous, nothing synchronises;
  *   - every function returns 0 on success or a negative STOF_ERR_* code; no launch
@@ -39,6 +39,9 @@
  *                              and matmul + bias + residual + F.layer_norm, src/benchmk_end2end.py:73-76
  *   stof_gemm_bias_res_ln_cluster  the same interfaces (a second launch form of the operator)
  *   stof_*_dt                  the entry points above with the element format as an argument (fp16 or bfloat16)
+ *   stof_score_attn_*, stof_linear_i8*, stof_quantize_rows_i8, stof_gemm_i8_bias_act
+ *                              additions without a counterpart: attention with score rules (the reference's operators take 0/1
+ *                              masks, src/ops/package_op.py:10-74) and the linear operator in 8-bit integers
  */
 #ifndef STOF_ABI_H
 #define STOF_ABI_H
