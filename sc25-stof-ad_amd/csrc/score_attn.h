@@ -44,6 +44,17 @@ __device__ __forceinline__ bool ranges_one(const DocRange& a, const DocRange& b)
   return a.all && b.all && a.lo == a.hi && b.lo == b.hi && a.lo == b.lo;
 }
 
+// That of block `blk` of a sequence of S documents, by one wave; every lane gets it.
+__device__ __forceinline__ DocRange doc_range(const int* docs, int S, int blk, int lane) {
+  const int i = blk * kBlock + lane;
+  const bool inside = i < S;
+  const int d = inside ? docs[i] : -1;
+  int lo = d >= 0 ? d : 0x7fffffff, hi = d >= 0 ? d : -1;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64)); }
+  return DocRange{lo, hi, !__any(inside && d < 0), 0};
+}
+
 struct ScoreParams {
   const half_t* q; const half_t* k; const half_t* v; half_t* out; float* lse;
   int64_t qs[3], ks[3], vs[3], os[3];      // element strides (batch, head, row)
@@ -222,6 +233,19 @@ __device__ __forceinline__ void load_table(const ScoreParams& p, int head, float
   }
 }
 
+// Distances lo .. hi of a piece of scores that all clip to one end of the table add one number to each: instead of a
+// look-up per score, `add` then goes with the row's constant before the exponential (in log2 units, the scores stay raw).  Ends that
+// would swallow a score when added to it (the lowest values of a format, infinities) or are NaN take the look-ups.
+struct FarPiece { bool far; float add; };
+__device__ __forceinline__ FarPiece far_piece(const ScoreParams& p, const float* tab, int lo, int hi) {
+  FarPiece f = {false, 0.f};
+  if (hi <= -p.radius || lo >= p.radius) {
+    const float end = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, tab[hi <= -p.radius ? 0 : 2 * (p.radius + kTabPad)])));
+    if (__builtin_fabsf(end) < 4096.f) { f.far = true; f.add = end; }
+  }
+  return f;
+}
+
 // What one lane knows of its query.
 struct LaneRow { int pos, limit, doc; float slope; const float* tab; const half_t* gtab; };
 
@@ -263,6 +287,15 @@ __device__ __forceinline__ void doc_scores(const LaneRow& L, const int* ids, flo
   for (int r = 0; r < 16; ++r) s[r] = ids[key_off(r)] == L.doc ? s[r] : -INFINITY;
 }
 
+// Range number n of a call's B (nq + nk): the blocks of the queries of all samples, then those of the keys; by one wave.
+__device__ __forceinline__ void write_doc_range(const ScoreParams& p, int n, int lane) {
+  const int nq = (p.Sq + kBlock - 1) / kBlock, nk = (p.Sk + kBlock - 1) / kBlock;
+  const bool is_q = n < p.B * nq;
+  const int idx = is_q ? n : n - p.B * nq, blocks = is_q ? nq : nk, S = is_q ? p.Sq : p.Sk, b = idx / blocks;
+  const DocRange r = doc_range((is_q ? p.docs_q : p.docs_k) + (int64_t)b * S, S, idx - b * blocks, lane);
+  if (lane == 0) const_cast<DocRange*>(is_q ? p.dr_q : p.dr_k)[idx] = r;
+}
+
 // Document of position i, -1 for none (queries) or -2 (keys), so that they never match.
 __device__ __forceinline__ int doc_or(int d, int none) { return d < 0 ? none : d; }
 __device__ __forceinline__ int doc_at(const int* docs, int64_t i, bool inside, int none) { return doc_or(inside ? docs[i] : none, none); }
@@ -274,5 +307,5 @@ int score_attn_check(const void* const* req, int n_req, const int64_t* const* st
 void score_attn_params(ScoreParams& p, const void* q, const void* k, const void* v, const void* table, const void* slopes, const void* prefix,
                        const void* kv_len, const void* docs_q, const void* docs_k, float scale, float cap, int radius, int causal, int q_start,
                        int q_end, const int64_t* qs, const int64_t* ks, const int64_t* vs, int B, int Hq, int Hkv, int Sq, int Sk);
-void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st);
+int score_attn_ranges_at(ScoreParams& p, void* ws);      // places the document ranges; how many there are
 #pragma GCC visibility pop

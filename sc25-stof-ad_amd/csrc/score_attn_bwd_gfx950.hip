@@ -32,6 +32,7 @@ struct BwdParams {
   float* tab_part; half_t* dtable;           // per (b, h), key tile and split: sums of the 2 R + 1 distances
   float scale;
   int q_tiles, k_tiles, q_chunk, k_chunk;
+  int ranges;                                // document ranges to form (0: none)
   int splits; float* kv_part;                // workgroups that share a key tile; their fp32 sums, [2][splits][B Hkv Sk D]
 };
 
@@ -48,7 +49,8 @@ template <int D> __device__ __forceinline__ int dt_shift(float mdo, float mv) {
 }
 
 // Per row of dO: (lse in log2 units, delta), and for fp16 the largest |dO| and |V| of every 64 rows.
-// Grid: B Hq ceil(Sq / 64) workgroups of query rows, then (fp16) B Hkv ceil(Sk / 64) of value rows.
+// Also the document ranges, one per wave.  Grid: B Hq ceil(Sq / 64) workgroups of query rows, then (fp16) B Hkv ceil(Sk / 64) of value
+// rows, then a quarter of the ranges.
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void score_attn_bwd_prep_kernel(const BwdParams p) {
   const ScoreParams& s = p.s;
@@ -58,6 +60,12 @@ __global__ __launch_bounds__(256) void score_attn_bwd_prep_kernel(const BwdParam
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane % kC;
   const int nq = (s.Sq + 63) / 64, nk = (s.Sk + 63) / 64;
   const bool is_q = (int)blockIdx.x < s.B * s.Hq * nq;
+  const int range0 = s.B * s.Hq * nq + (BF ? 0 : s.B * s.Hkv * nk);
+  if ((int)blockIdx.x >= range0) {
+    const int n = 4 * ((int)blockIdx.x - range0) + wave;
+    if (n < p.ranges) write_doc_range(s, n, lane);
+    return;
+  }
   float mx = 0.f;
   if (is_q) {
     const int bh = blockIdx.x / nq, t = blockIdx.x - bh * nq;
@@ -343,8 +351,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
     };
     floatx16 s[2] = {zero16(), zero16()}, dp[2] = {zero16(), zero16()}, w[2];
     half8_t x[2][2], y[2][2];
+    float cc[2] = {p.cc, p.cc}, add[2] = {0.f, 0.f};
     auto softmax = [&](int mt, int r) {
-      float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], p.cc, shift - lse));
+      float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], cc[mt], shift - lse + add[mt]));
       float d = pr * (dp[mt][r] - delta);
       off += d;
       if constexpr (CAP) { d *= w[mt][r]; pr *= w[mt][r]; }
@@ -354,7 +363,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
     auto rule = [&](int mt) {
       const int j0 = cur.t * kBlock + 32 * mt + 4 * g;
       if constexpr (CAP) cap_scores_grad(p, s[mt], w[mt]);
-      bias_scores<BIAS>(p, L, j0, s[mt]);
+      bool look_up = true;
+      if constexpr (BIAS == kBiasTable) {
+        const int at = cur.t * kBlock + 32 * mt - (first + row0);
+        const FarPiece f = far_piece(p, tab, at - 31, at + 31);
+        if (f.far) { look_up = false; cc[mt] = p.c; add[mt] = f.add; }
+      }
+      if (look_up) bias_scores<BIAS>(p, L, j0, s[mt]);
       if (!cur.full) {
         limit_scores(L, j0, s[mt]);
         if (docs) doc_scores(L, &doc_ids[wave][32 * mt + 4 * g], s[mt]);
@@ -639,7 +654,15 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
     __syncthreads();
     if (nxt.t >= 0) issue(nxt, qn, dn);
     if (!cur.mine) return;
-    st_lse[wave][lane] = cur_st[0] - (BF ? 0.f : (float)kPShift);   // fp16: P comes out times 2^kPShift
+    FarPiece far[2] = {};
+    if constexpr (TAB) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const int d_lo = key0 - (first + cur.t * kBlock + 32 * mt) - 31;
+        far[mt] = far_piece(p, tab, d_lo, d_lo + 62);
+      }
+    }
+    st_lse[wave][lane] = cur_st[0] - (BF ? 0.f : (float)kPShift) - (g ? far[1].add : far[0].add);   // fp16: P comes out times 2^kPShift
     st_del[wave][lane] = cur_st[1];
     if (docs && !cur.full) doc_ids[wave][lane] = cur_id;
     __builtin_amdgcn_wave_barrier();
@@ -665,7 +688,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
         ls = *reinterpret_cast<const floatx4*>(&st_lse[wave][32 * mt + 2 * r + 4 * g]);
         de = *reinterpret_cast<const floatx4*>(&st_del[wave][32 * mt + 2 * r + 4 * g]);
       }
-      const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], p.cc, -ls[r % 4]));
+      const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], TAB && far[mt].far ? p.c : p.cc, -ls[r % 4]));
       y[mt][r >> 3][r & 7] = to_elem<BF>(pr);
       float d = pr * (dp[mt][r] - de[r % 4]);
       if constexpr (TAB) s[mt][r] = d;
@@ -676,10 +699,12 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
       const int pos0 = first + cur.t * kBlock + 32 * mt + 4 * g;    // position of the lane's score 0; score r: + key_off(r)
       if constexpr (CAP) cap_scores_grad(p, s[mt], w[mt]);
       if constexpr (TAB) {
-        const int at = min(max(j - pos0, -p.radius), p.radius + kTabPad);   // distance j - p falls with the row
-        const float* t = tab + (at + p.radius + kTabPad);
+        if (!far[mt].far) {
+          const int at = min(max(j - pos0, -p.radius), p.radius + kTabPad);   // distance j - p falls with the row
+          const float* t = tab + (at + p.radius + kTabPad);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], p.c, t[-key_off(r)]);
+          for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_fmaf(s[mt][r], p.c, t[-key_off(r)]);
+        }
       } else if constexpr (BIAS == kBiasSlopes) {
         const float at = (float)(j - pos0);
 #pragma unroll
@@ -868,7 +893,7 @@ template <int D, bool BF>
 void launch_bwd(BwdParams& p, hipStream_t st) {
   const ScoreParams& s = p.s;
   const int nq = (s.Sq + 63) / 64, nk = (s.Sk + 63) / 64;
-  score_attn_bwd_prep_kernel<D, BF><<<dim3((unsigned)(s.B * s.Hq * nq + (BF ? 0 : s.B * s.Hkv * nk))), dim3(256), 0, st>>>(p);
+  score_attn_bwd_prep_kernel<D, BF><<<dim3((unsigned)(s.B * s.Hq * nq + (BF ? 0 : s.B * s.Hkv * nk) + (p.ranges + 3) / 4)), dim3(256), 0, st>>>(p);
   s.k1 != 0.f ? launch_bias<D, BF, true>(p, st) : launch_bias<D, BF, false>(p, st);
   if (p.splits > 1) {
     const int64_t n = (int64_t)s.B * s.Hkv * s.Sk * D;
@@ -921,7 +946,7 @@ extern "C" int stof_score_attn_bwd(const void* dout, const void* q, const void* 
   p.kv_part = (float*)(ws + l.kv);
   p.k_chunk = (B * Hkv * p.k_tiles * p.splits + 7) / 8;
   hipStream_t st = (hipStream_t)stream;
-  if (docs_q) score_attn_ranges(p.s, ws, st);
+  p.ranges = docs_q ? score_attn_ranges_at(p.s, ws) : 0;
   if (D == 64) { if (dtype == STOF_DTYPE_BF16) launch_bwd<64, true>(p, st); else launch_bwd<64, false>(p, st); }
   else { if (dtype == STOF_DTYPE_BF16) launch_bwd<128, true>(p, st); else launch_bwd<128, false>(p, st); }
   return stof_check_launch();

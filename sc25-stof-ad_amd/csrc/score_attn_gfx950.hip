@@ -22,21 +22,7 @@ namespace {
 constexpr float kLazy = 8.0f;       // log2 slack before the running maximum is raised
 
 // Document ranges of the 64-position blocks of both sequences: one wave per block.
-__global__ __launch_bounds__(64) void doc_ranges_kernel(const int* docs_q, const int* docs_k, DocRange* dr_q, DocRange* dr_k,
-                                                        int B, int Sq, int Sk) {
-  const int nq = (Sq + kBlock - 1) / kBlock, nk = (Sk + kBlock - 1) / kBlock;
-  const bool is_q = (int)blockIdx.x < B * nq;
-  const int idx = is_q ? blockIdx.x : blockIdx.x - B * nq;
-  const int n = is_q ? nq : nk, S = is_q ? Sq : Sk;
-  const int b = idx / n, blk = idx - b * n, i = blk * kBlock + threadIdx.x;
-  const bool inside = i < S;
-  const int d = inside ? (is_q ? docs_q : docs_k)[(int64_t)b * S + i] : -1;
-  int lo = d >= 0 ? d : 0x7fffffff, hi = d >= 0 ? d : -1;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64)); }
-  const int all = !__any(inside && d < 0);
-  if (threadIdx.x == 0) (is_q ? dr_q : dr_k)[idx] = DocRange{lo, hi, all, 0};
-}
+__global__ __launch_bounds__(64) void doc_ranges_kernel(const ScoreParams p) { write_doc_range(p, blockIdx.x, threadIdx.x); }
 
 // Online softmax of one wave over 16 MT scores per lane: raises the running maximum (rescaling O when it
 // moves by more than kLazy), turns scores into probabilities in the tensors' format (the B operand of the
@@ -52,13 +38,13 @@ struct Softmax {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
   }
-  __device__ __forceinline__ void step(float cc, const floatx16 (&s)[MT], half8_t (&pf)[MT][2]) {
+  __device__ __forceinline__ void step(float cc, float add, const floatx16 (&s)[MT], half8_t (&pf)[MT][2]) {   // scores times cc plus add: log2 units
     float mx = s[0][0];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mt][r]);
-    mx = pair_max(mx) * cc;
+    mx = __builtin_fmaf(pair_max(mx), cc, add);
     if (__any(mx > raise_at)) {
       const float m_new = mx > raise_at ? mx : m;
       const float m_sub = m_new == -INFINITY ? 0.f : m_new;   // a row that has seen no key: exp2(-inf) = 0 and no inf - inf
@@ -72,12 +58,13 @@ struct Softmax {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
     }
+    const float base = add - mc;
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], cc, -mc));
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], cc, base));
         sum[r & 1] += e;
         pf[mt][r >> 3][r & 7] = to_elem<BF>(e);
       }
@@ -127,7 +114,7 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
 }
 
 // ---- wide form.  Bound: vector issue beside the MFMAs.  A wave's 32 x 64 scores cost 4 D / 16 MFMAs of 32 cycles and, without
-// a rule, 107 vector instructions of 4 cycles and 32 exponentials (+ 64 for slopes, 32 and as many LDS reads for a table, 32
+// a rule, 107 vector instructions of 4 cycles and 32 exponentials (+ 64 for slopes, 32 and as many LDS reads for a table within its radius, 32
 // and 64 transcendental for a cap), and the two kinds of issue overlap by about a third.  bf16, B2 H16 S2048: D64
 // 50 us (680 TFLOP/s, MFMA busy 36 %), with a table 60, capped and causal 45; D128 73 us (940 TFLOP/s, 51 %), table
 // 80, capped and causal 58.  Tiles of 64 keys keep a 32-row wave within 170 registers at D64 (three workgroups per unit; held to
@@ -290,8 +277,17 @@ __global__ __launch_bounds__(256 * KG, 2) void score_attn_wide_kernel(const Scor
     }
     const int j0 = cur.t * kBlock + 4 * g;
     if constexpr (CAP) { cap_scores(p, s[0]); cap_scores(p, s[1]); }
-    bias_scores<BIAS>(p, L, j0, s[0]);
-    bias_scores<BIAS>(p, L, j0 + 32, s[1]);
+    float cc = p.cc, add = 0.f;
+    bool look_up = true;
+    if constexpr (BIAS == kBiasTable) {
+      const int at = cur.t * kBlock - (first + row0);
+      const FarPiece f = far_piece(p, tab, at - 31, at + kBlock - 1);
+      if (f.far) { look_up = false; cc = p.c; add = f.add; }
+    }
+    if (look_up) {
+      bias_scores<BIAS>(p, L, j0, s[0]);
+      bias_scores<BIAS>(p, L, j0 + 32, s[1]);
+    }
     if (!cur.full) {
       limit_scores(L, j0, s[0]);
       limit_scores(L, j0 + 32, s[1]);
@@ -303,7 +299,7 @@ __global__ __launch_bounds__(256 * KG, 2) void score_attn_wide_kernel(const Scor
       }
     }
     half8_t pf[2][2];
-    sm.step(p.cc, s, pf);
+    sm.step(cc, add, s, pf);
 #pragma unroll
     for (int n = NS; n < NS + NV; ++n) {
       const int m = n - NS, u = m / (D / 32), dt = m % (D / 32);
@@ -524,7 +520,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
       if (docs) doc_scores(L, &doc_ids[wave][4 * g], s[0]);
     }
     half8_t pf[1][2];
-    sm.step(p.cc, s, pf);
+    sm.step(p.cc, 0.f, s, pf);
     if (nxt.t >= 0) __builtin_amdgcn_s_waitcnt(kAllButOne);             // V has landed (the next K may be out)
     else __builtin_amdgcn_s_waitcnt(0x0F70);
     asm volatile("" ::: "memory");
@@ -741,12 +737,11 @@ void score_attn_params(ScoreParams& p, const void* q, const void* k, const void*
   p.slope_mul = kLog2e / p.c;
 }
 
-void score_attn_ranges(ScoreParams& p, void* ws, hipStream_t st) {
+int score_attn_ranges_at(ScoreParams& p, void* ws) {
   const int nq = (p.Sq + kBlock - 1) / kBlock, nk = (p.Sk + kBlock - 1) / kBlock;
-  DocRange* dq = (DocRange*)ws;
-  DocRange* dk = dq + (int64_t)p.B * nq;
-  p.dr_q = dq; p.dr_k = dk;
-  doc_ranges_kernel<<<dim3((unsigned)(p.B * (nq + nk))), dim3(64), 0, st>>>(p.docs_q, p.docs_k, dq, dk, p.B, p.Sq, p.Sk);
+  p.dr_q = (DocRange*)ws;
+  p.dr_k = p.dr_q + (int64_t)p.B * nq;
+  return p.B * (nq + nk);
 }
 
 template <int D, bool BF, bool CAP, int BIAS>
@@ -817,7 +812,7 @@ extern "C" int stof_score_attn_fwd(const void* q, const void* k, const void* v, 
   p.tiles = f.tiles; p.splits = f.splits;
   p.table_in_lds = table && tables_fit(p.group, radius);
   hipStream_t st = (hipStream_t)stream;
-  if (docs_q) score_attn_ranges(p, workspace, st);
+  if (docs_q) doc_ranges_kernel<<<dim3((unsigned)score_attn_ranges_at(p, workspace)), dim3(64), 0, st>>>(p);
   p.part = (float*)((char*)workspace + (docs_q ? ranges_bytes(B, Sq, Sk) : 0));
   if (D == 64) { if (dtype == STOF_DTYPE_BF16) launch_fwd<64, true>(p, f, st); else launch_fwd<64, false>(p, f, st); }
   else { if (dtype == STOF_DTYPE_BF16) launch_fwd<128, true>(p, f, st); else launch_fwd<128, false>(p, f, st); }

@@ -125,6 +125,18 @@ def test_table_radius(radius):
     _run(q, k, v, dout, dict(causal=True), bias=bias.to(torch.bfloat16), forms=("wide",))
 
 
+@pytest.mark.parametrize("low,high", [(0.5, -0.5), (12.0, 3.0), (-40.0, 25.0), (2800.0, 0.0), (0.0, -2800.0), (2900.0, 2900.0), (-math.inf, 1.0), (2.0, -math.inf)])
+@pytest.mark.parametrize("D,dtype,cap", [(64, "fp16", None), (64, "bf16", 20.0), (128, "bf16", None)])
+def test_distances_far_beyond_the_table(low, high, D, dtype, cap):
+    """Most pairs clip to an end of a short table: whole pieces of scores that share one entry, whatever it holds."""
+    q, k, v, dout = _qkv(1, 4, 2, 330, 270, D, DT[dtype], seed=25)
+    bias = torch.randn(4, 2 * 6 + 1, generator=_gen(26)).to(DT[dtype])
+    bias[:, 0], bias[:, -1] = low, high
+    finite = math.isfinite(low) and math.isfinite(high)
+    _run(q, k, v, dout if finite else None, dict(q_start=0), bias=bias, cap=cap, train=finite)
+    _run(q, k, v, dout if finite else None, dict(causal=True, q_start=-20), bias=bias, cap=cap, train=finite)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_table_entries_at_the_ends_of_the_format(dtype):
     """-inf closes a distance, a row whose every distance is closed gives zeros; the lowest finite value is
