@@ -26,6 +26,7 @@ __all__ = ["block_attn", "BoundAttention", "block_attn_packed_qkv", "rowwise_att
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (for callers that hold a tensor of a GPU already)
 
 
 def _stream(device=None):

@@ -16,12 +16,13 @@ import torch
 from . import _lib
 from ._lib import StofError, check
 from .fused import ACT, _DTYPES, _p, _stream
+from .ops import _current_device
 
 __all__ = ["quantize_rows_i8", "gemm_i8", "linear_i8"]
 
 
 def _call(dev, fn, what, *args):
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         rc = fn(*args)
         if rc:
             check(rc, what)

@@ -24,7 +24,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import StofError, check
-from .ops import _DTYPES, _require, _stream
+from .ops import _DTYPES, _current_device, _require, _stream
 
 __all__ = ["ScoreMask", "score_attn", "score_attn_backward", "MAX_RADIUS", "MAX_CAP"]
 
@@ -71,16 +71,18 @@ class ScoreMask:
         self.docs_q, self.docs_k = dq, dk
 
     def _check(self, B, Sq, Sk, dev):
-        def fits(name, t, *shape):
-            if t.shape != shape or t.device != dev:
-                raise StofError(f"{name} must be {list(shape)} on q's device, got {list(t.shape)} on {t.device}")
-        if self.prefix is not None:
-            fits("prefix", self.prefix, B)
         if self.kv_len is not None:
-            fits("kv_len", self.kv_len, B)
+            _fits("kv_len", self.kv_len, (B,), dev)
+        if self.prefix is not None:
+            _fits("prefix", self.prefix, (B,), dev)
         if self.docs_q is not None:
-            fits("docs", self.docs_q, B, Sq)
-            fits("docs", self.docs_k, B, Sk)
+            _fits("docs", self.docs_q, (B, Sq), dev)
+            _fits("docs", self.docs_k, (B, Sk), dev)
+
+
+def _fits(name, t, shape, dev):
+    if t.shape != shape or t.device != dev:
+        raise StofError(f"{name} must be {list(shape)} on q's device, got {list(t.shape)} on {t.device}")
 
 
 _NO_MASK = ScoreMask()
@@ -153,7 +155,8 @@ class _Rule:
             _refuse(q, k, v, mask, scale, cap, bias, slopes)
         B, Hq, Sq, D = qs
         Hkv, Sk = ks[1], ks[2]
-        mask._check(B, Sq, Sk, dev)
+        if mask is not _NO_MASK:
+            mask._check(B, Sq, Sk, dev)
         start = mask.q_start
         self.mask, self.dt, self.dev, self.sizes = mask, _DTYPES[dtype], dev, (B, Hq, Hkv, Sq, Sk, D)
         self.scale, self.cap, self.radius = scale, cap, radius
@@ -202,7 +205,7 @@ def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
             _at(mask.kv_len), _at(docs_q), _at(mask.docs_k), r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end,
             qs, ks, vs, _lib.i64x3(ostr[0], ostr[1], ostr[2]),
             *sizes, r.dt, form, _at(ws), nbytes, _stream(dev))
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         check(lib.stof_score_attn_fwd(*args), "stof_score_attn_fwd")
     else:
         with torch.cuda.device(dev):
@@ -256,7 +259,7 @@ def _backward(dout, q, k, v, out, lse, r, bias, slopes):
             dv.data_ptr(), _at(db), _at(bias), _at(slopes), _at(mask.prefix), _at(mask.kv_len), _at(mask.docs_q), _at(mask.docs_k),
             r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end, i64x3(ds[0], ds[1], ds[2]), *r.strides,
             i64x3(os_[0], os_[1], os_[2]), *sizes, r.dt, ws.data_ptr(), nbytes, _stream(dev))
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         check(lib.stof_score_attn_bwd(*args), "stof_score_attn_bwd")
     else:
         with torch.cuda.device(dev):
