@@ -66,6 +66,7 @@ struct ScoreParams {
   int radius, causal;
   int q_start, q_end;                      // p_0 = q_start, or kv_len - Sq with q_end
   int tiles, chunk, cus_per_xcd;           // workgroups per (batch, head); workgroups per XCD; compute units of an XCD
+  int uneven;                              // placement of the query kernels, see place()
   float c, k1, lse_add;                    // raw scores to log2 units: scale log2e, or 2 cap log2e; 2 scale log2e / cap (0: no cap); cap log2e or 0
   float cc, slope_mul;                     // what turns a rule's result into log2 units: c when it is in raw units, else 1 (tables); slopes to raw units
   // form for few rows
@@ -108,10 +109,22 @@ __device__ __forceinline__ float pair_sum(float x) {
 // unit that starts with a long tile gets a short one beside it; what follows goes to whichever unit is free.
 // rank counts tiles from the longest; the order is a bijection for any sizes.  Head by head, longest first, before:
 // B2 H16 S2048 causal, D128: forward 65 -> 52 us, backward 113 -> 83 (queries) and 132 -> 97 (keys).
+//
+// `uneven` work (samples of different documents or lengths; the rules stand where it is set): whole key heads would leave an XCD with
+// some of the samples only, so the query heads of every sample are dealt to all XCDs, or, where they do not divide, all
+// tiles in turn.  The latter, longest first, is also the order of causal work whose key heads do not divide (B3 H12
+// S2048 D64 causal: forward 53 -> 37 us, backward 136 -> 119).
+enum { kEven = 0, kUnevenHeads = 1, kUnevenTiles = 2 };
 struct Placed { int head, rank; };
-__device__ __forceinline__ bool place(const int index, const int heads, const int group, const int tiles, const int chunk,
-                                      const int cus_per_xcd, const int resident, const bool graded, Placed& out) {
+__device__ __forceinline__ bool place(const int index, const int heads, int group, const int tiles, const int chunk,
+                                      const int cus_per_xcd, const int resident, const bool graded, const int uneven, Placed& out) {
   const int x = index & 7, i = index >> 3;
+  if (uneven == kUnevenHeads) group = 1;
+  if (uneven == kUnevenTiles || (graded && (heads / group) % 8 != 0)) {     // (turned by one head per rank: 8 heads would else be 8 XCDs)
+    out.rank = index / heads;
+    out.head = (index - out.rank * heads + out.rank) % heads;
+    return out.rank < tiles;
+  }
   if ((heads / group) % 8 != 0) {          // key heads do not divide over the XCDs: contiguous shares, head by head
     const int id = x * chunk + i;
     out.head = id / tiles;

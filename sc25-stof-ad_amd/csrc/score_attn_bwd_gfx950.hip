@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
   Placed at;
-  if (!place(blockIdx.x, p.B * p.Hq, p.group, bp.q_tiles, bp.q_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, at)) return;
+  if (!place(blockIdx.x, p.B * p.Hq, p.group, bp.q_tiles, bp.q_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, p.uneven, at)) return;
   const int bh = at.head, tile = bp.q_tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
   const Sample sample = sample_of(p, b);
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
   Placed at;
-  if (!place(blockIdx.x, p.B * p.Hkv, 1, bp.k_tiles * bp.splits, bp.k_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, at)) return;
+  if (!place(blockIdx.x, p.B * p.Hkv, 1, bp.k_tiles * bp.splits, bp.k_chunk, p.cus_per_xcd, D == 64 ? 2 : 1, p.causal, p.uneven != kEven ? kUnevenTiles : kEven, at)) return;
   const int bk = at.head, slot = at.rank;
   const int tile = slot / bp.splits, split = slot - tile * bp.splits;   // (causal: the first keys have most queries)
   const int b = bk / p.Hkv, hk = bk - b * p.Hkv;
@@ -946,6 +946,9 @@ extern "C" int stof_score_attn_bwd(const void* dout, const void* q, const void* 
   p.kv_part = (float*)(ws + l.kv);
   p.k_chunk = (B * Hkv * p.k_tiles * p.splits + 7) / 8;
   hipStream_t st = (hipStream_t)stream;
+  // The backward kernels, one or two workgroups per unit, also gain from spreading documents of key heads that divide (mean
+  // of three: B2 H16/4 S2048 D128 138 | 133 us, B8 H12 S1024 D64 84 | 68), unless each XCD gets the same heads of every sample.
+  if (docs_q && Hkv % 8 != 0) p.s.uneven = Hq % 8 == 0 ? kUnevenHeads : kUnevenTiles;
   p.ranges = docs_q ? score_attn_ranges_at(p.s, ws) : 0;
   if (D == 64) { if (dtype == STOF_DTYPE_BF16) launch_bwd<64, true>(p, st); else launch_bwd<64, false>(p, st); }
   else { if (dtype == STOF_DTYPE_BF16) launch_bwd<128, true>(p, st); else launch_bwd<128, false>(p, st); }

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256 * KG, 2) void score_attn_wide_kernel(const Scor
   const int lane = threadIdx.x & 63, j32 = lane & 31, g = lane >> 5;
 
   Placed at;
-  if (!place(blockIdx.x, p.B * p.Hq, p.group, p.tiles, p.chunk, p.cus_per_xcd, KG == 2 ? 1 : D == 64 ? 3 : 2, p.causal, at)) return;
+  if (!place(blockIdx.x, p.B * p.Hq, p.group, p.tiles, p.chunk, p.cus_per_xcd, KG == 2 ? 1 : D == 64 ? 3 : 2, p.causal, p.uneven, at)) return;
   const int bh = at.head, tile = p.tiles - 1 - at.rank;
   const int b = bh / p.Hq, h = bh - b * p.Hq, hk = h / p.group;
 
@@ -733,6 +733,14 @@ void score_attn_params(ScoreParams& p, const void* q, const void* k, const void*
   p.lse_add = cap * kLog2e;
   int cus = stof_device_compute_units();
   p.cus_per_xcd = cus >= 8 ? cus / 8 : 32;
+  // Samples of different work, and key heads that do not divide over the XCDs or leave each of them only some of the samples
+  // (us, whole key heads | spread): lengths, B2 H16/4 S2048 D128 forward 68 | 51, backward 287 | 242, B3 H12 S2048 D64 56 | 50
+  // and 215 | 147; documents, B3 H8/4 S2048 D64 41 | 35 and 109 | 94.  Twelve key heads or more that divide reach every XCD from
+  // most samples, and keep their L2: lengths, B8 H12 S1024 27.7 | 29.7.  So do documents that divide (B2 H16/4
+  // S2048 D128, mean of three: 32 | 33).
+  const bool divides = (int64_t)B * Hkv % 8 == 0;
+  const bool uneven = divides ? kv_len && Hkv < 8 : kv_len || docs_q;
+  p.uneven = !uneven ? kEven : Hq % 8 == 0 ? kUnevenHeads : kUnevenTiles;
   p.cc = table ? 1.f : p.c;
   p.slope_mul = kLog2e / p.c;
 }

@@ -267,6 +267,14 @@ def test_causal_work_placed_over_the_xcds(B, Hq, Hkv, S, D):
     _run(q, k, v, dout, dict(kv_len=torch.randint(0, S + 1, (B,), generator=_gen(S), dtype=torch.int32)))
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,S,D", [(3, 12, 12, 300, 64), (2, 16, 4, 260, 128), (3, 8, 4, 200, 64), (5, 3, 1, 270, 64), (1, 12, 6, 520, 64), (8, 12, 12, 140, 64)])
+def test_uneven_samples_placed_over_the_xcds(B, Hq, Hkv, S, D):
+    q, k, v, dout = _qkv(B, Hq, Hkv, S, S, D, torch.bfloat16, seed=27)
+    _run(q, k, v, dout, dict(causal=True))
+    _run(q, k, v, dout, dict(causal=True, docs=_docs(B, S, 28)))
+    _run(q, k, v, dout, dict(kv_len=torch.randint(0, S + 1, (B,), generator=_gen(S + 1), dtype=torch.int32)))
+
+
 def test_gradient_of_an_expanded_scalar_and_of_broadcast_keys():
     """out.sum() hands an expanded gradient back; one key head expanded over four collects the sum of their gradients."""
     q, k, v, _ = _qkv(2, 4, 1, 50, 70, 64, torch.float16, seed=20)
