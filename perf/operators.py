@@ -234,18 +234,12 @@ def _table_gradient(ds, sq, sk):
 
 # ---- the framework's calls
 
-_modules = []
-
-
 def _package():
-    """The framework's modules, looked up once, as a program's imports are."""
-    if not _modules:
-        here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sc25-stof-ad_amd")
-        if here not in sys.path:
-            sys.path.insert(0, here)
-        from stof import quant, scores
-        _modules.extend((quant, scores))
-    return _modules
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sc25-stof-ad_amd")
+    if here not in sys.path:
+        sys.path.insert(0, here)
+    from stof import quant, scores
+    return quant, scores
 
 
 def _own(s):
