@@ -14,8 +14,9 @@
 //
 // dT enters its products in the tensors' format.  In fp16 its small values would vanish (P of long rows is
 // below 1e-4) and its large ones overflow, so it carries a power of two that is taken out of the sums
-// again: |dT| <= 2 D max|dO| max|V| =: bound, and dT 2^k with k = 14 - ceil(log2 bound) stays below 2^15 and
-// keeps 11 bits down to 2^-29 of the bound.  P is carried as 2^12 P.  bfloat16 needs neither.
+// again: |dT| <= 2 D max|dO| max|V| =: bound, with the maximum of V over all keys of the head (delta holds
+// them all), and dT 2^k with k = 14 - ceil(log2 bound) stays below 2^15 and keeps 11 bits down to 2^-29 of the
+// bound.  P is carried as 2^12 P.  bfloat16 needs neither.
 #include "score_attn.h"
 
 #include <type_traits>
@@ -520,12 +521,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(
   }
   float up = 1.f, down = bp.scale;
   if constexpr (!BF) {
-    float m = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, __builtin_fabsf((float)vf[ks][e]));
-    const int k = dt_shift<D>(wave_max_of(bp.domax + ((int64_t)b * p.Hq + hk * p.group) * nqb, p.group * nqb), pair_max(m));
+    // (the head's largest |V|, not the lane's own key's: a heavily attended key of small values has the delta of the others')
+    const int k = dt_shift<D>(wave_max_of(bp.domax + ((int64_t)b * p.Hq + hk * p.group) * nqb, p.group * nqb),
+                              wave_max_of(bp.vmax + ((int64_t)b * p.Hkv + hk) * nkb, nkb));
     up = pow2(k - kPShift);
     down = bp.scale * pow2(-k);
   }
