@@ -129,7 +129,7 @@ def _refuse(q, k, v, mask, scale, cap, bias, slopes):
 class _Rule:
     """A call's checked numbers, as the C ABI takes them; what the backward pass keeps of the forward pass."""
 
-    __slots__ = ("mask", "dt", "dev", "sizes", "scale", "cap", "radius", "q_start", "q_end", "strides")
+    __slots__ = ("mask", "elem", "dt", "dev", "sizes", "scale", "cap", "radius", "q_start", "q_end")
 
     def __init__(self, q, k, v, mask, scale, cap, bias, slopes):
         # (one pass over the conditions: this runs on every call; which of them failed is found out by _refuse)
@@ -158,12 +158,10 @@ class _Rule:
         if mask is not _NO_MASK:
             mask._check(B, Sq, Sk, dev)
         start = mask.q_start
-        self.mask, self.dt, self.dev, self.sizes = mask, _DTYPES[dtype], dev, (B, Hq, Hkv, Sq, Sk, D)
+        self.mask, self.elem, self.dt, self.dev, self.sizes = mask, dtype, _DTYPES[dtype], dev, (B, Hq, Hkv, Sq, Sk, D)
         self.scale, self.cap, self.radius = scale, cap, radius
         self.q_end = 1 if start == "end" else 0
         self.q_start = 0 if self.q_end else (Sk - Sq if start is None else start)
-        i64x3 = _lib.i64x3
-        self.strides = (i64x3(qt[0], qt[1], qt[2]), i64x3(kt[0], kt[1], kt[2]), i64x3(vt[0], vt[1], vt[2]))
 
 
 def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
@@ -200,10 +198,10 @@ def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
     docs_q = mask.docs_q
     nbytes = lib.stof_score_attn_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, docs_q is not None, form)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None   # this call's own: calls may overlap on other streams and graphs
-    qs, ks, vs = r.strides
+    i64x3, qs, ks, vs = _lib.i64x3, q.stride(), k.stride(), v.stride()
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(lse), _at(bias), _at(slopes), _at(mask.prefix),
             _at(mask.kv_len), _at(docs_q), _at(mask.docs_k), r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end,
-            qs, ks, vs, _lib.i64x3(ostr[0], ostr[1], ostr[2]),
+            i64x3(qs[0], qs[1], qs[2]), i64x3(ks[0], ks[1], ks[2]), i64x3(vs[0], vs[1], vs[2]), i64x3(ostr[0], ostr[1], ostr[2]),
             *sizes, r.dt, form, _at(ws), nbytes, _stream(dev))
     if dev.index == _current_device():
         check(lib.stof_score_attn_fwd(*args), "stof_score_attn_fwd")
@@ -249,22 +247,39 @@ def _backward(dout, q, k, v, out, lse, r, bias, slopes):
             if t is not None:
                 t.zero_()
         return dq, dk, dv, db
-    dout, out = _rows(dout), _rows(out)
+    dout, q, k, v, out = _rows(dout), _rows(q), _rows(k), _rows(v), _rows(out)
     lib = _lib.lib()
     nbytes = lib.stof_score_attn_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, r.radius, mask.docs_q is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    ds, os_ = dout.stride(), out.stride()
-    i64x3 = _lib.i64x3
+    strides3 = _lib.strides3
     args = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), _at(db), _at(bias), _at(slopes), _at(mask.prefix), _at(mask.kv_len), _at(mask.docs_q), _at(mask.docs_k),
-            r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end, i64x3(ds[0], ds[1], ds[2]), *r.strides,
-            i64x3(os_[0], os_[1], os_[2]), *sizes, r.dt, ws.data_ptr(), nbytes, _stream(dev))
+            r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end, strides3(dout), strides3(q), strides3(k), strides3(v),
+            strides3(out), *sizes, r.dt, ws.data_ptr(), nbytes, _stream(dev))
     if dev.index == _current_device():
         check(lib.stof_score_attn_bwd(*args), "stof_score_attn_bwd")
     else:
         with torch.cuda.device(dev):
             check(lib.stof_score_attn_bwd(*args), "stof_score_attn_bwd")
     return dq, dk, dv, db
+
+
+def _unpacked(saved, r, out_layout):
+    """The saved q, k, v, out, lse, bias and slopes as the backward pass takes them.  Saved-tensor hooks (activations kept on the
+    host, copies) may hand back tensors that lie in memory otherwise than those of the forward pass."""
+    B, Hq, Hkv, Sq, Sk, D = r.sizes
+    keys = (B, Hkv, Sk, D)
+    shapes = ((B, Hq, Sq, D), keys, keys, (B, Sq, Hq * D) if out_layout == "bshd" else (B, Hq, Sq, D), (B, Hq, Sq), (Hq, 2 * r.radius + 1), (Hq,))
+    kinds = (r.elem, r.elem, r.elem, r.elem, torch.float32, r.elem, torch.float32)
+    for t, shape, kind in zip(saved, shapes, kinds):
+        if t is not None and not (t.shape == shape and t.dtype == kind and t.device == r.dev):
+            raise StofError(f"a saved tensor came back as {t.dtype} {list(t.shape)} on {t.device}; saved was {kind} {list(shape)} on {r.dev}")
+    return *saved[:4], *(_flat(t) for t in saved[4:7])
+
+
+def _flat(t):
+    """t contiguous and 16-byte aligned (else a copy)."""
+    return t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(memory_format=torch.contiguous_format)
 
 
 class _ScoreAttn(Function):
@@ -284,7 +299,7 @@ class _ScoreAttn(Function):
     def backward(ctx, dout, _dlse):
         if dout is None:
             return (None,) * 8
-        q, k, v, out, lse, bias, slopes = ctx.saved_tensors[:7]
+        q, k, v, out, lse, bias, slopes = _unpacked(ctx.saved_tensors, ctx.rule, ctx.out_layout)
         if ctx.out_layout == "bshd":
             B, H, S, D = q.shape
             out, dout = (t.reshape(B, S, H, D).permute(0, 2, 1, 3) for t in (out, dout))
