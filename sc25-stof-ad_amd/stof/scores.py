@@ -127,9 +127,10 @@ def _refuse(q, k, v, mask, scale, cap, bias, slopes):
 
 
 class _Rule:
-    """A call's checked numbers, as the C ABI takes them; what the backward pass keeps of the forward pass."""
+    """A call's checked numbers, as the C ABI takes them: what the backward pass keeps of the rule beside its tensors.  (Not the
+    mask object, which may hold another rule by then.)"""
 
-    __slots__ = ("mask", "elem", "dt", "dev", "sizes", "scale", "cap", "radius", "q_start", "q_end")
+    __slots__ = ("elem", "dt", "dev", "sizes", "scale", "cap", "radius", "causal", "q_start", "q_end")
 
     def __init__(self, q, k, v, mask, scale, cap, bias, slopes):
         # (one pass over the conditions: this runs on every call; which of them failed is found out by _refuse)
@@ -158,18 +159,18 @@ class _Rule:
         if mask is not _NO_MASK:
             mask._check(B, Sq, Sk, dev)
         start = mask.q_start
-        self.mask, self.elem, self.dt, self.dev, self.sizes = mask, dtype, _DTYPES[dtype], dev, (B, Hq, Hkv, Sq, Sk, D)
-        self.scale, self.cap, self.radius = scale, cap, radius
+        self.elem, self.dt, self.dev, self.sizes = dtype, _DTYPES[dtype], dev, (B, Hq, Hkv, Sq, Sk, D)
+        self.scale, self.cap, self.radius, self.causal = scale, cap, radius, mask.causal
         self.q_end = 1 if start == "end" else 0
         self.q_start = 0 if self.q_end else (Sk - Sq if start is None else start)
 
 
-def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
+def _forward(q, k, v, r, mask, bias, slopes, out, out_layout, want_lse, launch_form):
     if launch_form not in _FORMS:
         raise StofError(f"launch form must be one of None, 'auto', 'wide', 'wide2', 'rows', got {launch_form!r}")
     form = _FORMS[launch_form]
     B, Hq, Hkv, Sq, Sk, D = sizes = r.sizes
-    dev, mask = r.dev, r.mask
+    dev = r.dev
     if out_layout == "bhsd":
         if out is None:
             out = q.new_empty((B, Hq, Sq, D))
@@ -200,7 +201,7 @@ def _forward(q, k, v, r, bias, slopes, out, out_layout, want_lse, launch_form):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None   # this call's own: calls may overlap on other streams and graphs
     i64x3, qs, ks, vs = _lib.i64x3, q.stride(), k.stride(), v.stride()
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(lse), _at(bias), _at(slopes), _at(mask.prefix),
-            _at(mask.kv_len), _at(docs_q), _at(mask.docs_k), r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end,
+            _at(mask.kv_len), _at(docs_q), _at(mask.docs_k), r.scale, r.cap, r.radius, r.causal, r.q_start, r.q_end,
             i64x3(qs[0], qs[1], qs[2]), i64x3(ks[0], ks[1], ks[2]), i64x3(vs[0], vs[1], vs[2]), i64x3(ostr[0], ostr[1], ostr[2]),
             *sizes, r.dt, form, _at(ws), nbytes, _stream(dev))
     if dev.index == _current_device():
@@ -228,18 +229,19 @@ def score_attn_backward(dout, q, k, v, out, lse, mask=None, scale=None, cap=None
     contiguous, ``dbias`` None without a table.  What autograd calls; on its own
     it is for training loops that keep their own graph of calls, a captured one among them.  ``dout`` and ``out``
     are ``[B,Hq,Sq,D]`` views; the rule must be the forward pass's."""
-    r = _Rule(q, k, v, _NO_MASK if mask is None else mask, scale, cap, bias, slopes)
+    mask = _NO_MASK if mask is None else mask
+    r = _Rule(q, k, v, mask, scale, cap, bias, slopes)
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != r.dev:
             raise StofError(f"{name} must have q's shape, dtype and device")
     if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != r.dev:
         raise StofError(f"lse must be the float32 {list(q.shape[:3])} tensor of the forward pass")
-    return _backward(dout, q, k, v, out, lse, r, bias, slopes)
+    return _backward(dout, r, q, k, v, out, lse, bias, slopes, mask.prefix, mask.kv_len, mask.docs_q, mask.docs_k)
 
 
-def _backward(dout, q, k, v, out, lse, r, bias, slopes):
+def _backward(dout, r, q, k, v, out, lse, bias, slopes, prefix, kv_len, docs_q, docs_k):
     B, Hq, Hkv, Sq, Sk, D = sizes = r.sizes
-    dev, mask = r.dev, r.mask
+    dev = r.dev
     dq, dk, dv = q.new_empty((B, Hq, Sq, D)), q.new_empty((B, Hkv, Sk, D)), q.new_empty((B, Hkv, Sk, D))
     db = torch.empty_like(bias) if bias is not None else None
     if B == 0 or Hq == 0 or Sq == 0 or Sk == 0:
@@ -249,12 +251,12 @@ def _backward(dout, q, k, v, out, lse, r, bias, slopes):
         return dq, dk, dv, db
     dout, q, k, v, out = _rows(dout), _rows(q), _rows(k), _rows(v), _rows(out)
     lib = _lib.lib()
-    nbytes = lib.stof_score_attn_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, r.radius, mask.docs_q is not None)
+    nbytes = lib.stof_score_attn_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, r.radius, docs_q is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     strides3 = _lib.strides3
     args = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), _at(db), _at(bias), _at(slopes), _at(mask.prefix), _at(mask.kv_len), _at(mask.docs_q), _at(mask.docs_k),
-            r.scale, r.cap, r.radius, mask.causal, r.q_start, r.q_end, strides3(dout), strides3(q), strides3(k), strides3(v),
+            dv.data_ptr(), _at(db), _at(bias), _at(slopes), _at(prefix), _at(kv_len), _at(docs_q), _at(docs_k),
+            r.scale, r.cap, r.radius, r.causal, r.q_start, r.q_end, strides3(dout), strides3(q), strides3(k), strides3(v),
             strides3(out), *sizes, r.dt, ws.data_ptr(), nbytes, _stream(dev))
     if dev.index == _current_device():
         check(lib.stof_score_attn_bwd(*args), "stof_score_attn_bwd")
@@ -265,16 +267,17 @@ def _backward(dout, q, k, v, out, lse, r, bias, slopes):
 
 
 def _unpacked(saved, r, out_layout):
-    """The saved q, k, v, out, lse, bias and slopes as the backward pass takes them.  Saved-tensor hooks (activations kept on the
+    """The saved tensors (``_ScoreAttn.forward``) as the backward pass takes them.  Saved-tensor hooks (activations kept on the
     host, copies) may hand back tensors that lie in memory otherwise than those of the forward pass."""
     B, Hq, Hkv, Sq, Sk, D = r.sizes
     keys = (B, Hkv, Sk, D)
-    shapes = ((B, Hq, Sq, D), keys, keys, (B, Sq, Hq * D) if out_layout == "bshd" else (B, Hq, Sq, D), (B, Hq, Sq), (Hq, 2 * r.radius + 1), (Hq,))
-    kinds = (r.elem, r.elem, r.elem, r.elem, torch.float32, r.elem, torch.float32)
+    shapes = ((B, Hq, Sq, D), keys, keys, (B, Sq, Hq * D) if out_layout == "bshd" else (B, Hq, Sq, D), (B, Hq, Sq), (Hq, 2 * r.radius + 1), (Hq,),
+              (B,), (B,), (B, Sq), (B, Sk))
+    kinds = (r.elem, r.elem, r.elem, r.elem, torch.float32, r.elem, torch.float32, torch.int32, torch.int32, torch.int32, torch.int32)
     for t, shape, kind in zip(saved, shapes, kinds):
         if t is not None and not (t.shape == shape and t.dtype == kind and t.device == r.dev):
             raise StofError(f"a saved tensor came back as {t.dtype} {list(t.shape)} on {t.device}; saved was {kind} {list(shape)} on {r.dev}")
-    return *saved[:4], *(_flat(t) for t in saved[4:7])
+    return *saved[:4], *(_flat(t) for t in saved[4:])
 
 
 def _flat(t):
@@ -284,10 +287,10 @@ def _flat(t):
 
 class _ScoreAttn(Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, slopes, rule, out_layout, launch_form):
-        out, lse = _forward(q, k, v, rule, bias, slopes, None, out_layout, True, launch_form)
-        mask = rule.mask
-        # the rule's tensors are saved too, so that one changed in place before the backward pass is noticed
+    def forward(ctx, q, k, v, bias, slopes, rule, mask, out_layout, launch_form):
+        out, lse = _forward(q, k, v, rule, mask, bias, slopes, None, out_layout, True, launch_form)
+        # the rule's tensors are saved too: one changed in place before the backward pass is noticed, a mask object that
+        # was given others by then changes nothing
         ctx.save_for_backward(q, k, v, out, lse, bias, slopes, mask.prefix, mask.kv_len, mask.docs_q, mask.docs_k)
         ctx.rule, ctx.out_layout = rule, out_layout
         ctx.mark_non_differentiable(lse)
@@ -298,15 +301,15 @@ class _ScoreAttn(Function):
     @once_differentiable
     def backward(ctx, dout, _dlse):
         if dout is None:
-            return (None,) * 8
-        q, k, v, out, lse, bias, slopes = _unpacked(ctx.saved_tensors, ctx.rule, ctx.out_layout)
+            return (None,) * 9
+        q, k, v, out, *rest = _unpacked(ctx.saved_tensors, ctx.rule, ctx.out_layout)
         if ctx.out_layout == "bshd":
             B, H, S, D = q.shape
             out, dout = (t.reshape(B, S, H, D).permute(0, 2, 1, 3) for t in (out, dout))
         need = ctx.needs_input_grad
-        dq, dk, dv, db = _backward(dout, q, k, v, out, lse, ctx.rule, bias, slopes)
+        dq, dk, dv, db = _backward(dout, ctx.rule, q, k, v, out, *rest)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, db if need[3] else None,
-                None, None, None, None)
+                None, None, None, None, None)
 
 
 def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None, out=None, out_layout="bhsd",
@@ -320,11 +323,12 @@ def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None,
     output, not through lse).  ``launch_form``: None, "wide" (128-query tiles), "wide2" (those with the keys
     in two parts; small grids) or "rows" (32-row tiles with the keys split; single tokens and smaller grids) - the rule by
     sizes is in the library."""
-    r = _Rule(q, k, v, _NO_MASK if mask is None else mask, scale, cap, bias, slopes)
+    mask = _NO_MASK if mask is None else mask
+    r = _Rule(q, k, v, mask, scale, cap, bias, slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         if out is not None:
             raise StofError("out= has no gradient: leave it out, or call under torch.no_grad()")
-        o, lse = _ScoreAttn.apply(q, k, v, bias, slopes, r, out_layout, launch_form)
+        o, lse = _ScoreAttn.apply(q, k, v, bias, slopes, r, mask, out_layout, launch_form)
     else:
-        o, lse = _forward(q, k, v, r, bias, slopes, out, out_layout, return_lse, launch_form)
+        o, lse = _forward(q, k, v, r, mask, bias, slopes, out, out_layout, return_lse, launch_form)
     return (o, lse) if return_lse else o

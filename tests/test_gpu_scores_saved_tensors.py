@@ -55,3 +55,20 @@ def test_expanded_keys_and_slopes(how):
         out = score_attn(lq, kx, vx, slopes=slopes.cuda())
     for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (lq, kx, vx), dout.cuda())):
         _within(got, want[name], name)
+
+
+def test_rule_of_the_forward_pass_when_the_mask_object_changes():
+    """A mask object that is given other tensors or another causality between the passes: the gradients are of the rule that ran."""
+    g = torch.Generator().manual_seed(5)
+    n = lambda: torch.randn(2, 2, 90, 64, generator=g).half()
+    q, k, v, dout = n(), n(), n(), n()
+    docs = (torch.arange(90, dtype=torch.int32) // 20).expand(2, 90).contiguous()
+    rule = dict(causal=True, kv_len=torch.tensor([90, 60], dtype=torch.int32), prefix=torch.tensor([0, 30], dtype=torch.int32), docs=docs)
+    want = os_.score_attn(q, k, v, dout=dout, **rule)
+    m = ScoreMask(causal=True, kv_len=rule["kv_len"].cuda(), prefix=rule["prefix"].cuda(), docs=docs.cuda())
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out = score_attn(*leaves, m)
+    m.causal, m.prefix, m.kv_len = 0, None, torch.tensor([3, 90], dtype=torch.int32, device="cuda")
+    m.docs_q = m.docs_k = torch.zeros(2, 90, dtype=torch.int32, device="cuda")
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout.cuda())):
+        _within(got, want[name], name)

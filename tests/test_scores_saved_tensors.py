@@ -120,3 +120,37 @@ def test_tensors_of_another_kind_are_refused(library, change, which):
     with pytest.raises(StofError, match="saved"):
         out.backward(torch.zeros_like(out))
     assert library.bwd is None
+
+
+def test_rule_tensors_that_come_back_strided(library):
+    i32 = lambda *s: _gpu(torch.arange(1, 1 + torch.Size(s).numel(), dtype=torch.int32).view(*s))
+    mask = ScoreMask(causal=True, prefix=i32(2), kv_len=i32(2), docs=i32(2, 100))
+    library.read = {PREFIX: (ctypes.c_int32, 2), KV_LEN: (ctypes.c_int32, 2), DOCS_Q: (ctypes.c_int32, 200), DOCS_K: (ctypes.c_int32, 200)}
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _every_second):
+        out = score_attn(*_packed(), mask)
+    out.backward(torch.zeros_like(out))
+    for at, (_, n) in library.read.items():
+        assert library.values[at] == list(range(1, n + 1)), at
+
+
+@pytest.mark.parametrize("change", ["type", "shape", "device"])
+def test_rule_tensors_of_another_kind_are_refused(library, change):
+    change = {"type": lambda t: t.long(), "shape": lambda t: t[..., :1], "device": lambda t: t.to("meta")}[change]
+    mask = ScoreMask(kv_len=_gpu(torch.zeros(2, dtype=torch.int32)))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.dtype == torch.int32 else t):
+        out = score_attn(*_packed(), mask)
+    with pytest.raises(StofError, match="saved"):
+        out.backward(torch.zeros_like(out))
+    assert library.bwd is None
+
+
+def test_a_mask_object_changed_between_the_passes(library):
+    """The backward pass takes the rule of the forward pass, whatever the object holds by then."""
+    i32 = lambda *s: _gpu(torch.arange(1, 1 + torch.Size(s).numel(), dtype=torch.int32).view(*s))
+    mask = ScoreMask(causal=True, prefix=i32(2), kv_len=i32(2), docs=i32(2, 100))
+    was = {PREFIX: mask.prefix.data_ptr(), KV_LEN: mask.kv_len.data_ptr(), DOCS_Q: mask.docs_q.data_ptr(), DOCS_K: mask.docs_k.data_ptr(), CAUSAL: 1}
+    out = score_attn(*_packed(), mask)
+    keep = [mask.prefix, mask.kv_len, mask.docs_q]
+    mask.causal, mask.prefix, mask.kv_len, mask.docs_q, mask.docs_k = 0, None, i32(1), i32(2, 3), None
+    out.backward(torch.zeros_like(out))
+    assert {at: library.bwd[at] for at in was} == was and len(keep) == 3
