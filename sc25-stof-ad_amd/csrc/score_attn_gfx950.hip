@@ -687,6 +687,7 @@ inline Form pick_form(int B, int Hq, int Hkv, int Sq, int Sk, int form) {
   const int64_t most = ((Sk + kRowKeys - 1) / kRowKeys + 2 * kRowWaves - 1) / (2 * kRowWaves);   // two tiles per wave
   if (splits > most) splits = most;
   if (splits > 64) splits = 64;                                            // one lane each in the join
+  if (splits < 1) splits = 1;                                              // no keys: the outputs are still written
   return Form{true, 1, (int)tiles, (int)splits};
 }
 
