@@ -81,8 +81,9 @@ class ScoreMask:
 
 
 def _fits(name, t, shape, dev):
-    if t.shape != shape or t.device != dev:
-        raise StofError(f"{name} must be {list(shape)} on q's device, got {list(t.shape)} on {t.device}")
+    # (type and layout again: a mask object may have been given another tensor since it was made)
+    if t.shape != shape or t.device != dev or t.dtype != torch.int32 or not t.is_contiguous():
+        raise StofError(f"{name} must be a contiguous int32 {list(shape)} tensor on q's device, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 _NO_MASK = ScoreMask()

@@ -154,3 +154,17 @@ def test_a_mask_object_changed_between_the_passes(library):
     mask.causal, mask.prefix, mask.kv_len, mask.docs_q, mask.docs_k = 0, None, i32(1), i32(2, 3), None
     out.backward(torch.zeros_like(out))
     assert {at: library.bwd[at] for at in was} == was and len(keep) == 3
+
+
+def test_tensors_given_to_a_mask_object_later_are_checked(library):
+    """Another type is read as other numbers, an expanded tensor past its end: both refused, as by the constructor."""
+    q, k, v = (t.detach() for t in _packed())
+    i32 = lambda *s: _gpu(torch.zeros(*s, dtype=torch.int32))
+    for name, good, bad in (("kv_len", i32(2), i32(1).expand(2)), ("kv_len", i32(2), i32(2).long()), ("prefix", i32(2), i32(4)[::2]),
+                            ("docs_q", i32(2, 100), i32(2, 1).expand(2, 100)), ("docs_k", i32(2, 100), i32(2, 100).short())):
+        mask = ScoreMask(causal=True, kv_len=i32(2), prefix=i32(2), docs=i32(2, 100))
+        setattr(mask, name, good)
+        score_attn(q, k, v, mask)
+        setattr(mask, name, bad)
+        with pytest.raises(StofError):
+            score_attn(q, k, v, mask)
