@@ -45,6 +45,18 @@ def _require(cond, msg):
         raise StofError(msg)
 
 
+_forward_ad = torch.autograd.forward_ad
+
+
+def _refuse_tangents(*tensors):
+    """Raise if one of the tensors (or None) carries a forward-mode tangent, which the result would not have."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:       # outside of every dual_level
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise StofError("an argument carries a forward-mode tangent: this operator has no forward-mode derivative")
+
+
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}   # STOF_DTYPE_*
 _LAUNCH_FORMS = {None: -1, "default": -1, "auto": -1, "two_rows": 0, "key_split": 1, "pipelined": 2}
 

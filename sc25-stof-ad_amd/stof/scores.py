@@ -24,7 +24,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import StofError, check
-from .ops import _DTYPES, _current_device, _require, _stream
+from .ops import _DTYPES, _current_device, _refuse_tangents, _require, _stream
 
 __all__ = ["ScoreMask", "score_attn", "score_attn_backward", "MAX_RADIUS", "MAX_CAP"]
 
@@ -232,6 +232,7 @@ def score_attn_backward(dout, q, k, v, out, lse, mask=None, scale=None, cap=None
     are ``[B,Hq,Sq,D]`` views; the rule must be the forward pass's."""
     mask = _NO_MASK if mask is None else mask
     r = _Rule(q, k, v, mask, scale, cap, bias, slopes)
+    _refuse_tangents(dout, q, k, v, out, lse, bias, slopes)
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != r.dev:
             raise StofError(f"{name} must have q's shape, dtype and device")
@@ -326,6 +327,7 @@ def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None,
     sizes is in the library."""
     mask = _NO_MASK if mask is None else mask
     r = _Rule(q, k, v, mask, scale, cap, bias, slopes)
+    _refuse_tangents(q, k, v, bias, slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         if out is not None:
             raise StofError("out= has no gradient: leave it out, or call under torch.no_grad()")
