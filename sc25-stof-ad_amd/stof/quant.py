@@ -35,10 +35,14 @@ def _elems(name, t):
     dt = _DTYPES.get(t.dtype) if t.is_cuda else None
     if dt is None:
         raise StofError(f"{name} must be a CUDA float16 or bfloat16 tensor")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise StofError(f"{name} requires a gradient: the 8-bit operators have none (call them under torch.no_grad())")
+    _no_gradient(name, t)
     _refuse_tangents(t)
     return dt
+
+
+def _no_gradient(name, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise StofError(f"{name} requires a gradient: the 8-bit operators have none (call them under torch.no_grad())")
 
 
 def _rows2d(name, t, align):
@@ -84,6 +88,9 @@ def _weights(wq, w_scale, bias, K, dev, dtype, act):
         raise StofError(f"w_scale must be a contiguous float32 [{N}] tensor on x's device")
     if bias is not None and not (bias.dtype == dtype and bias.shape == (N,) and bias.is_contiguous() and bias.device == dev):
         raise StofError(f"bias must be a contiguous [{N}] tensor of the output's dtype on x's device")
+    _no_gradient("w_scale", w_scale)
+    if bias is not None:
+        _no_gradient("bias", bias)
     _refuse_tangents(w_scale, bias)
     if act not in ACT:
         raise StofError(f"act must be one of {sorted(ACT)}, got {act!r}")
@@ -111,6 +118,7 @@ def gemm_i8(xq, x_scale, wq, w_scale, bias=None, act="none", dtype=torch.float16
     M = x2.shape[0]
     if not (x_scale.dtype == torch.float32 and x_scale.shape == xq.shape[:-1] and x_scale.device == xq.device):
         raise StofError(f"x_scale must be a float32 {list(xq.shape[:-1])} tensor on xq's device")
+    _no_gradient("x_scale", x_scale)
     _refuse_tangents(x_scale)
     x_scale = x_scale.contiguous()
     y = _output(out, xq.shape[:-1] + (N,), dtype, xq.device)

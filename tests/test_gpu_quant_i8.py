@@ -260,3 +260,17 @@ def test_refusals():
         with pytest.raises(StofError):
             call()
             pytest.fail(f"refusal {n} was accepted")
+
+
+def test_parameters_that_ask_for_a_gradient():
+    h = lambda *s, d=torch.float16: torch.zeros(*s, dtype=d, device="cuda")
+    x, w, s, b = h(4, 64), h(16, 64, d=torch.int8), h(16, d=torch.float32), h(16)
+    ask = lambda t: t.clone().requires_grad_()
+    calls = [lambda: linear_i8(x, w, s, ask(b)), lambda: linear_i8(x, w, ask(s), b), lambda: gemm_i8(w[:4], s[:4], w, s, ask(b)),
+             lambda: gemm_i8(w[:4], s[:4], w, ask(s), b), lambda: gemm_i8(w[:4], ask(s[:4]), w, s)]
+    for n, call in enumerate(calls):
+        with pytest.raises(StofError, match="gradient"):
+            call()
+            pytest.fail(f"call {n} was accepted")
+        with torch.no_grad():
+            call()
