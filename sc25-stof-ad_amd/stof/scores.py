@@ -123,7 +123,7 @@ def _refuse(q, k, v, mask, scale, cap, bias, slopes):
     if slopes is not None:
         if not (slopes.shape == (Hq,) and slopes.dtype == torch.float32 and slopes.is_contiguous() and slopes.device == dev):
             raise StofError(f"slopes must be a contiguous float32 [{Hq}] tensor on q's device")
-        raise StofError("slopes are constants of the rule: there is no gradient for them")
+        raise StofError("slopes are constants of the rule: there is no gradient for them (detach them, or call under torch.no_grad())")
     raise StofError("these tensors cannot be used together")
 
 
@@ -152,7 +152,7 @@ class _Rule:
             radius = n[-1] // 2
         elif ok and slopes is not None:
             ok = (slopes.shape == qs[1:2] and slopes.dtype == torch.float32 and slopes.is_contiguous() and slopes.device == dev
-                  and not slopes.requires_grad)
+                  and not (slopes.requires_grad and torch.is_grad_enabled()))
         if not ok:
             _refuse(q, k, v, mask, scale, cap, bias, slopes)
         B, Hq, Sq, D = qs

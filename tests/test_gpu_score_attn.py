@@ -534,3 +534,13 @@ def test_refusals():
         with pytest.raises(StofError):
             call()
             pytest.fail(f"refusal {n} was accepted")
+
+
+def test_slopes_kept_as_a_parameter():
+    """Refused where a gradient would be asked for, taken under no_grad."""
+    x = torch.randn(1, 4, 20, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    slopes = torch.nn.Parameter(torch.rand(4, generator=torch.Generator().manual_seed(2)).cuda())
+    with pytest.raises(StofError, match="gradient"):
+        score_attn(x, x, x, slopes=slopes)
+    with torch.no_grad():
+        assert torch.equal(score_attn(x, x, x, slopes=slopes), score_attn(x, x, x, slopes=slopes.detach()))
