@@ -54,7 +54,7 @@ def _rows2d(name, t, align):
         t = t.reshape(-1, K)
     s = t.stride(0) if t.shape[0] > 1 else K
     if t.stride(1) != 1 or s % align or s < K or t.data_ptr() % 16:
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)     # (contiguous() returns rows at an odd address as they are)
         s = K
     return t, s
 

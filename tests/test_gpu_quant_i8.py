@@ -274,3 +274,20 @@ def test_parameters_that_ask_for_a_gradient():
             pytest.fail(f"call {n} was accepted")
         with torch.no_grad():
             call()
+
+
+def test_contiguous_rows_at_an_odd_address():
+    """A view at an odd offset of a flat buffer is contiguous and cannot be read as it lies: a copy, as for odd strides."""
+    x = torch.randn(4, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    w, ws = quantize_rows_i8(torch.randn(16, 64, generator=torch.Generator().manual_seed(4)).half().cuda())
+    flat = torch.empty(4 * 64 + 1, dtype=torch.float16, device="cuda")
+    odd = flat[1:].view(4, 64)
+    odd.copy_(x)
+    q, s = quantize_rows_i8(x)
+    q2, s2 = quantize_rows_i8(odd)
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+    assert torch.equal(linear_i8(odd, w, ws), linear_i8(x, w, ws)) and torch.equal(linear_i8(odd[:1], w, ws), linear_i8(x[:1], w, ws))
+    flat8 = torch.empty(4 * 64 + 8, dtype=torch.int8, device="cuda")
+    odd8 = flat8[8:].view(4, 64)
+    odd8.copy_(q)
+    assert torch.equal(gemm_i8(odd8, s, w, ws), gemm_i8(q, s, w, ws))
