@@ -218,11 +218,12 @@ def _at(t):
 
 
 def _rows(t):
-    """t as the kernels read it: unit stride in D, other strides multiples of 8, 16-byte aligned (else a copy)."""
+    """t as the kernels read it: unit stride in D, other strides multiples of 8, rows at most 2^23 apart, 16-byte aligned (else a
+    copy; ``contiguous()`` would return a contiguous tensor at an odd address as it is)."""
     s = t.stride()
-    if s[3] == 1 and not (s[0] % 8 or s[1] % 8 or s[2] % 8 or t.data_ptr() % 16):
+    if s[3] == 1 and not (s[0] % 8 or s[1] % 8 or s[2] % 8 or s[2] > 1 << 23 or t.data_ptr() % 16):
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def score_attn_backward(dout, q, k, v, out, lse, mask=None, scale=None, cap=None, bias=None, slopes=None):

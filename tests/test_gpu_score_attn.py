@@ -544,3 +544,16 @@ def test_slopes_kept_as_a_parameter():
         score_attn(x, x, x, slopes=slopes)
     with torch.no_grad():
         assert torch.equal(score_attn(x, x, x, slopes=slopes), score_attn(x, x, x, slopes=slopes.detach()))
+
+
+@pytest.mark.parametrize("layout", ["bhsd", "bshd"])
+def test_gradient_that_arrives_at_an_odd_address(layout):
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(2, 3, 70, 64, generator=g).half().cuda().requires_grad_() for _ in range(3))
+    out = score_attn(q, k, v, ScoreMask(causal=True), out_layout=layout)
+    flat = torch.randn(out.numel() + 1, generator=g).half().cuda()
+    odd = flat[1:].view(out.shape)
+    assert odd.is_contiguous() and odd.data_ptr() % 16
+    want = torch.autograd.grad(out, (q, k, v), odd.clone(), retain_graph=True)
+    got = torch.autograd.grad(out, (q, k, v), odd)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -168,3 +168,13 @@ def test_tensors_given_to_a_mask_object_later_are_checked(library):
         setattr(mask, name, bad)
         with pytest.raises(StofError):
             score_attn(q, k, v, mask)
+
+
+def test_gradients_the_kernels_cannot_read_as_they_lie_are_copied(library):
+    """Rows more than 2^23 elements apart, an odd address, an odd stride."""
+    q, k, v = (_gpu(torch.zeros(1, 2, 3, 64, dtype=torch.float16)).requires_grad_() for _ in range(3))
+    out = score_attn(q, k, v)
+    base = torch.zeros(2 * (1 << 23) + 4096, dtype=torch.float16)
+    for dout in (base.as_strided((1, 2, 3, 64), (64, 64, (1 << 23) + 8, 1)), base[1:385].view(1, 2, 3, 64), base.as_strided((1, 2, 3, 64), (400, 200, 65, 1))):
+        torch.autograd.grad(out, (q, k, v), _gpu(dout), retain_graph=True)
+        assert library.bwd[STRIDES[DOUT]] == (384, 192, 64) and library.bwd[DOUT] % 16 == 0
