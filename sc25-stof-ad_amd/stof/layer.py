@@ -27,7 +27,7 @@ import torch
 
 from . import fused
 from ._lib import StofError
-from .ops import block_attn, block_attn_packed_qkv
+from .ops import block_attn_packed_qkv
 from .quant import linear_i8, quantize_rows_i8
 from .scores import ScoreMask, score_attn
 
@@ -153,17 +153,12 @@ class EncoderLayer:
         can be timed on its own (the reference's layer has no QKV projection,
         src/benchmk_end2end.py:37: its figure is the sum without "qkv_gemm")."""
         qkv = self._linear(x, self.Wqkv, self.bqkv)
-        q, k, v = self._split_heads(qkv)
-        if isinstance(lut, ScoreMask):
-            attention = lambda: score_attn(q, k, v, lut, out_layout="bshd", **self.scores)
-        else:
-            attention = lambda: block_attn(q, k, v, lut, block, block, out_layout="bshd")
-        attn = attention()
+        attn = self._attn(qkv, lut, block)
         h = self._gemm_ln(attn, self.Wo, self.bo, x, self.g1, self.be1)
         f = self._linear(h, self.W1, self.b1, self.act)
         return [
             ("qkv_gemm", lambda: self._linear(x, self.Wqkv, self.bqkv)),
-            ("attention", attention),
+            ("attention", lambda: self._attn(qkv, lut, block)),
             ("out_proj_ln", lambda: self._gemm_ln(attn, self.Wo, self.bo, x, self.g1, self.be1)),
             ("ffn1_gelu", lambda: self._linear(h, self.W1, self.b1, self.act)),
             ("ffn2_ln", lambda: self._gemm_ln(f, self.W2, self.b2, h, self.g2, self.be2)),

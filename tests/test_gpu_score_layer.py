@@ -113,3 +113,19 @@ def test_end_to_end_command_with_table_and_int8():
            "--linear", "int8", "--warmup_iters", "1", "--running_iters", "1"]
     r = subprocess.run(cmd, capture_output=True, text=True, timeout=110)
     assert r.returncode == 0 and "STOF" in r.stdout and "max abs difference" in r.stdout, r.stdout + r.stderr
+
+
+def test_stages_run_the_layer_s_own_attention():
+    """A layer with a score rule refuses a LUT in ``stages`` as in ``forward``, and its stages give what ``forward`` gives."""
+    w, x = _weights(), _x(1, 64)
+    lut = pm.get_sparse_storage(torch.ones(1, 64, 64).cuda(), 64, 64)[1:]
+    layer = EncoderLayer(w, H, scores=dict(cap=3.0))
+    for call in (lambda: layer(x, lut), lambda: layer.stages(x, lut)):
+        with pytest.raises(StofError, match="ScoreMask"):
+            call()
+    m = ScoreMask(causal=True)
+    stages = dict(layer.stages(x, m))
+    assert torch.equal(stages["attention"](), layer._attn(stages["qkv_gemm"](), m, 64)) and torch.equal(stages["ffn2_ln"](), layer(x, m))
+    plain = EncoderLayer(w, H)
+    stages = dict(plain.stages(x, lut))
+    assert torch.equal(stages["attention"](), plain._attn(stages["qkv_gemm"](), lut, 64)) and torch.equal(stages["ffn2_ln"](), plain(x, lut))
