@@ -469,9 +469,10 @@ int stof_score_attn_bwd(const void* dout, const void* q, const void* k, const vo
  * wq [N, K] int8 (rows ldw apart) with fp32 scales sw [N], bias [N] and out [M, N] in x's format.  A row of zeros has
  * scale 0; a row that is not finite has scale NaN.  K a multiple of 16 up to 131056 (sums stay in int32 for any
  * bytes), N a multiple of 8, ldx and ldo multiples of 8, ldw and ldq multiples of 16; pointers 16-byte aligned (sx: 4).
- * stof_linear_i8 quantises and multiplies: one launch up to 16 tokens (workspace 0 bytes), else two through the
- * workspace, which needs no initial contents.  stof_gemm_i8_bias_act takes rows already quantised, for
- * several products on one x.
+ * stof_linear_i8 quantises and multiplies: one launch (workspace 0 bytes) for up to 16 tokens whose quantised rows, each
+ * K rounded up to 64 and 16 bytes more, fit 64 KB together (16 tokens up to K = 4032, one up to 65472), else two launches
+ * through the workspace, which needs no initial contents: always ask stof_linear_i8_workspace_bytes.
+ * stof_gemm_i8_bias_act takes rows already quantised, for several products on one x.
  */
 int stof_quantize_rows_i8(const void* x, int8_t* xq, float* sx, int64_t M, int64_t K, int64_t ldx, int64_t ldq, int dtype, void* stream);
 int stof_gemm_i8_bias_act(const int8_t* xq, const float* sx, const int8_t* wq, const float* sw, const void* bias, void* out,

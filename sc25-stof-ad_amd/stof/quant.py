@@ -131,8 +131,8 @@ def gemm_i8(xq, x_scale, wq, w_scale, bias=None, act="none", dtype=torch.float16
 
 def linear_i8(x, wq, w_scale, bias=None, act="none", out=None):
     """``act(x @ (wq * w_scale)^T + bias)`` with x quantised per token: x ``[..., K]`` fp16 or bfloat16, wq int8 ``[N, K]``
-    with scales fp32 ``[N]`` (``quantize_rows_i8``), bias ``[N]`` of x's dtype.  One launch up to 16 tokens, else two.
-    ``out`` must not overlap the inputs."""
+    with scales fp32 ``[N]`` (``quantize_rows_i8``), bias ``[N]`` of x's dtype.  One launch up to 16 tokens
+    whose quantised rows fit 64 KB of LDS (16 of them up to K = 4032), else two.  ``out`` must not overlap the inputs."""
     dt = _elems("x", x)
     K = x.shape[-1] if x.dim() else 0
     N, ldw = _weights(wq, w_scale, bias, K, x.device, x.dtype, act)

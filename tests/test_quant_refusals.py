@@ -40,3 +40,13 @@ def test_argument_checks(lib):
     assert ln(x=None) == -1 and ln(ws=None) == -1 and ln(ws=P + 4) == -4 and ln(n=40 * 64) == -2 and ln(ldx=68) == -4 and ln(ldx=56) == -2
     assert lib.stof_linear_i8_workspace_bytes(1, 64) == 0 and lib.stof_linear_i8_workspace_bytes(40, 64) == 40 * 64 + 160
     assert lib.stof_linear_i8_workspace_bytes(16, 8192) > 0        # the rows do not fit into a workgroup's LDS
+
+
+def test_where_the_one_launch_form_ends(lib):
+    """Up to 16 tokens whose quantised rows (K rounded up to 64, and 16 bytes) fit 64 KB; beyond, a workspace is asked for."""
+    need = lib.stof_linear_i8_workspace_bytes
+    for M, last in ((1, 65472), (2, 32704), (15, 4352), (16, 4032)):
+        assert M * (last + 16) <= 65536 < M * (last + 64 + 16)
+        assert need(M, last) == 0 and need(M, last + 16) == M * (last + 16) + (4 * M + 15) // 16 * 16
+    assert need(17, 16) == 17 * 16 + 80
+    assert lib.stof_linear_i8(P, P, P, None, P, 16, 16, 4096, 4096, 4096, 16, 0, 0, None, 0, None) == -1
