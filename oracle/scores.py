@@ -77,7 +77,7 @@ def score_attn(q, k, v, scale=None, cap=None, bias=None, slopes=None, dout=None,
     lse = (torch.log(tot) + torch.where(top == -math.inf, 0.0, top))[..., 0]
     eP = 2 * torch.where(ok, err, 0.0).amax(-1, keepdim=True) + 2.0 ** -20 if Sk else torch.zeros(B, Hq, Sq, 1)
     out = P @ V
-    floor = 2.0 ** -25 if q.dtype == torch.float16 else 0.0      # half the smallest fp16 number, by which a small P may be off
+    floor = 2.0 ** -32 if q.dtype == torch.float16 else 0.0      # P times 2^7 by half the smallest fp16 number: what a small P may be off
     res = {"out": (out, ((u + eP) * P + floor * ok) @ V.abs() + u * out.abs() + tiny),
            "lse": (lse, eP[..., 0] + 2.0 ** -21 * lse.abs().nan_to_num(posinf=0.0))}
     if dout is None:

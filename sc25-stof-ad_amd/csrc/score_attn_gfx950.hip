@@ -20,6 +20,10 @@
 namespace {
 
 constexpr float kLazy = 8.0f;       // log2 slack before the running maximum is raised
+// fp16: P is carried times 2^7, in its product and in the running sum alike.  With the slack it stays below 2^15, and a P is off
+// by at most 2^-32 of the maximum's: held plainly, what lies below 2^-25 of it vanished from the product and stayed in the
+// sum (65536 keys at 2^-25.2 of one other: outputs of 0 for 1.6e-3).  bfloat16 has the exponents of fp32.
+template <bool BF> constexpr float kPUp = BF ? 0.f : 7.f;
 
 // Document ranges of the 64-position blocks of both sequences: one wave per block.
 __global__ __launch_bounds__(64) void doc_ranges_kernel(const ScoreParams p) { write_doc_range(p, blockIdx.x, threadIdx.x); }
@@ -58,7 +62,7 @@ struct Softmax {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
     }
-    const float base = add - mc;
+    const float base = (add - mc) + kPUp<BF>;
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -358,7 +362,7 @@ __global__ __launch_bounds__(256 * KG, 2) void score_attn_wide_kernel(const Scor
   if (rows <= 0) return;
   const float l = pair_sum(sm.l);
   const float inv = l == 0.f ? 0.f : 1.f / l;              // no allowed key at all: zeros
-  if (p.lse && g == 0 && i < p.Sq) p.lse[(int64_t)bh * p.Sq + i] = l == 0.f ? -INFINITY : (sm.m + __builtin_amdgcn_logf(l) + p.lse_add) * kLn2;
+  if (p.lse && g == 0 && i < p.Sq) p.lse[(int64_t)bh * p.Sq + i] = l == 0.f ? -INFINITY : (sm.m + (__builtin_amdgcn_logf(l) - kPUp<BF>) + p.lse_add) * kLn2;
   stage_rows<D, BF>(sm.o, inv, stage, j32, g);
   half_t* ob = p.out + b * p.os[0] + h * p.os[1] + (int64_t)row0 * p.os[2];
   const __amdgpu_buffer_rsrc_t o_rsrc = stof_wave_rsrc(ob);
@@ -600,7 +604,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 1) void score_attn_rows_kernel(cons
     for (int e = 0; e < 4; ++e) o4[e] = to_elem<BF>(part[x + e] * inv);
     *reinterpret_cast<half4_t*>(orow + col) = o4;
   }
-  if (p.lse && wave == 0 && g == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l) + p.lse_add) * kLn2;
+  if (p.lse && wave == 0 && g == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + (__builtin_amdgcn_logf(l) - kPUp<BF>) + p.lse_add) * kLn2;
 }
 
 // Joins the splits of the row form: one workgroup per row, every fourth split to a wave, D / 64 columns per lane; the
@@ -647,7 +651,7 @@ __global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams 
     const int c = kC * lane + x;
     orow[c] = to_elem<BF>(((sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c])) * inv);
   }
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l) + p.lse_add) * kLn2;
+  if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = l == 0.f ? -INFINITY : (m + (__builtin_amdgcn_logf(l) - kPUp<BF>) + p.lse_add) * kLn2;
 }
 
 }  // namespace
