@@ -277,15 +277,15 @@ def _unpacked(saved, r, out_layout):
     shapes = ((B, Hq, Sq, D), keys, keys, (B, Sq, Hq * D) if out_layout == "bshd" else (B, Hq, Sq, D), (B, Hq, Sq), (Hq, 2 * r.radius + 1), (Hq,),
               (B,), (B,), (B, Sq), (B, Sk))
     kinds = (r.elem, r.elem, r.elem, r.elem, torch.float32, r.elem, torch.float32, torch.int32, torch.int32, torch.int32, torch.int32)
+    dev, tensors = r.dev, []
     for t, shape, kind in zip(saved, shapes, kinds):
-        if t is not None and not (t.shape == shape and t.dtype == kind and t.device == r.dev):
-            raise StofError(f"a saved tensor came back as {t.dtype} {list(t.shape)} on {t.device}; saved was {kind} {list(shape)} on {r.dev}")
-    return *saved[:4], *(_flat(t) for t in saved[4:])
-
-
-def _flat(t):
-    """t contiguous and 16-byte aligned (else a copy)."""
-    return t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(memory_format=torch.contiguous_format)
+        if t is not None:
+            if t.shape != shape or t.dtype is not kind or t.device != dev:
+                raise StofError(f"a saved tensor came back as {t.dtype} {list(t.shape)} on {t.device}; saved was {kind} {list(shape)} on {dev}")
+            if len(shape) < 4 and (t.data_ptr() % 16 or not t.is_contiguous()):        # ([B,H,S,D] views: _backward reads their strides)
+                t = t.clone(memory_format=torch.contiguous_format)
+        tensors.append(t)
+    return tensors
 
 
 class _ScoreAttn(Function):
