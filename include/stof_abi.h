@@ -449,7 +449,7 @@ int stof_score_attn_fwd(const void* q, const void* k, const void* v, void* out, 
                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
- * Its gradients, from the forward pass's out and lse: dq [B, Hq, Sq, D], dk and dv [B, Hkv, Sk, D] contiguous, dtable
+ * Its gradients (Sk >= 1), from the forward pass's out and lse: dq [B, Hq, Sq, D], dk and dv [B, Hkv, Sk, D] contiguous, dtable
  * [Hq, 2 radius + 1] in the tensors' format.  No atomics: the same inputs give the same bits.  The rule's tensors must hold what they held in the forward pass.
  */
 int64_t stof_score_attn_bwd_workspace_bytes(int B, int Hq, int Hkv, int Sq, int Sk, int D, int radius, int docs);

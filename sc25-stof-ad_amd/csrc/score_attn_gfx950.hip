@@ -117,9 +117,11 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
     }
 }
 
-// ---- wide form.  Bound: vector issue beside the MFMAs.  A wave's 32 x 64 scores cost 4 D / 16 MFMAs of 32 cycles and, without
-// a rule, 107 vector instructions of 4 cycles and 32 exponentials (+ 64 for slopes, 32 and as many LDS reads for a table within its radius, 32
-// and 64 transcendental for a cap), and the two kinds of issue overlap by about a third.  bf16, B2 H16 S2048: D64
+// ---- wide form.  Bound: the present order of vector issue and MFMAs.  A wave's 32 x 64 scores cost 4 D / 16 MFMAs of 32 cycles and,
+// without a rule, 107 vector instructions of 4 cycles and 32 exponentials (+ 64 for slopes, 32 and as many LDS reads for a table within its
+// radius, 32 and 64 transcendental for a cap).  A wave does them one after the other - all score MFMAs, the rule and the exponentials, all
+// MFMAs of the second product - so that the two kinds of issue overlap only where another wave of the SIMD is in the other kind: by
+// about a third.  That is this schedule's figure and no limit of the machine.  bf16, B2 H16 S2048: D64
 // 50 us (680 TFLOP/s, MFMA busy 36 %), with a table 60, capped and causal 45; D128 73 us (940 TFLOP/s, 51 %), table
 // 80, capped and causal 58.  Tiles of 64 keys keep a 32-row wave within 170 registers at D64 (three workgroups per unit; held to
 // four it spilled: B8 H12 S1024 with a table 41 -> 50 us) and 232 at D128 (two).
@@ -666,11 +668,13 @@ __global__ __launch_bounds__(256) void score_attn_join_kernel(const ScoreParams 
 //  * The wide form walks the keys in two parts while every workgroup can have a compute unit to itself: 256
 //    workgroups, B2 H8 S2048, one part | two: 31.8 | 28.3, causal 29.9 | 25.2, D128 causal 42.1 | 35.0; 384, B8 H12 S512
 //    13.9 | 17.9, B3 H8 S2048 44.7 | 50.2.
+//    (256 units, as every MI355X has: the workspace's size is asked for without a device.)
 //  * Splitting costs a launch (3 us) and the partial results.  Past 2048 keys the row form's splits give every unit a workgroup:
 //    64 workgroups over 4096 keys 20.6 unsplit, 13.8 with four splits, 18.8 with six, over 16384 keys 64.8 | 25.2 | 35.3;
 //    but 2048 keys 12.1 | 13.6 | 16.3.  Single tokens of many heads are bound by memory and gain from splits only what
 //    evens out caches of different length: 128 workgroups, equal | uneven lengths, D128 over 16384 keys 203 | 179 unsplit, 186 | 129
-//    with four splits, 190 | 130 with eight, over 4096 keys 41 | 32 unsplit, 47 | 34 with four.
+//    with four splits, 190 | 130 with eight, over 4096 keys 41 | 32 unsplit, 47 | 34 with four.  These figures are of 64 and of 128
+//    workgroups; single tokens of 65 to 127 workgroups follow the rule of 128 without a measurement of their own.
 namespace {
 
 struct Form { bool rows; int parts, tiles, splits; };

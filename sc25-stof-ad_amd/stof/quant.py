@@ -10,7 +10,8 @@ counterpart of ``fused.gemm_bias_act``.
 
 A row's scale is its largest magnitude / 127; values are ``round(127 x / max)``, ties to even, from the exact
 quotient.  Rows of zeros have scale 0; a row with an infinity or NaN has scale NaN, so its outputs are NaN.
-For inference: there is no gradient, and tensors that ask for one are refused."""
+For inference: there is no gradient, and tensors that ask for one (x, scales, bias) or carry a forward-mode tangent are
+refused; under ``torch.no_grad()`` parameters are taken."""
 import torch
 
 from . import _lib

@@ -46,6 +46,8 @@ class ScoreMask:
 
     The tensors are read by the launches, not here: a serving loop keeps one object and writes new lengths
     into ``kv_len``.  Contents are not checked (that would synchronise); lengths are clamped to [0, Sk].
+    A backward pass uses the rule and the tensors of its forward pass: attributes assigned in between change nothing, a
+    tensor written to in between is an error.
     Keys past ``kv_len``, keys that causality closes to every query of the sample and keys without a document are
     never used as values, whatever they hold (the free part of a cache).  A non-finite key or value that SOME
     query of a sample may attend to can reach other rows of its 64 x 64 tile, as it does in a dense product."""
@@ -89,7 +91,7 @@ def _fits(name, t, shape, dev):
 _NO_MASK = ScoreMask()
 
 
-def _refuse(q, k, v, mask, scale, cap, bias, slopes):
+def _refuse(q, k, v, scale, cap, bias, slopes):
     """The refusal of a call that ``_rule`` found wanting, by name."""
     if not q.is_cuda:
         raise StofError("q must be a CUDA tensor (this path has no CPU implementation)")
@@ -154,7 +156,7 @@ class _Rule:
             ok = (slopes.shape == qs[1:2] and slopes.dtype == torch.float32 and slopes.is_contiguous() and slopes.device == dev
                   and not (slopes.requires_grad and torch.is_grad_enabled()))
         if not ok:
-            _refuse(q, k, v, mask, scale, cap, bias, slopes)
+            _refuse(q, k, v, scale, cap, bias, slopes)
         B, Hq, Sq, D = qs
         Hkv, Sk = ks[1], ks[2]
         if mask is not _NO_MASK:
@@ -320,10 +322,11 @@ def score_attn(q, k, v, mask=None, scale=None, cap=None, bias=None, slopes=None,
     """Attention with a score rule (module docstring).  ``q`` ``[B,Hq,Sq,D]``, ``k`` and ``v`` ``[B,Hkv,Sk,D]``:
     fp16 or, all alike, bfloat16, head size 64 or 128, any lengths, unit stride in D and other strides
     multiples of 8.  ``mask``: a ``ScoreMask`` (None: every key).  ``scale``: default ``1/sqrt(D)``.
-    ``bias``: learned distance table ``[Hq, 2R+1]`` of q's dtype, R up to 1024; ``slopes``: fp32 ``[Hq]``, constants.
+    ``bias``: learned distance table ``[Hq, 2R+1]`` of q's dtype, R up to 1024; ``slopes``: fp32 ``[Hq]``, constants
+    (a parameter is taken under ``torch.no_grad()`` only).
     ``out`` must not overlap the inputs.  Returns ``[B,Hq,Sq,D]`` (``out_layout="bhsd"``) or ``[B,Sq,Hq*D]`` (``"bshd"``), with ``return_lse`` also the
     logarithm of the softmax's denominator, fp32 ``[B,Hq,Sq]``.  Differentiable in q, k, v and bias (through the
-    output, not through lse).  ``launch_form``: None, "wide" (128-query tiles), "wide2" (those with the keys
+    output, not through lse; reverse mode only: forward-mode tangents are refused).  ``launch_form``: None, "wide" (128-query tiles), "wide2" (those with the keys
     in two parts; small grids) or "rows" (32-row tiles with the keys split; single tokens and smaller grids) - the rule by
     sizes is in the library."""
     mask = _NO_MASK if mask is None else mask
