@@ -36,14 +36,15 @@ def _elems(name, t):
     dt = _DTYPES.get(t.dtype) if t.is_cuda else None
     if dt is None:
         raise StofError(f"{name} must be a CUDA float16 or bfloat16 tensor")
-    _no_gradient(name, t)
-    _refuse_tangents(t)
     return dt
 
 
-def _no_gradient(name, t):
-    if t.requires_grad and torch.is_grad_enabled():
-        raise StofError(f"{name} requires a gradient: the 8-bit operators have none (call them under torch.no_grad())")
+def _no_gradient(**tensors):
+    """Refuses tensors (or None) that ask for a gradient or carry a forward-mode tangent."""
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise StofError(f"{name} requires a gradient: the 8-bit operators have none (call them under torch.no_grad())")
+    _refuse_tangents(*tensors.values())
 
 
 def _rows2d(name, t, align):
@@ -63,6 +64,7 @@ def _rows2d(name, t, align):
 def quantize_rows_i8(x):
     """``x`` ``[..., K]`` (fp16 or bfloat16, K a multiple of 16) -> int8 ``[..., K]`` and its scales, fp32 ``[...]``."""
     dt = _elems("x", x)
+    _no_gradient(x=x)
     K = x.shape[-1] if x.dim() else 0
     if K % 16 or K == 0 or K > 131056:
         raise StofError(f"K must be a multiple of 16 up to 131056, got {K}")
@@ -89,10 +91,6 @@ def _weights(wq, w_scale, bias, K, dev, dtype, act):
         raise StofError(f"w_scale must be a contiguous float32 [{N}] tensor on x's device")
     if bias is not None and not (bias.dtype == dtype and bias.shape == (N,) and bias.is_contiguous() and bias.device == dev):
         raise StofError(f"bias must be a contiguous [{N}] tensor of the output's dtype on x's device")
-    _no_gradient("w_scale", w_scale)
-    if bias is not None:
-        _no_gradient("bias", bias)
-    _refuse_tangents(w_scale, bias)
     if act not in ACT:
         raise StofError(f"act must be one of {sorted(ACT)}, got {act!r}")
     return N, ldw
@@ -119,8 +117,7 @@ def gemm_i8(xq, x_scale, wq, w_scale, bias=None, act="none", dtype=torch.float16
     M = x2.shape[0]
     if not (x_scale.dtype == torch.float32 and x_scale.shape == xq.shape[:-1] and x_scale.device == xq.device):
         raise StofError(f"x_scale must be a float32 {list(xq.shape[:-1])} tensor on xq's device")
-    _no_gradient("x_scale", x_scale)
-    _refuse_tangents(x_scale)
+    _no_gradient(x_scale=x_scale, w_scale=w_scale, bias=bias)
     x_scale = x_scale.contiguous()
     y = _output(out, xq.shape[:-1] + (N,), dtype, xq.device)
     if M:
@@ -137,6 +134,7 @@ def linear_i8(x, wq, w_scale, bias=None, act="none", out=None):
     dt = _elems("x", x)
     K = x.shape[-1] if x.dim() else 0
     N, ldw = _weights(wq, w_scale, bias, K, x.device, x.dtype, act)
+    _no_gradient(x=x, w_scale=w_scale, bias=bias)
     x2, ldx = _rows2d("x", x, 8)
     M = x2.shape[0]
     shape = (M, N) if x.dim() == 2 else x.shape[:-1] + (N,)

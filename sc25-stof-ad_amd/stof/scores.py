@@ -220,12 +220,13 @@ def _at(t):
 
 
 def _rows(t):
-    """t as the kernels read it: unit stride in D, other strides multiples of 8, rows at most 2^23 apart, 16-byte aligned (else a
-    copy; ``contiguous()`` would return a contiguous tensor at an odd address as it is)."""
+    """t as the kernels read it and its strides: unit stride in D, other strides multiples of 8, rows at most 2^23 apart, 16-byte
+    aligned (else a copy; ``contiguous()`` would return a contiguous tensor at an odd address as it is)."""
     s = t.stride()
-    if s[3] == 1 and not (s[0] % 8 or s[1] % 8 or s[2] % 8 or s[2] > 1 << 23 or t.data_ptr() % 16):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or s[2] > 1 << 23 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = t.stride()
+    return t, _lib.i64x3(s[0], s[1], s[2])
 
 
 def score_attn_backward(dout, q, k, v, out, lse, mask=None, scale=None, cap=None, bias=None, slopes=None):
@@ -254,15 +255,13 @@ def _backward(dout, r, q, k, v, out, lse, bias, slopes, prefix, kv_len, docs_q, 
             if t is not None:
                 t.zero_()
         return dq, dk, dv, db
-    dout, q, k, v, out = _rows(dout), _rows(q), _rows(k), _rows(v), _rows(out)
+    (dout, ds), (q, qs), (k, ks), (v, vs), (out, os_) = _rows(dout), _rows(q), _rows(k), _rows(v), _rows(out)
     lib = _lib.lib()
     nbytes = lib.stof_score_attn_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, r.radius, docs_q is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    strides3 = _lib.strides3
     args = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), _at(db), _at(bias), _at(slopes), _at(prefix), _at(kv_len), _at(docs_q), _at(docs_k),
-            r.scale, r.cap, r.radius, r.causal, r.q_start, r.q_end, strides3(dout), strides3(q), strides3(k), strides3(v),
-            strides3(out), *sizes, r.dt, ws.data_ptr(), nbytes, _stream(dev))
+            r.scale, r.cap, r.radius, r.causal, r.q_start, r.q_end, ds, qs, ks, vs, os_, *sizes, r.dt, ws.data_ptr(), nbytes, _stream(dev))
     if dev.index == _current_device():
         check(lib.stof_score_attn_bwd(*args), "stof_score_attn_bwd")
     else:
