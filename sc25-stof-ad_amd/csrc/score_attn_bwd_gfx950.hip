@@ -194,8 +194,8 @@ __device__ __forceinline__ void store_rows(const floatx16 (&o)[D / 32], float mu
 //     dQ = scale (dT(delta) K - (delta' - delta) M)
 // is exact in delta while the second term stays small.  delta' replaces delta for the kernel of the keys.
 //
-// Bound: MFMA and vector issue, 4 products of 2 D FLOP a pair.  bf16, B2 H16 S2048: D64 75 us (914 TFLOP/s, MFMA busy 51 %), D128
-// 140 us (984 TFLOP/s, 51 %; one workgroup of four waves per unit, whose accumulators take 380 registers).
+// Bound: MFMA and vector issue, 4 products of 2 D FLOP a pair.  bf16, B2 H16 S2048: D64 80 us (860 TFLOP/s, MFMA busy 51 %), D128
+// 133 us (1030 TFLOP/s, 50 %; one workgroup of four waves per unit, whose accumulators take 380 registers).
 template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_q_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(1024) void score_attn_bwd_table_kernel(const BwdPar
 // workspace, which a last kernel adds up over batch and key tiles.
 //
 // Bound: LDS reads beside MFMA and vector issue (both operands of the sums' products are transposed on the way; 1.8 to 2.1 reads
-// per MFMA).  bf16, B2 H16 S2048: D64 93 us (740 TFLOP/s, MFMA busy 43 %), with a table 115; D128 166 us (828 TFLOP/s, 41 %), table 206.
+// per MFMA).  bf16, B2 H16 S2048: D64 90 us (760 TFLOP/s, MFMA busy 43 %), with a table 112; D128 157 us (875 TFLOP/s, 41 %), table 190.
 template <int D, bool BF, bool CAP, int BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void score_attn_bwd_k_kernel(const BwdParams bp) {
   const ScoreParams& p = bp.s;

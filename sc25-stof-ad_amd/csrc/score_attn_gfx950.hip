@@ -122,8 +122,8 @@ __device__ __forceinline__ void stage_rows(const floatx16 (&o)[D / 32], float in
 // radius, 32 and 64 transcendental for a cap).  A wave does them one after the other - all score MFMAs, the rule and the exponentials, all
 // MFMAs of the second product - so that the two kinds of issue overlap only where another wave of the SIMD is in the other kind: by
 // about a third.  That is this schedule's figure and no limit of the machine.  bf16, B2 H16 S2048: D64
-// 50 us (680 TFLOP/s, MFMA busy 36 %), with a table 60, capped and causal 45; D128 73 us (940 TFLOP/s, 51 %), table
-// 80, capped and causal 58.  Tiles of 64 keys keep a 32-row wave within 170 registers at D64 (three workgroups per unit; held to
+// 50 us (685 TFLOP/s, MFMA busy 35 %), with a table 57, capped and causal 45; D128 70 us (980 TFLOP/s, 51 %), table
+// 73, capped and causal 56.  Tiles of 64 keys keep a 32-row wave within 170 registers at D64 (three workgroups per unit; held to
 // four it spilled: B8 H12 S1024 with a table 41 -> 50 us) and 232 at D128 (two).
 //
 // CAP is a template argument: with the cap behind a run-time branch the compiler computes it speculatively for every
