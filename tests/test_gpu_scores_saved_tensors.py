@@ -1,6 +1,7 @@
 """Gradients of attention with score rules whose saved tensors pass through hooks, against the float64 oracle."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from oracle import scores as os_
 from stof.scores import ScoreMask, score_attn
@@ -72,3 +73,23 @@ def test_rule_of_the_forward_pass_when_the_mask_object_changes():
     m.docs_q = m.docs_k = torch.zeros(2, 90, dtype=torch.int32, device="cuda")
     for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout.cuda())):
         _within(got, want[name], name)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_step_has_the_gradients_of_a_plain_one(reentrant):
+    """Activations formed again in the backward pass: the same bits."""
+    B, H, S, D = 2, 4, 130, 64
+    g = torch.Generator().manual_seed(43)
+    packed = torch.randn(B, S, 3 * H * D, generator=g).half().cuda().requires_grad_()
+    tab = torch.randn(H, 21, generator=g).half().cuda().requires_grad_()
+    dout = torch.randn(B, S, H * D, generator=g).half().cuda()
+    m = ScoreMask(causal=True, kv_len=torch.tensor([130, 70], dtype=torch.int32, device="cuda"))
+
+    def step(x, t):
+        return score_attn(*(x[..., n * H * D:(n + 1) * H * D].view(B, S, H, D).permute(0, 2, 1, 3) for n in range(3)), m, bias=t, out_layout="bshd")
+
+    step(packed, tab).backward(dout)
+    want = packed.grad.clone(), tab.grad.clone()
+    packed.grad = tab.grad = None
+    torch.utils.checkpoint.checkpoint(step, packed, tab, use_reentrant=reentrant).backward(dout)
+    assert torch.equal(packed.grad, want[0]) and torch.equal(tab.grad, want[1])
